@@ -263,6 +263,235 @@ def attention_decoder(q16, k16, v16, items: int, q_heads: int, kv_heads: int, kp
     return out
 
 
+# ------------------------------------------------------------------ generation operators
+def _heads(name, x, dtype=None, device=None):
+    """A packed tensor [rows, heads, 128] whose rows may be strided (a view of a wider projection); returns
+    its row stride."""
+    if x.dim() != 3 or x.shape[2] != 128 or x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != 128):
+        raise ValueError(f"{name}: a tensor [rows, heads, 128] with dense rows is wanted")
+    if (dtype is not None and x.dtype != dtype) or (device is not None and x.device != device) or not x.is_cuda:
+        raise ValueError(f"{name}: type or device differs from the other tensors'")
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * 128
+
+
+def _array(name, x, dtype, shape, device):
+    """A dense device tensor of one type and shape; None passes."""
+    if x is not None and (x.dtype != dtype or tuple(x.shape) != tuple(shape) or not x.is_contiguous() or
+                          x.device != device):
+        raise ValueError(f"{name}: a dense {dtype} tensor {list(shape)} on {device} is wanted")
+    return x.data_ptr() if x is not None else None
+
+
+def _raw_stream(device):
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _code(dtype, name):
+    import torch
+    if dtype == torch.bfloat16:
+        return 2
+    if dtype == torch.float16:
+        return 1
+    raise ValueError(f"{name}: float16 or bfloat16 is wanted")
+
+
+def gated_delta(q, k, v, g, beta, items: int = 1, cu_seqlens=None, max_len: int | None = None, state=None,
+                scale: float | None = None, norm_eps: float | None = 1e-6, state_out=None, out=None):
+    """The gated delta rule over packed sequences -> (out [rows, v_heads, 128], states after the last rows
+    f32 [items, v_heads, 128 (value), 128 (key)]).
+
+    q, k [rows, k_heads, 128], v [rows, v_heads, 128] (f16 or bf16; rows may be views of one wider
+    projection), g (log decay) and beta f32 [rows, v_heads].  Without cu_seqlens (int32 [items + 1] on the
+    device) the items are equal; with it max_len is the longest item's rows (default: all rows, which
+    is only slower).  state: f32 [items, v_heads, 128, 128], or with one item in front a kept state that
+    every item starts from; None: zeros.  state_out may be state itself.  q and k are divided by their
+    lengths unless norm_eps is None; scale defaults to 128^-0.5."""
+    import torch
+    dev, dt = v.device, v.dtype
+    code = _code(dt, "gated_delta")
+    ldq, ldk, ldv = _heads("q", q, dt, dev), _heads("k", k, dt, dev), _heads("v", v, dt, dev)
+    rows, hv, hk = v.shape[0], v.shape[1], k.shape[1]
+    if q.shape != k.shape or k.shape[0] != rows:
+        raise ValueError("gated_delta: q, k and v differ in their rows or heads")
+    for name, x in (("g", g), ("beta", beta)):
+        if x.shape != (rows, hv) or x.dtype != torch.float32 or x.stride(1) != 1 and hv > 1 or x.device != dev:
+            raise ValueError(f"{name}: a float32 tensor [rows, v_heads] with dense rows is wanted")
+    if cu_seqlens is not None:
+        _array("cu_seqlens", cu_seqlens, torch.int32, (items + 1,), dev)
+        max_len = rows if max_len is None else min(max_len, rows)
+    else:
+        if items and rows % items:
+            raise ValueError("gated_delta: rows do not divide into equal items")
+        max_len = rows // items if items else 0
+    stride = 0
+    if state is not None:
+        one = state.shape[0] == 1
+        _array("state", state, torch.float32, (1 if one else items, hv, 128, 128), dev)
+        stride = 0 if one and items != 1 else hv * 128 * 128
+    if state_out is None:
+        state_out = torch.empty((items, hv, 128, 128), dtype=torch.float32, device=dev)
+    so = _array("state_out", state_out, torch.float32, (items, hv, 128, 128), dev)
+    if out is None:
+        out = torch.empty((rows, hv, 128), dtype=dt, device=dev)
+    ldo = _heads("out", out, dt, dev)
+    if out.shape != (rows, hv, 128):
+        raise ValueError("gated_delta: out differs from v in its shape")
+    lib = load()
+    need = lib.db_gated_delta_workspace_bytes(items, rows, max_len, hk, hv)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.db_gated_delta(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ldq, ldk, ldv, g.data_ptr(),
+                             beta.data_ptr(), g.stride(0) if rows > 1 else hv, beta.stride(0) if rows > 1 else hv,
+                             cu_seqlens.data_ptr() if cu_seqlens is not None else None, items, rows, max_len, hk, hv,
+                             128, 128 ** -0.5 if scale is None else scale, -1.0 if norm_eps is None else norm_eps,
+                             state.data_ptr() if state is not None else None, stride, so, out.data_ptr(), ldo,
+                             ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
+    return out, state_out
+
+
+class KvCache8:
+    """The tensors of an 8-bit paged key/value cache (db_kv8_cache): int8 codes of full blocks of 64 tokens
+    with one f32 scale per block, kv head and keys / values, and the open blocks in 16 bits.
+
+    k_codes [pages, kv_heads, 64, 128], v_codes [pages, kv_heads, 128, 64] int8; k_scales, v_scales f32
+    [pages, kv_heads]; k_tail [sequences, kv_heads, 64, 128], v_tail [sequences, kv_heads, 128, 64] f16 or
+    bf16; page_table int32 [sequences, table_width]: the page of each block, the caller's to fill."""
+
+    BLOCK = 64
+
+    def __init__(self, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, page_table):
+        import torch
+        dev = k_tail.device
+        pages, heads = k_scales.shape
+        sequences, width = page_table.shape
+        code = _code(k_tail.dtype, "KvCache8")
+        self._c = _lib.KvCache8(
+            _array("k_codes", k_codes, torch.int8, (pages, heads, 64, 128), dev),
+            _array("k_scales", k_scales, torch.float32, (pages, heads), dev),
+            _array("v_codes", v_codes, torch.int8, (pages, heads, 128, 64), dev),
+            _array("v_scales", v_scales, torch.float32, (pages, heads), dev),
+            _array("k_tail", k_tail, k_tail.dtype, (sequences, heads, 64, 128), dev),
+            _array("v_tail", v_tail, k_tail.dtype, (sequences, heads, 128, 64), dev),
+            _array("page_table", page_table, torch.int32, (sequences, width), dev),
+            pages, width, sequences, heads, 128, code)
+        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
+        self.k_tail, self.v_tail, self.page_table = k_tail, v_tail, page_table
+        self.ref = C.byref(self._c)
+
+    @classmethod
+    def allocate(cls, sequences: int, pages: int, table_width: int, kv_heads: int, dtype, device="cuda") -> "KvCache8":
+        """An empty cache; block i of sequence b is page b * table_width + i where the pool is large
+        enough for that, else the table is left at -1 (no page) for the caller to fill."""
+        import torch
+        dev = torch.device(device)
+        dev = torch.device("cuda", torch.cuda.current_device()) if dev.index is None else dev
+        table = torch.full((sequences, table_width), -1, dtype=torch.int32, device=dev)
+        if pages >= sequences * table_width:
+            table = torch.arange(sequences * table_width, dtype=torch.int32, device=dev).view(sequences, table_width)
+        z = lambda dt, *shape: torch.zeros(shape, dtype=dt, device=dev)  # noqa: E731
+        return cls(z(torch.int8, pages, kv_heads, 64, 128), z(torch.float32, pages, kv_heads),
+                   z(torch.int8, pages, kv_heads, 128, 64), z(torch.float32, pages, kv_heads),
+                   z(dtype, sequences, kv_heads, 64, 128), z(dtype, sequences, kv_heads, 128, 64), table)
+
+
+def _kv8_rows(cache, x, lengths, cu_seqlens, max_rows):
+    import torch
+    dev, rows, items = cache.k_tail.device, x.shape[0], lengths.shape[0]
+    _array("lengths", lengths, torch.int32, (items,), dev)
+    if cu_seqlens is not None:
+        _array("cu_seqlens", cu_seqlens, torch.int32, (items + 1,), dev)
+        return items, rows, rows if max_rows is None else min(max_rows, rows), cu_seqlens.data_ptr()
+    if items and rows % items:
+        raise ValueError("kv8: rows do not divide into equal items")
+    return items, rows, rows // items if items else 0, None
+
+
+def kv8_append(cache: KvCache8, k, v, lengths, cu_seqlens=None, max_rows: int | None = None) -> None:
+    """Writes the items' new rows (k, v [rows, kv_heads, 128]) at positions lengths[b] (int32, device) on;
+    blocks that fill up are quantised.  The lengths stay as they are: advance them once every layer has
+    taken the step.  cu_seqlens and max_rows as in gated_delta."""
+    dt, dev = cache.k_tail.dtype, cache.k_tail.device
+    ldk, ldv = _heads("k", k, dt, dev), _heads("v", v, dt, dev)
+    if k.shape != v.shape or k.shape[1] != cache.k_tail.shape[1]:
+        raise ValueError("kv8_append: k or v differs from the cache in its heads or rows")
+    items, rows, most, cu = _kv8_rows(cache, k, lengths, cu_seqlens, max_rows)
+    check(load().db_kv8_append(cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, lengths.data_ptr(), cu, items, rows,
+                               most, _raw_stream(dev)))
+
+
+def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | None = None, max_keys: int = 0,
+                  scale: float | None = None, out=None):
+    """Attention over the cache after the append of the same rows: row i of item b sees the cached keys
+    0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: an upper bound on the longest item's keys, if
+    the caller knows one below the table's width (it only sizes the launch)."""
+    import torch
+    dt, dev = cache.k_tail.dtype, cache.k_tail.device
+    ldq = _heads("q", q, dt, dev)
+    items, rows, most, cu = _kv8_rows(cache, q, lengths, cu_seqlens, max_rows)
+    if out is None:
+        out = torch.empty(q.shape, dtype=dt, device=dev)
+    ldo = _heads("out", out, dt, dev)
+    if out.shape != q.shape:
+        raise ValueError("kv8_attention: out differs from q in its shape")
+    check(load().db_kv8_attention(cache.ref, q.data_ptr(), ldq, lengths.data_ptr(), cu, items, rows, most, max_keys,
+                                  q.shape[1], 128 ** -0.5 if scale is None else scale, out.data_ptr(), ldo,
+                                  _raw_stream(dev)))
+    return out
+
+
+def kv8_read(cache: KvCache8, lengths, max_keys: int):
+    """The cached keys and values of tokens 0 .. max_keys - 1, f32 [items, max_keys, kv_heads, 128] each
+    (0 from lengths[b] on)."""
+    import torch
+    dev, items = cache.k_tail.device, lengths.shape[0]
+    _array("lengths", lengths, torch.int32, (items,), dev)
+    k, v = (torch.empty((items, max_keys, cache.k_tail.shape[1], 128), dtype=torch.float32, device=dev)
+            for _ in range(2))
+    check(load().db_kv8_read(cache.ref, lengths.data_ptr(), items, max_keys, k.data_ptr(), v.data_ptr(),
+                             _raw_stream(dev)))
+    return k, v
+
+
+def logit_rules(logits, history=None, history_lengths=None, repetition=None, presence=None, frequency=None,
+                bias_ids=None, bias_values=None, mask=None, out=None):
+    """Penalties for repeated tokens, biases and a grammar mask on logits [rows, vocab] -> (values f32
+    [rows, vocab], best token int32 [rows], log-sum-exp f32 [rows]); values - lse are log-probabilities.
+
+    history int32 [rows, n] with history_lengths int32 [rows] (None: all n); repetition, presence and
+    frequency f32 [rows]; bias_ids int32 and bias_values f32 [rows, m]; mask int32 [rows, ceil(vocab / 32)],
+    bit id % 32 of word id / 32 set where a token is allowed.  A row with nothing allowed has best -1
+    and lse -inf.  out may be f32 logits themselves."""
+    import torch
+    rows, vocab = logits.shape
+    dev = logits.device
+    if vocab > 1 and logits.stride(1) != 1 or not logits.is_cuda:
+        raise ValueError("logit_rules: logits with dense rows on a device are wanted")
+    if str(logits.dtype).split(".")[1] not in DTYPES:
+        raise ValueError("logit_rules: logits are float32, float16 or bfloat16")
+    f32, i32 = torch.float32, torch.int32
+    cols = history.shape[1] if history is not None else 0
+    hist = _array("history", history, i32, (rows, cols), dev)
+    lens = _array("history_lengths", history_lengths, i32, (rows,), dev)
+    pen = [_array(n, x, f32, (rows,), dev)
+           for n, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency))]
+    biases = bias_ids.shape[1] if bias_ids is not None else 0
+    ids = _array("bias_ids", bias_ids, i32, (rows, biases), dev)
+    vals = _array("bias_values", bias_values, f32, (rows, biases), dev)
+    words = (vocab + 31) // 32
+    bits = _array("mask", mask, i32, (rows, words), dev)
+    if out is None:
+        out = torch.empty((rows, vocab), dtype=f32, device=dev)
+    elif out.shape != logits.shape or out.dtype != f32 or vocab > 1 and out.stride(1) != 1 or out.device != dev:
+        raise ValueError("logit_rules: out is f32 with dense rows, of the logits' shape")
+    best = torch.empty(rows, dtype=i32, device=dev)
+    lse = torch.empty(rows, dtype=f32, device=dev)
+    check(load().db_logit_rules(logits.data_ptr(), DTYPES[str(logits.dtype).split(".")[1]],
+                                logits.stride(0) if rows > 1 else vocab, rows, vocab, hist, cols, lens, cols, *pen, ids,
+                                vals, biases, bits, words, out.data_ptr(), out.stride(0) if rows > 1 else vocab,
+                                best.data_ptr(), lse.data_ptr(), _raw_stream(dev)))
+    return out, best, lse
+
+
 def synthetic_bf16(seed: int, tensor: int, shape, std: float, device="cuda"):
     import torch
     out = torch.empty(shape, dtype=torch.int16, device=device)

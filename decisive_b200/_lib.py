@@ -36,6 +36,13 @@ class Parameters(C.Structure):
     _fields_ = [("max_sequence_tokens", C.c_int32)]
 
 
+class KvCache8(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+                ("k_tail", C.c_void_p), ("v_tail", C.c_void_p), ("page_table", C.c_void_p), ("pages", C.c_int32),
+                ("table_width", C.c_int32), ("sequences", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
 _u16pp = C.POINTER(C.POINTER(C.c_uint16))
 _fpp = C.POINTER(C.POINTER(C.c_float))
 
@@ -82,6 +89,14 @@ SIGNATURES = [
     ("db_attention", _i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _f, _vp, _i64, _vp]),
     ("db_attention_decoder", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, C.c_int, _i64, _i64, _i64, _f, _vp,
                                     _i64, _vp]),
+    ("db_gated_delta_workspace_bytes", _sz, [_i64] * 5),
+    ("db_gated_delta", _i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
+                              _i64, _i64, _i64, _f, _f, _vp, _i64, _vp, _vp, _i64, _vp, _vp]),
+    ("db_kv8_append", _i32, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
+    ("db_kv8_attention", _i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f, _vp, _i64, _vp]),
+    ("db_kv8_read", _i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
+    ("db_logit_rules", _i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
+                              _i64, _vp, _i64, _vp, _vp, _vp]),
     ("db_synthetic_bf16", _i32, [C.c_uint64, C.c_uint64, _i64, _f, _vp, _vp]),
     ("db_model_create", _vp, [_i32, C.POINTER(EncoderConfig), C.POINTER(EncoderWeights), C.POINTER(DbError)]),
     ("db_model_create_synthetic", _vp, [_i32, C.POINTER(EncoderConfig), C.c_uint64, _f, C.POINTER(DbError)]),

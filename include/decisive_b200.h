@@ -258,6 +258,86 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
                          const void *vp, int64_t P, int causal, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                          float scale, float *out, int64_t ldo, void *stream);
 
+/* ---- generation operators.  Packed rows: `items` sequences' rows lie one after another; cu_seqlens
+ * (device, int32 [items + 1]) gives their offsets, NULL means equal items (rows = items * max_len).
+ * max_len / max_rows is the longest item's rows (longer items are cut to it; it sizes the launch).
+ * Row strides are in elements; rows of 16-bit tensors start on 16-byte boundaries (stride % 8 == 0).
+ * head_dim is 128; other values give DB_ERR_UNSUPPORTED.  Device-side offsets, lengths and page numbers outside
+ * their tensors are brought back inside or skipped; the cache entries note them in the error word
+ * (db_device_error_word). ---- */
+
+/* The gated delta rule (linear attention with a 128 x 128 state per value head; the recurrence
+ * of backbone.rs:349-469).  q, k [rows, k_heads, 128], v [rows, v_heads, 128] (f16 or bf16), g (log decay) and
+ * beta (writing strength) f32 [rows, v_heads]; value head h uses key head h / (v_heads / k_heads).
+ * Per sequence and value head, token by token, with S [128 (value), 128 (key)] in f32:
+ *   S <- e^g S;  u = beta (v - S k');  S <- S + u k'^T;  out = S q'
+ * norm_eps >= 0: k' = k / sqrt(sum k^2 + norm_eps), q' = scale * q / sqrt(sum q^2 + norm_eps); norm_eps < 0:
+ * k' = k, q' = scale * q.  g = -inf forgets everything before the token.  state_in f32 [v_heads, 128, 128]
+ * per item, state_stride floats apart (0: one kept prefix state for all items; NULL: zeros); state_out
+ * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own).
+ * An item without rows passes its state on.  out [rows, v_heads, 128] in v's type.  workspace: device
+ * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0). */
+size_t db_gated_delta_workspace_bytes(int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads);
+int db_gated_delta(const void *q, const void *k, const void *v, int dtype, int64_t ldq, int64_t ldk, int64_t ldv,
+                   const float *g, const float *beta, int64_t ldg, int64_t ldb, const int32_t *cu_seqlens,
+                   int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads, int64_t head_dim,
+                   float scale, float norm_eps, const float *state_in, int64_t state_stride, float *state_out,
+                   void *out, int64_t ldo, void *workspace, void *stream);
+
+/* The 8-bit paged key/value cache.  A sequence's tokens lie in blocks of DB_KV8_BLOCK; a full block is
+ * one page (page_table [sequences, table_width]: block i of sequence b is page page_table[b, i]) of
+ * int8 codes per kv head with one f32 scale for keys and one for values: scale = max(max|x| * (1.0f / 127),
+ * FLT_MIN), code = round half even (x / scale).  The open block of a sequence stays in 16 bits (k_tail,
+ * v_tail, of `dtype`: token p in slot p % 64) until its last token comes; the codes are the same
+ * however the tokens were split over appends.  A full block with a non-finite value reads as NaN as
+ * a whole.  All tensors are the caller's, dense, 16-byte aligned. */
+#define DB_KV8_BLOCK 64
+typedef struct db_kv8_cache {
+    int8_t *k_codes;           /* [pages, kv_heads, 64 (token), 128] */
+    float *k_scales;           /* [pages, kv_heads] */
+    int8_t *v_codes;           /* [pages, kv_heads, 128, 64 (token)] */
+    float *v_scales;           /* [pages, kv_heads] */
+    void *k_tail;              /* [sequences, kv_heads, 64 (token), 128] of dtype */
+    void *v_tail;              /* [sequences, kv_heads, 128, 64 (token)] of dtype */
+    const int32_t *page_table; /* [sequences, table_width] */
+    int32_t pages, table_width, sequences, kv_heads, head_dim;
+    int32_t dtype; /* DB_DTYPE_F16 or DB_DTYPE_BF16: the tails', and that of k, v, q and out */
+} db_kv8_cache;
+/* Writes the new rows of items 0 .. items - 1 (k, v [rows, kv_heads, 128]) at positions lengths[b]
+ * (int32, device) on.  The lengths are the caller's to advance, once all layers have taken the step. */
+int db_kv8_append(const db_kv8_cache *cache, const void *k, int64_t ldk, const void *v, int64_t ldv,
+                  const int32_t *lengths, const int32_t *cu_seqlens, int64_t items, int64_t rows, int64_t max_rows,
+                  void *stream);
+/* Attention over the cache after an append: row i of item b (position p = lengths[b] + i, the same
+ * lengths as the append's) sees the cached keys 0 .. p: out = softmax(scale q.k) v.  q, out
+ * [rows, q_heads, 128]; query head h uses kv head h / (q_heads / kv_heads).  max_keys: an upper bound on
+ * lengths + rows over the items, which sizes the split of the keys (0: the table's width).  A row that
+ * can read no key (its pages are missing) is 0. */
+int db_kv8_attention(const db_kv8_cache *cache, const void *q, int64_t ldq, const int32_t *lengths,
+                     const int32_t *cu_seqlens, int64_t items, int64_t rows, int64_t max_rows, int64_t max_keys,
+                     int64_t q_heads, float scale, void *out, int64_t ldo, void *stream);
+/* The cached values of tokens 0 .. max_keys - 1 (0 from lengths[b] on): k, v f32 [items, max_keys,
+ * kv_heads, 128]. */
+int db_kv8_read(const db_kv8_cache *cache, const int32_t *lengths, int64_t items, int64_t max_keys, float *k, float *v,
+                void *stream);
+
+/* Rules on logits and the answer they lead to.  Per row and token id, in f32 and in this order, with c
+ * the token's count in history[row, 0 .. history_lens[row]) (ids outside the vocabulary do not count;
+ * history_lens NULL: history_cols):
+ *   c > 0: x = x > 0 ? x / repetition : x * repetition;  x = x - (presence + frequency * c)
+ *   x = x + bias, for every entry j with bias_ids[row, j] = id, in order
+ *   x = -inf where bit id % 32 of mask[row, id / 32] is 0
+ * out f32 [rows, vocab] = x (may be the logits themselves when they are f32); best[row] = the lowest id of
+ * the largest x (-1: nothing allowed), lse[row] = log sum e^x (-inf: nothing allowed), so out - lse are
+ * log-probabilities.  A NaN is never the best and makes lse NaN.  repetition, presence, frequency
+ * f32 [rows], bias_ids / bias_values [rows, biases] (at most 1024 a row), mask, history, best and lse may be
+ * NULL.  logits f32, f16 or bf16, vocab <= 786432. */
+int db_logit_rules(const void *logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const int32_t *history,
+                   int64_t ldh, const int32_t *history_lens, int64_t history_cols, const float *repetition,
+                   const float *presence, const float *frequency, const int32_t *bias_ids, const float *bias_values,
+                   int64_t biases, const uint32_t *mask, int64_t ldm, float *out, int64_t ldo, int32_t *best,
+                   float *lse, void *stream);
+
 /* Deterministic synthetic bf16 tensor on the device: value_i = std * N(0,1) from a
  * counter-based generator keyed by (seed, tensor). */
 int db_synthetic_bf16(uint64_t seed, uint64_t tensor, int64_t n, float std, uint16_t *out, void *stream);
