@@ -338,7 +338,7 @@ def gated_delta(q, k, v, g, beta, items: int = 1, cu_seqlens=None, max_len: int 
     if out.shape != (rows, hv, 128):
         raise ValueError("gated_delta: out differs from v in its shape")
     lib = load()
-    need = lib.db_gated_delta_workspace_bytes(items, rows, max_len, hk, hv)
+    need = lib.db_gated_delta_workspace_bytes(items, rows, max_len, hk, hv, code)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     check(lib.db_gated_delta(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ldq, ldk, ldv, g.data_ptr(),
                              beta.data_ptr(), g.stride(0) if rows > 1 else hv, beta.stride(0) if rows > 1 else hv,

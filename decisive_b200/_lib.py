@@ -89,7 +89,7 @@ SIGNATURES = [
     ("db_attention", _i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _f, _vp, _i64, _vp]),
     ("db_attention_decoder", _i32, [_vp, _vp, _vp, _i64, _i64, _vp, _vp, _i64, C.c_int, _i64, _i64, _i64, _f, _vp,
                                     _i64, _vp]),
-    ("db_gated_delta_workspace_bytes", _sz, [_i64] * 5),
+    ("db_gated_delta_workspace_bytes", _sz, [_i64] * 5 + [_i32]),
     ("db_gated_delta", _i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
                               _i64, _i64, _i64, _f, _f, _vp, _i64, _vp, _vp, _i64, _vp, _vp]),
     ("db_kv8_append", _i32, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),

@@ -277,7 +277,8 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
  * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own).
  * An item without rows passes its state on.  out [rows, v_heads, 128] in v's type.  workspace: device
  * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0). */
-size_t db_gated_delta_workspace_bytes(int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads);
+size_t db_gated_delta_workspace_bytes(int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads,
+                                      int dtype);
 int db_gated_delta(const void *q, const void *k, const void *v, int dtype, int64_t ldq, int64_t ldk, int64_t ldv,
                    const float *g, const float *beta, int64_t ldg, int64_t ldb, const int32_t *cu_seqlens,
                    int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads, int64_t head_dim,
