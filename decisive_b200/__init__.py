@@ -419,11 +419,11 @@ def kv8_append(cache: KvCache8, k, v, lengths, cu_seqlens=None, max_rows: int | 
                                most, _raw_stream(dev)))
 
 
-def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | None = None, max_keys: int = 0,
-                  scale: float | None = None, out=None):
+def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | None = None,
+                  max_keys: int | None = None, scale: float | None = None, out=None):
     """Attention over the cache after the append of the same rows: row i of item b sees the cached keys
-    0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: an upper bound on the longest item's keys, if
-    the caller knows one below the table's width (it only sizes the launch)."""
+    0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: the longest item's keys, as far as the caller
+    knows (default: the table's width); it only sizes the launch and the workspace."""
     import torch
     dt, dev = cache.k_tail.dtype, cache.k_tail.device
     ldq = _heads("q", q, dt, dev)
@@ -433,9 +433,13 @@ def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | 
     ldo = _heads("out", out, dt, dev)
     if out.shape != q.shape:
         raise ValueError("kv8_attention: out differs from q in its shape")
-    check(load().db_kv8_attention(cache.ref, q.data_ptr(), ldq, lengths.data_ptr(), cu, items, rows, most, max_keys,
-                                  q.shape[1], 128 ** -0.5 if scale is None else scale, out.data_ptr(), ldo,
-                                  _raw_stream(dev)))
+    lib, heads = load(), q.shape[1]
+    keys = max(1, max_keys or cache.page_table.shape[1] * 64)
+    need = lib.db_kv8_attention_workspace_bytes(items, most, keys, cache.k_tail.shape[1], heads)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.db_kv8_attention(cache.ref, q.data_ptr(), ldq, lengths.data_ptr(), cu, items, rows, most, keys, heads,
+                               128 ** -0.5 if scale is None else scale, out.data_ptr(), ldo,
+                               ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
     return out
 
 

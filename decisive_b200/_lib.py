@@ -93,7 +93,8 @@ SIGNATURES = [
     ("db_gated_delta", _i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64,
                               _i64, _i64, _i64, _f, _f, _vp, _i64, _vp, _vp, _i64, _vp, _vp]),
     ("db_kv8_append", _i32, [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
-    ("db_kv8_attention", _i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f, _vp, _i64, _vp]),
+    ("db_kv8_attention_workspace_bytes", _sz, [_i64] * 5),
+    ("db_kv8_attention", _i32, [_vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _f, _vp, _i64, _vp, _vp]),
     ("db_kv8_read", _i32, [_vp, _vp, _i64, _i64, _vp, _vp, _vp]),
     ("db_logit_rules", _i32, [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _vp,
                               _i64, _vp, _i64, _vp, _vp, _vp]),

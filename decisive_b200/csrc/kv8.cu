@@ -7,18 +7,17 @@
 // quantised once, when its last token comes, so the codes do not depend on how the tokens were
 // split over appends.  Keys are stored [64 tokens, 128], values [128, 64 tokens]: both are then
 // read along the axis that their product sums over, 16 bytes at a time and without a transpose.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <float.h>
 
+#include <algorithm>
+#include <string>
 #include <type_traits>
 
 #include "../../include/decisive_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
 #include "kernels.h"
-
-namespace cg = cooperative_groups;
 
 namespace db {
 namespace {
@@ -63,8 +62,6 @@ __device__ __forceinline__ int page_of(const Kv8Args& a, int b, int i) {
 
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f32(float x, __half& y) { y = __float2half_rn(x); }
-__device__ __forceinline__ void from_f32(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
 template <typename T>
 __device__ __forceinline__ float from_bits(uint32_t b) {
     const unsigned short h = (unsigned short)b;
@@ -86,6 +83,7 @@ __global__ void __launch_bounds__(APPEND_THREADS)
     __shared__ uint32_t largest[2];
     __shared__ __align__(16) T vt[BLK * V_PITCH];
     pdl_wait();
+    pdl_trigger();
     const int tid = threadIdx.x, h = blockIdx.y, b = blockIdx.z, Hk = a.c.kv_heads;
     int start, count, len;
     item_of(a, b, start, count, len);
@@ -141,12 +139,21 @@ __global__ void __launch_bounds__(APPEND_THREADS)
         }
         most(kmax, key[i]);
     }
-    for (int e = tid; e < D * kept; e += APPEND_THREADS) {
-        const int c = e / kept, r = e % kept;
-        const T x = v_tail[c * BLK + r];
-        vmax = max(vmax, (uint32_t) * reinterpret_cast<const unsigned short*>(&x) & 0x7fffu);
-        vt[r * V_PITCH + c] = x;
-    }
+    if (kept)
+        for (int e = tid; e < D * BLK / 8; e += APPEND_THREADS) {
+            // (slots past the kept ones hold older tokens)
+            const int c = e % D, r0 = e / D * 8;
+            const uint4 x = *reinterpret_cast<const uint4*>(v_tail + c * BLK + r0);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const unsigned short u = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
+                if (r0 + j < kept) {
+                    vmax = max(vmax, (uint32_t)u & 0x7fffu);
+                    vt[(r0 + j) * V_PITCH + c] = *reinterpret_cast<const T*>(&u);
+                }
+            }
+        }
     __syncthreads();
     kmax = __reduce_max_sync(0xffffffffu, kmax);
     vmax = __reduce_max_sync(0xffffffffu, vmax);
@@ -166,29 +173,50 @@ __global__ void __launch_bounds__(APPEND_THREADS)
             a.c.k_scales[ph] = ks;
             a.c.v_scales[ph] = vs;
         }
-        auto code = [](float x, float s) {
-            const float c = rintf(__fdiv_rn(x, s));
-            return (uint32_t)(c == c ? (int)fminf(fmaxf(c, -127.f), 127.f) : 0) & 0xffu;
+        // round half even (x / s): the product with 1 / s decides unless it lies near a half.  1.5 x 2^23 + code
+        // has the code's two's complement in its low byte, and |x / s| never passes 127.
+        const float ki = __fdiv_rn(1.f, ks), vi = __fdiv_rn(1.f, vs);
+        constexpr float MAGIC = 12582912.f;
+        auto four = [](const float (&x)[4], float s, float inverse) {
+            uint32_t r[4];
+            bool near = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float y = fmaf(x[j], inverse, MAGIC), left = fmaf(x[j], inverse, -(y - MAGIC));
+                near |= !(fabsf(left) < 0.499f);
+                r[j] = __float_as_uint(y);
+            }
+            if (near) {
+#pragma unroll 1
+                for (int j = 0; j < 4; ++j) {
+                    const float v = j == 0 ? x[0] : j == 1 ? x[1] : j == 2 ? x[2] : x[3];
+                    const uint32_t y = s == s ? __float_as_uint(rintf(__fdiv_rn(v, s)) + MAGIC) : 0u;
+                    r[0] = j == 0 ? y : r[0], r[1] = j == 1 ? y : r[1], r[2] = j == 2 ? y : r[2], r[3] = j == 3 ? y : r[3];
+                }
+            }
+            return __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
         };
         int8_t* kp = a.c.k_codes + ph * BLK * D;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int e = tid + i * APPEND_THREADS;
-            const uint32_t w[4] = {key[i].x, key[i].y, key[i].z, key[i].w};
-            uint32_t o[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[j >> 1] |= code(from_bits<T>(w[j] & 0xffffu), ks) << (16 * (j & 1));
-                o[j >> 1] |= code(from_bits<T>(w[j] >> 16), ks) << (16 * (j & 1) + 8);
-            }
-            *reinterpret_cast<uint2*>(kp + (int64_t)e * 8) = make_uint2(o[0], o[1]);
+            const float x[4] = {from_bits<T>(key[i].x & 0xffffu), from_bits<T>(key[i].x >> 16), from_bits<T>(key[i].y & 0xffffu),
+                                from_bits<T>(key[i].y >> 16)};
+            const float y[4] = {from_bits<T>(key[i].z & 0xffffu), from_bits<T>(key[i].z >> 16), from_bits<T>(key[i].w & 0xffffu),
+                                from_bits<T>(key[i].w >> 16)};
+            *reinterpret_cast<uint2*>(kp + (int64_t)e * 8) = make_uint2(four(x, ks, ki), four(y, ks, ki));
         }
         int8_t* vp = a.c.v_codes + ph * D * BLK;
-        for (int e = tid; e < D * BLK / 16; e += APPEND_THREADS) {
-            const int c = e % D, r0 = e / D * 16;  // value feature c, tokens r0 .. r0 + 15
-            uint32_t o[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j >> 2] |= code(to_f32(vt[(r0 + j) * V_PITCH + c]), vs) << (8 * (j & 3));
+        for (int i = 0; i < D * BLK / 16 / APPEND_THREADS; ++i) {
+            const int e = tid + i * APPEND_THREADS, c = e % D, r0 = e / D * 16;  // value feature c, tokens r0 .. r0 + 15
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x[4] = {to_f32(vt[(r0 + 4 * j) * V_PITCH + c]), to_f32(vt[(r0 + 4 * j + 1) * V_PITCH + c]),
+                                    to_f32(vt[(r0 + 4 * j + 2) * V_PITCH + c]), to_f32(vt[(r0 + 4 * j + 3) * V_PITCH + c])};
+                o[j] = four(x, vs, vi);
+            }
             *reinterpret_cast<uint4*>(vp + c * BLK + r0) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
@@ -197,11 +225,17 @@ __global__ void __launch_bounds__(APPEND_THREADS)
 }
 
 // ------------------------------------------------------------------ read back
-// The cached values of tokens 0 .. max_keys - 1 in f32 (0 past an item's length).
+// The cached values of tokens 0 .. max_keys - 1 in f32 (0 past an item's length).  One CTA per block, kv head and
+// keys or values; HBM bound.  16-byte loads and stores; the values turn in shared memory.
+constexpr int READ_THREADS = 256, READ_PITCH = D + 4;
+
 template <typename T>
-__global__ void kv8_read_kernel(Kv8Args a, int64_t max_keys, float* __restrict__ k, float* __restrict__ v) {
-    __shared__ float tile[BLK][D + 1];
-    const int tid = threadIdx.x, block = blockIdx.x, h = blockIdx.y, b = blockIdx.z, Hk = a.c.kv_heads;
+__global__ void __launch_bounds__(READ_THREADS)
+    kv8_read_kernel(Kv8Args a, int64_t max_keys, float* __restrict__ k, float* __restrict__ v) {
+    __shared__ __align__(16) float tile[BLK * READ_PITCH];
+    pdl_wait();
+    const int tid = threadIdx.x, which = blockIdx.x & 1, block = blockIdx.x >> 1, h = blockIdx.y, b = blockIdx.z;
+    const int Hk = a.c.kv_heads;
     int start, count, len;
     item_of(a, b, start, count, len);
     const int n = (int)min((int64_t)BLK, max_keys - (int64_t)block * BLK);
@@ -209,21 +243,44 @@ __global__ void kv8_read_kernel(Kv8Args a, int64_t max_keys, float* __restrict__
     const int inside = min(max(len - block * BLK, 0), BLK);
     const int page = full ? page_of(a, b, block) : -1;
     const int64_t ph = (int64_t)page * Hk + h, tail = ((int64_t)b * Hk + h) * BLK * D;
-    for (int which = 0; which < 2; ++which) {
-        const float scale = page >= 0 ? (which ? a.c.v_scales : a.c.k_scales)[ph] : 0.f;
-        for (int e = tid; e < BLK * D; e += blockDim.x) {
-            const int r = which ? e % BLK : e / D, c = which ? e / BLK : e % D;
-            float x = 0.f;
-            if (page >= 0)
-                x = __fmul_rn((float)(which ? a.c.v_codes : a.c.k_codes)[ph * BLK * D + e], scale);
-            else if (!full && r < inside)
-                x = to_f32(static_cast<const T*>(which ? a.c.v_tail : a.c.k_tail)[tail + e]);
-            tile[r][c] = x;
+    // 16 values at a time: of one token for keys (row r, features c ..), of one feature for values
+    for (int e = tid; e < BLK * D / 16; e += READ_THREADS) {
+        const int r = which ? e / D * 16 : e / (D / 16), c = which ? e % D : e % (D / 16) * 16;
+        const int64_t at = which ? (int64_t)c * BLK + r : (int64_t)r * D + c;
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = 0.f;
+        if (page >= 0) {
+            const uint4 w = *reinterpret_cast<const uint4*>((which ? a.c.v_codes : a.c.k_codes) + ph * BLK * D + at);
+            const float scale = (which ? a.c.v_scales : a.c.k_scales)[ph];
+            const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                x[j] = __fmul_rn((float)(int)(int8_t)(q[j >> 2] >> (8 * (j & 3))), scale);
+        } else if (!full && (which || r < inside)) {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(which ? a.c.v_tail : a.c.k_tail) + tail + at);
+            const uint4 w0 = src[0], w1 = src[1];
+            const uint32_t q[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (!which || r + j < inside) x[j] = from_bits<T>((q[j >> 1] >> (16 * (j & 1))) & 0xffffu);
         }
-        __syncthreads();
-        float* out = (which ? v : k) + (((int64_t)b * max_keys + (int64_t)block * BLK) * Hk + h) * D;
-        for (int e = tid; e < n * D; e += blockDim.x) out[(int64_t)(e / D) * Hk * D + e % D] = tile[e / D][e % D];
-        __syncthreads();
+        if (which) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) tile[(r + j) * READ_PITCH + c] = x[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float4*>(&tile[r * READ_PITCH + c + 4 * j]) =
+                    make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+        }
+    }
+    __syncthreads();
+    float* out = (which ? v : k) + (((int64_t)b * max_keys + (int64_t)block * BLK) * Hk + h) * D;
+    for (int e = tid; e < n * (D / 4); e += READ_THREADS) {
+        const int r = e / (D / 4), c = e % (D / 4) * 4;
+        __stcs(reinterpret_cast<float4*>(out + (int64_t)r * Hk * D + c),
+               *reinterpret_cast<const float4*>(&tile[r * READ_PITCH + c]));
     }
 }
 
@@ -240,6 +297,12 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 2^x on the special-function unit
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 // The 8 x 8 matrix of 16-bit values that a warp holds, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -278,6 +341,7 @@ struct AttnArgs {
     int64_t ldo;
     int group;     // query heads per kv head
     float factor;  // scale * log2 e
+    float* parts;  // decode: partial results, see kv8_decode_kernel
 };
 
 // Scores and the context are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that the codes are
@@ -290,86 +354,96 @@ struct AttnArgs {
 // half `half` of score tile s, which makes P^T's fragment the four bytes 4s..4s+3 of each 16 of V^T.
 // Codes become f16 exactly; q is scaled by a power of two per row into f16 (bf16 has fewer bits
 // and more range), so the scores' product rounds neither operand.  P is rounded after its f32 sum is
-// taken, to one f16 for bf16 outputs and to two for f16 ones.  A block's own context is scaled by its value scale when
-// it joins the running one, in f32.
+// taken, to one f16 for bf16 outputs and to two for f16 ones (one rounding of P to f16 is as large as the
+// output's own).  A block's own context is scaled by its value scale when it joins the running one, in f32.
 //
-// A warp takes whole blocks, with running maxima and sums of its own; the warps of a CTA and the
-// CTAs of a cluster share a tile's keys and join once at the end, in a fixed order.
+// The tile of 8 NT query rows that a warp works on, with its running maxima and sums (log2 domain; column
+// 2 t + j of n tile n in [n][j], equal in the 8 lanes g) and its context (feature 16 d + 8 (j >> 1) + g).
 template <typename T, int NT>
-struct Warp {
-    float O[8][NT][4];
+struct Tile {
+    static constexpr bool TWO = std::is_same<T, __half>::value;
+    // query fragments, k step 4 c + s: in registers, or for more rows in shared memory ([NT][8][32], the warp's own)
+    uint2 qf[NT == 1 ? 8 : 1];
+    uint2* qs;
+    float factor[NT][2];   // scale * log2 e / the row's power of two
+    int limit[NT][2];      // last key that a column's row sees; -1: none
+    int first_limit;       // of the tile's first row
+    bool ragged;           // rows past the item's end
     float m[NT][2], l[NT][2];
-};
+    float O[8][NT][4];
+    // where the rows are
+    const T* q;
+    int row0, rows, group;
+    int64_t ldq;
+    float plain;           // scale * log2 e
 
-template <typename T, int NT, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) kv8_attention_kernel(AttnArgs a) {
-    constexpr int ROWS = 8 * NT;
-    constexpr bool TWO = std::is_same<T, __half>::value;
-    extern __shared__ __align__(16) uint8_t attn_smem[];
-    cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int split = cluster.block_rank(), splits = cluster.num_blocks();
-    const int h = blockIdx.y, b = blockIdx.z, tile = blockIdx.x / splits, Hk = a.kv.c.kv_heads;
-    // shared memory: query fragments and factors, then (over them) the joined results
-    uint2* qfrag = reinterpret_cast<uint2*>(attn_smem);                // [NT][8][32]
-    float* qfactor = reinterpret_cast<float*>(qfrag + NT * 8 * 32);    // [ROWS]
-    pdl_wait();
-    pdl_trigger();
-    int start, count, len;
-    item_of(a.kv, b, start, count, len);
-    const int rows = count * a.group, row0 = tile * ROWS;
-    if (row0 >= rows) return;  // the whole cluster leaves: tile is the cluster's
-    const T* q = static_cast<const T*>(a.q);
-    auto q_at = [&](int r) { return q + (int64_t)(start + r / a.group) * a.ldq + ((int64_t)h * a.group + r % a.group) * D; };
-
-    // queries: one warp per row, 4 values a lane; scaled to [0.5, 1) x 2^8 at the row's largest value
-    for (int r = warp; r < ROWS; r += WARPS) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row0 + r < rows) {
-            const uint2 w = *reinterpret_cast<const uint2*>(q_at(row0 + r) + 4 * lane);
-            x[0] = from_bits<T>(w.x & 0xffffu), x[1] = from_bits<T>(w.x >> 16);
-            x[2] = from_bits<T>(w.y & 0xffffu), x[3] = from_bits<T>(w.y >> 16);
-        }
-        float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int e = top > 0.f && top < INFINITY ? min(max(8 - ilogbf(top), -126), 126) : 0;
-        const float up = ldexpf(1.f, e);
-        if (lane == 0) qfactor[r] = ldexpf(1.f, -e);
-        // dims 4 lane .. 4 lane + 3 = half c, quarter t' of it (16 dims), k step s
-        const int c = lane >> 4, tt = (lane >> 2) & 3, s = lane & 3;
-        qfrag[((r >> 3) * 8 + c * 4 + s) * 32 + (r & 7) * 4 + tt] =
-            make_uint2(pack2<__half>(x[0] * up, x[1] * up), pack2<__half>(x[2] * up, x[3] * up));
+    __device__ uint2 query(int n, int step) const {
+        if constexpr (NT == 1) return qf[step];
+        return qs[(n * 8 + step) * 32 + (threadIdx.x & 31)];
     }
-    __syncthreads();
+    __device__ const T* row_at(int r) const { return q + (int64_t)(r / group) * ldq + (int64_t)(r % group) * D; }
 
-    Warp<T, NT> w;
-    float factor[NT][2];
-    int limit[NT][2];  // last key that a column's row sees; -1: none
-    int first_limit = 0x7fffffff, last_limit = -1;
+    // q: the item's first row at the kv head's first query head; the tile starts at row r0 of `all`
+    __device__ void open(uint2* shared, const T* base, int64_t ld, int r0, int all, int len, int grp, float fac) {
+        qs = shared;
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        q = base, ldq = ld, row0 = r0, rows = all, group = grp, plain = fac;
+        first_limit = len + r0 / grp;
+        ragged = r0 + 8 * NT > all;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+            const int r = r0 + n * 8 + g;
+            uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int r = row0 + n * 8 + 2 * t + j;
-            factor[n][j] = a.factor * qfactor[n * 8 + 2 * t + j];
-            limit[n][j] = r < rows ? len + r / a.group : -1;
-            w.m[n][j] = -INFINITY;
-            w.l[n][j] = 0.f;
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (r < all) x = *reinterpret_cast<const uint4*>(row_at(r) + 64 * c + 16 * t + 8 * i);
+                    w[8 * c + 4 * i] = x.x, w[8 * c + 4 * i + 1] = x.y, w[8 * c + 4 * i + 2] = x.z, w[8 * c + 4 * i + 3] = x.w;
+                }
+            // to [2^8, 2^9) at the row's largest value
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float big = from_bits<T>(top);
+            const int e = (int)(__float_as_uint(big) >> 23) - 127;
+            const int k = big > 0.f && e < 128 ? min(max(8 - e, -126), 126) : 0;
+            const float up = __uint_as_float((uint32_t)(127 + k) << 23), back = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                uint2 x;
+                x.x = pack2<__half>(from_bits<T>(w[2 * i] & 0xffffu) * up, from_bits<T>(w[2 * i] >> 16) * up);
+                x.y = pack2<__half>(from_bits<T>(w[2 * i + 1] & 0xffffu) * up, from_bits<T>(w[2 * i + 1] >> 16) * up);
+                if constexpr (NT == 1)
+                    qf[i] = x;
+                else
+                    qs[(n * 8 + i) * 32 + lane] = x;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                factor[n][j] = fac * __shfl_sync(0xffffffffu, back, 4 * (2 * t + j));
+                const int rr = r0 + n * 8 + 2 * t + j;
+                limit[n][j] = rr < all ? len + rr / grp : -1;
+                m[n][j] = -INFINITY;
+                l[n][j] = 0.f;
+            }
         }
-    first_limit = len + row0 / a.group;
-    last_limit = len + (min(row0 + ROWS, rows) - 1) / a.group;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w.O[i][n][j] = 0.f;
+                for (int j = 0; j < 4; ++j) O[i][n][j] = 0.f;
+    }
 
-    // S^T of one block is in s (16 keys per tile): softmax step; leaves P in f32 in s, returns the
-    // factors of the running context
-    auto soften = [&](float (&s)[4][NT][4], const float (&f)[NT][2], int base, float (&alpha)[NT][2]) {
-        const bool masked = base + BLK - 1 > first_limit || row0 + ROWS > rows;
+    // S^T of the block at key `base` is in s (16 keys per tile): softmax step; leaves P in f32 in s and the
+    // factors of the running context in alpha
+    __device__ void soften(float (&s)[4][NT][4], const float (&f)[NT][2], int base, float (&alpha)[NT][2]) {
+        const int lane = threadIdx.x & 31, g = lane >> 2;
+        const bool masked = base + BLK - 1 > first_limit || ragged;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             float top[2] = {-INFINITY, -INFINITY};
@@ -389,100 +463,61 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attention_kernel(AttnArgs a) {
             for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int o = 4; o < 32; o *= 2) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], o));
-                const float now = fmaxf(w.m[n][j], top[j]);
+                const float now = fmaxf(m[n][j], top[j]);
                 const float at = now == -INFINITY ? 0.f : now;
-                alpha[n][j] = exp2f(w.m[n][j] - at);
-                w.m[n][j] = now;
+                alpha[n][j] = ex2(m[n][j] - at);
+                m[n][j] = now;
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float p = exp2f(s[i][n][2 * half + j] - at);
+                        const float p = ex2(s[i][n][2 * half + j] - at);
                         s[i][n][2 * half + j] = p;
                         sum += p;
                     }
-                w.l[n][j] = w.l[n][j] * alpha[n][j] + sum;
+                l[n][j] = l[n][j] * alpha[n][j] + sum;
             }
         }
-    };
+    }
 
-    // this warp's blocks: the split's share, every WARPS-th
-    const int blocks = last_limit / BLK + 1, whole = (len + count) / BLK;
-    const int share = (blocks + splits - 1) / splits, from = split * share, to = min(from + share, blocks);
-    for (int i = from + warp; i < to; i += WARPS) {
-        if (i < whole) {
-            const int page = page_of(a.kv, b, i);
-            if (page < 0) continue;
-            const int64_t ph = (int64_t)page * Hk + h;
-            const int8_t* kp = a.kv.c.k_codes + ph * BLK * D;
-            const int8_t* vp = a.kv.c.v_codes + ph * BLK * D;
-            const float ks = a.kv.c.k_scales[ph], vs = a.kv.c.v_scales[ph];
-            uint4 kc[4][2][2];  // score tile, row half, 64-wide half of the key
+    // a lane's share of a block's key codes: score tile, row half, 64-wide half of the key
+    __device__ static void load_keys(uint4 (&kc)[4][2][2], const int8_t* kp) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    kc[s][r][c] = __ldcs(reinterpret_cast<const uint4*>(
+                        kp + (16 * (g >> 1) + 4 * s + 2 * r + (g & 1)) * D + 64 * c + 16 * t));
+    }
+
+    // one full block: 64 keys' and values' codes of one head.  Its values are on their way while the scores are
+    // formed, and the next block's keys (after: null for none) while the context is: a warp always has 8 KB of
+    // loads in flight.
+    __device__ void block(uint4 (&kc)[4][2][2], const int8_t* vp, float ks, float vs, int base, const int8_t* after) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        constexpr bool AHEAD = NT == 1;  // (more rows leave no registers for it)
+        uint4 vc[AHEAD ? 8 : 1][2];
+        if constexpr (AHEAD)
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
+                    vc[d][r] = __ldcs(reinterpret_cast<const uint4*>(vp + (16 * d + 8 * r + g) * BLK + 16 * t));
+        float s[4][NT][4];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        kc[s][r][c] = __ldcs(reinterpret_cast<const uint4*>(
-                            kp + (16 * (g >> 1) + 4 * s + 2 * r + (g & 1)) * D + 64 * c + 16 * t));
-            float s[4][NT][4];
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i2][n][j] = 0.f;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t lo[4] = {kc[i2][0][c].x, kc[i2][0][c].y, kc[i2][0][c].z, kc[i2][0][c].w};
-                    const uint32_t hi[4] = {kc[i2][1][c].x, kc[i2][1][c].y, kc[i2][1][c].z, kc[i2][1][c].w};
-#pragma unroll
-                    for (int st = 0; st < 4; ++st) {
-                        uint32_t f[4];
-                        codes_to_f16(lo[st], f[0], f[2]);
-                        codes_to_f16(hi[st], f[1], f[3]);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint2 qf = qfrag[(n * 8 + c * 4 + st) * 32 + lane];
-                            mma16(s[i2][n], f, qf.x, qf.y, __half());
-                        }
-                    }
-                }
-            }
-            float alpha[NT][2], scaled[NT][2];
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) scaled[n][j] = factor[n][j] * ks;
-            soften(s, scaled, i * BLK, alpha);
-            // f16 outputs need P's next 11 bits as well: one rounding of P to f16 is as large as the output's
-            uint32_t p[NT][4][2], rest[TWO ? NT : 1][4][2];
+                for (int j = 0; j < 4; ++j) s[i][n][j] = 0.f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i2 = 0; i2 < 4; ++i2)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float x = s[i2][n][2 * half], y = s[i2][n][2 * half + 1];
-                        const uint32_t hi = pack2<__half>(x, y);
-                        p[n][i2][half] = transpose8(hi);
-                        if constexpr (TWO)
-                            rest[n][i2][half] = transpose8(
-                                pack2<__half>(x - from_bits<__half>(hi & 0xffffu), y - from_bits<__half>(hi >> 16)));
-                    }
-            float vf[NT][2];  // a block that a row does not see at all must not reach it (0 x NaN)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) vf[n][j] = limit[n][j] >= i * BLK ? vs : 0.f;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                const uint4 v0 = __ldcs(reinterpret_cast<const uint4*>(vp + (16 * d + g) * BLK + 16 * t));
-                const uint4 v1 = __ldcs(reinterpret_cast<const uint4*>(vp + (16 * d + 8 + g) * BLK + 16 * t));
-                const uint32_t lo[4] = {v0.x, v0.y, v0.z, v0.w}, hi[4] = {v1.x, v1.y, v1.z, v1.w};
-                float o[NT][4] = {};
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t lo[4] = {kc[i][0][c].x, kc[i][0][c].y, kc[i][0][c].z, kc[i][0][c].w};
+                const uint32_t hi[4] = {kc[i][1][c].x, kc[i][1][c].y, kc[i][1][c].z, kc[i][1][c].w};
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
                     uint32_t f[4];
@@ -490,235 +525,502 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_attention_kernel(AttnArgs a) {
                     codes_to_f16(hi[st], f[1], f[3]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma16(o[n], f, p[n][st][0], p[n][st][1], __half());
-                        if constexpr (TWO) mma16(o[n], f, rest[n][st][0], rest[n][st][1], __half());
+                        const uint2 q2 = query(n, 4 * c + st);
+                        mma16(s[i][n], f, q2.x, q2.y, __half());
                     }
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        w.O[d][n][j] = fmaf(o[n][j], vf[n][j & 1], w.O[d][n][j] * alpha[n][j & 1]);
             }
-        } else {
-            // the open block, in 16 bits: the same walk on its own type
-            const T* kt = static_cast<const T*>(a.kv.c.k_tail) + ((int64_t)b * Hk + h) * BLK * D;
-            const T* vt = static_cast<const T*>(a.kv.c.v_tail) + ((int64_t)b * Hk + h) * BLK * D;
-            const int inside = len + count - i * BLK;  // tokens of the block that are there
-            float s[4][NT][4];
+        }
+        if (after) load_keys(kc, after);
+        float alpha[NT][2], scaled[NT][2], vf[NT][2];
 #pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int j = 0; j < 2; ++j) {
+                scaled[n][j] = factor[n][j] * ks;
+                vf[n][j] = limit[n][j] >= base ? vs : 0.f;  // a block that a row does not see must not reach it (0 x NaN)
+            }
+        soften(s, scaled, base, alpha);
+        uint32_t p[NT][4][2], rest[TWO ? NT : 1][4][2];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) s[i2][n][j] = 0.f;
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-                uint32_t qr[NT][8];
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float x = s[i][n][2 * half], y = s[i][n][2 * half + 1];
+                    const uint32_t hi = pack2<__half>(x, y);
+                    p[n][i][half] = transpose8(hi);
+                    if constexpr (TWO)
+                        rest[n][i][half] = transpose8(
+                            pack2<__half>(x - from_bits<__half>(hi & 0xffffu), y - from_bits<__half>(hi >> 16)));
+                }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            uint4 v0, v1;
+            if constexpr (AHEAD) {
+                v0 = vc[d][0], v1 = vc[d][1];
+            } else {
+                v0 = __ldcs(reinterpret_cast<const uint4*>(vp + (16 * d + g) * BLK + 16 * t));
+                v1 = __ldcs(reinterpret_cast<const uint4*>(vp + (16 * d + 8 + g) * BLK + 16 * t));
+            }
+            const uint32_t lo[4] = {v0.x, v0.y, v0.z, v0.w}, hi[4] = {v1.x, v1.y, v1.z, v1.w};
+            float o[NT][4] = {};
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                uint32_t f[4];
+                codes_to_f16(lo[st], f[0], f[2]);
+                codes_to_f16(hi[st], f[1], f[3]);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const int r = min(row0 + n * 8 + g, rows - 1);
-                    const uint4* src = reinterpret_cast<const uint4*>(q_at(r) + 64 * c + 16 * t);
-                    const uint4 x = src[0], y = src[1];
-                    qr[n][0] = x.x, qr[n][1] = x.y, qr[n][2] = x.z, qr[n][3] = x.w;
-                    qr[n][4] = y.x, qr[n][5] = y.y, qr[n][6] = y.z, qr[n][7] = y.w;
-                }
-#pragma unroll
-                for (int i2 = 0; i2 < 4; ++i2) {
-                    const int key = 16 * (g >> 1) + 4 * i2 + (g & 1);
-                    const uint4* k0 = reinterpret_cast<const uint4*>(kt + key * D + 64 * c + 16 * t);
-                    const uint4* k1 = reinterpret_cast<const uint4*>(kt + (key + 2) * D + 64 * c + 16 * t);
-                    const uint4 a0 = k0[0], a1 = k0[1], b0 = k1[0], b1 = k1[1];
-                    const uint32_t lo[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-                    const uint32_t hi[8] = {b0.x, b0.y, b0.z, b0.w, b1.x, b1.y, b1.z, b1.w};
-#pragma unroll
-                    for (int st = 0; st < 4; ++st) {
-                        const uint32_t f[4] = {lo[2 * st], hi[2 * st], lo[2 * st + 1], hi[2 * st + 1]};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) mma16(s[i2][n], f, qr[n][2 * st], qr[n][2 * st + 1], T());
-                    }
+                    mma16(o[n], f, p[n][st][0], p[n][st][1], __half());
+                    if constexpr (TWO) mma16(o[n], f, rest[n][st][0], rest[n][st][1], __half());
                 }
             }
-            float alpha[NT][2], plain[NT][2];  // the queries come unscaled here
-#pragma unroll
-            for (int n = 0; n < NT; ++n) plain[n][0] = plain[n][1] = a.factor;
-            soften(s, plain, i * BLK, alpha);
-            // P in two parts of the tail's type, so that bf16 loses no more than f16
-            uint32_t p[NT][4][2], rest[NT][4][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i2 = 0; i2 < 4; ++i2)
+                for (int j = 0; j < 4; ++j) O[d][n][j] = fmaf(o[n][j], vf[n][j & 1], O[d][n][j] * alpha[n][j & 1]);
+        }
+    }
+
+    // the open block, in 16 bits: the same walk on its own type, rolled up (it is one of many blocks, and code
+    // that runs once costs its fetching); `inside` tokens of it are there
+    __device__ void tail(const T* kt, const T* vt, int inside, int base) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        float s[4][NT][4];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float x = s[i2][n][2 * half], y = s[i2][n][2 * half + 1];
-                        const uint32_t hi = pack2<T>(x, y);
-                        const uint32_t lo = pack2<T>(x - from_bits<T>(hi & 0xffffu), y - from_bits<T>(hi >> 16));
-                        p[n][i2][half] = transpose8(hi);
-                        rest[n][i2][half] = transpose8(lo);
-                    }
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                float o[NT][4] = {};
-                uint32_t f[2][8];
-                bool odd = false;  // a NaN or an infinity among the values
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[i][n][j] = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {  // 8 of each lane's 16 dims of a half
+            const int at = 64 * (c >> 1) + 16 * t + 8 * (c & 1);
+            uint4 qr[NT], kr[4][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) qr[n] = *reinterpret_cast<const uint4*>(row_at(min(row0 + n * 8 + g, rows - 1)) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    kr[i][r] = *reinterpret_cast<const uint4*>(kt + (16 * (g >> 1) + 4 * i + 2 * r + (g & 1)) * D + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t f0[4] = {kr[i][0].x, kr[i][1].x, kr[i][0].y, kr[i][1].y};
+                const uint32_t f1[4] = {kr[i][0].z, kr[i][1].z, kr[i][0].w, kr[i][1].w};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    mma16(s[i][n], f0, qr[n].x, qr[n].y, T());
+                    mma16(s[i][n], f1, qr[n].z, qr[n].w, T());
+                }
+            }
+        }
+        float alpha[NT][2], unscaled[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) unscaled[n][0] = unscaled[n][1] = plain;
+        soften(s, unscaled, base, alpha);
+        // P in two parts of the tail's type, so that bf16 loses no more than f16
+        uint32_t p[NT][4][2], rest[NT][4][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float x = s[i][n][2 * half], y = s[i][n][2 * half + 1];
+                    const uint32_t hi = pack2<T>(x, y);
+                    p[n][i][half] = transpose8(hi);
+                    rest[n][i][half] = transpose8(pack2<T>(x - from_bits<T>(hi & 0xffffu), y - from_bits<T>(hi >> 16)));
+                }
+        constexpr int BATCH = NT == 1 ? 2 : 1;  // feature tiles whose values are loaded together
+#pragma unroll 1
+        for (int d0 = 0; d0 < 8; d0 += BATCH) {
+            uint32_t f[BATCH][2][8];
+#pragma unroll
+            for (int d = 0; d < BATCH; ++d)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint4* src = reinterpret_cast<const uint4*>(vt + (16 * d + 8 * r + g) * BLK + 16 * t);
+                    const uint4* src = reinterpret_cast<const uint4*>(vt + (16 * (d0 + d) + 8 * r + g) * BLK + 16 * t);
                     const uint4 x = src[0], y = src[1];
-                    f[r][0] = x.x, f[r][1] = x.y, f[r][2] = x.z, f[r][3] = x.w;
-                    f[r][4] = y.x, f[r][5] = y.y, f[r][6] = y.z, f[r][7] = y.w;
+                    f[d][r][0] = x.x, f[d][r][1] = x.y, f[d][r][2] = x.z, f[d][r][3] = x.w;
+                    f[d][r][4] = y.x, f[d][r][5] = y.y, f[d][r][6] = y.z, f[d][r][7] = y.w;
+                }
+            float o[BATCH][NT][4];
+            bool odd = false;  // a NaN or an infinity among the values
+#pragma unroll
+            for (int d = 0; d < BATCH; ++d) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         // slots that hold no token yet, and what is not finite, stay out of the product
+                        constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
                         const int key = 16 * t + 2 * e;
-                        uint32_t lo = f[r][e] & 0xffffu, hi = f[r][e] >> 16;
-                        if (key >= inside) lo = 0;
-                        if (key + 1 >= inside) hi = 0;
-                        const bool bl = !isfinite(from_bits<T>(lo)), bh = !isfinite(from_bits<T>(hi));
+                        uint32_t lo = key < inside ? f[d][r][e] & 0xffffu : 0, hi = key + 1 < inside ? f[d][r][e] >> 16 : 0;
+                        const bool bl = (lo & INF) == INF, bh = (hi & INF) == INF;
                         odd |= bl | bh;
-                        f[r][e] = (bl ? 0 : lo) | (bh ? 0 : hi) << 16;
+                        f[d][r][e] = (bl ? 0 : lo) | (bh ? 0 : hi) << 16;
                     }
-                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[d][n][j] = 0.f;
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
-                    const uint32_t fa[4] = {f[0][2 * st], f[1][2 * st], f[0][2 * st + 1], f[1][2 * st + 1]};
+                    const uint32_t fa[4] = {f[d][0][2 * st], f[d][1][2 * st], f[d][0][2 * st + 1], f[d][1][2 * st + 1]};
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma16(o[n], fa, p[n][st][0], p[n][st][1], T());
-                        mma16(o[n], fa, rest[n][st][0], rest[n][st][1], T());
+                        mma16(o[d][n], fa, p[n][st][0], p[n][st][1], T());
+                        mma16(o[d][n], fa, rest[n][st][0], rest[n][st][1], T());
                     }
                 }
-                if (__any_sync(0xffffffffu, odd)) {
-                    // such a value reaches the rows that see its key, and no other
+            }
+            if (__any_sync(0xffffffffu, odd)) {
+                // such a value reaches the rows that see its key, and no other
+#pragma unroll
+                for (int d = 0; d < BATCH; ++d)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
+#pragma unroll 1
                         for (int key = 0; key < min(inside, BLK); ++key) {
-                            const float x = to_f32(vt[(16 * d + 8 * r + g) * BLK + key]);
+                            const float x = to_f32(vt[(16 * (d0 + d) + 8 * r + g) * BLK + key]);
                             if (isfinite(x)) continue;
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
                                 for (int j = 0; j < 2; ++j)
-                                    if (i * BLK + key <= limit[n][j]) o[n][2 * r + j] += x;
+                                    if (base + key <= limit[n][j]) o[d][n][2 * r + j] += x;
                         }
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w.O[d][n][j] = fmaf(w.O[d][n][j], alpha[n][j & 1], o[n][j]);
             }
-        }
-    }
-
-    // join: sums over the lanes that share a column, then the warps, then the cluster's CTAs
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int o = 4; o < 32; o *= 2) w.l[n][j] += __shfl_xor_sync(0xffffffffu, w.l[n][j], o);
-    float* part_o = reinterpret_cast<float*>(attn_smem);          // [WARPS][ROWS][D + 4]
-    float* part_m = part_o + WARPS * ROWS * (D + 4);              // [WARPS][ROWS]
-    float* part_l = part_m + WARPS * ROWS;
-    float* cta_m = part_l + WARPS * ROWS;                         // [ROWS]
-    float* cta_l = cta_m + ROWS;
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int r = n * 8 + 2 * t + (j & 1);
 #pragma unroll
             for (int d = 0; d < 8; ++d)
-                part_o[(warp * ROWS + r) * (D + 4) + 16 * d + 8 * (j >> 1) + g] = w.O[d][n][j];
-            if (g == 0 && j < 2) {
-                part_m[warp * ROWS + r] = w.m[n][j];
-                part_l[warp * ROWS + r] = w.l[n][j];
+                if (d >= d0 && d < d0 + BATCH)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            O[d][n][j] = fmaf(O[d][n][j], alpha[n][j & 1], o[d % BATCH][n][j]);
+        }
+    }
+
+    // l over the lanes that share a column
+    __device__ void close() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int o = 4; o < 32; o *= 2) l[n][j] += __shfl_xor_sync(0xffffffffu, l[n][j], o);
+    }
+
+    // the finished rows; out: the item's first row at the kv head's first query head
+    __device__ void write(T* out, int64_t ldo) const {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float i0 = l[n][0] == 0.f ? 0.f : 1.f / l[n][0], i1 = l[n][1] == 0.f ? 0.f : 1.f / l[n][1];
+            const int r = row0 + n * 8 + g;
+            T* dst = out + (int64_t)(r / group) * ldo + (int64_t)(r % group) * D + 2 * t;
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t w = transpose8(pack2<T>(O[d][n][2 * half] * i0, O[d][n][2 * half + 1] * i1));
+                    if (r < rows) *reinterpret_cast<uint32_t*>(dst + 16 * d + 8 * half) = w;
+                }
+        }
+    }
+};
+
+// ------------------------------------------------------------------ few rows: the blocks dealt out evenly
+// All blocks of all items and kv heads form one row of units, (item, head, block), that is cut into equal runs,
+// one per warp; a tile's start counts TILE_COST units more (its queries, its open block, its end: short sequences
+// cost more than their blocks); so sequences of any lengths keep every warp busy alike, and no warp waits for another.  A
+// warp writes the tiles whose blocks it has all; of a tile that it shares it leaves (O, m, l) in its slot
+// 0 (the tile began before its run) or 1 (it goes on after it), and kv8_join_kernel adds the slots up in order.
+// HBM bound: the codes are read once, straight into the fragments' registers.
+constexpr int DECODE_WARPS = 4, TILE_COST = 2;
+__host__ __device__ constexpr int part_floats(int nt) { return (32 + 4) * nt * 32; }  // O and m, l in the lanes' order
+
+// Where a unit lies.  sums[i]: units (of one head) of the items before chunk i of `per` items.
+struct Units {
+    int64_t total;  // units of all items, one head
+    int per;
+};
+// Blocks that item b's rows see.
+__device__ __forceinline__ int item_blocks(const Kv8Args& a, int b, int& start, int& count, int& len) {
+    item_of(a, b, start, count, len);
+    return count > 0 ? (len + count - 1) / BLK + 1 : 0;
+}
+__device__ __forceinline__ int item_units(const Kv8Args& a, int b, int& start, int& count, int& len) {
+    const int n = item_blocks(a, b, start, count, len);
+    return n ? n + TILE_COST : 0;
+}
+template <int THREADS>
+__device__ Units count_units(const Kv8Args& a, int64_t* sums) {  // sums: [THREADS + 1] in shared memory
+    __shared__ int64_t warp_sum[THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31;
+    Units u;
+    u.per = (a.items + THREADS - 1) / THREADS;
+    int64_t mine = 0;
+    for (int b = tid * u.per; b < min((tid + 1) * u.per, a.items); ++b) {
+        int s, c, l;
+        mine += item_units(a, b, s, c, l);
+    }
+    int64_t run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += y;
+    }
+    if (lane == 31) warp_sum[tid >> 5] = run;
+    __syncthreads();
+    for (int w = 0; w < (tid >> 5); ++w) run += warp_sum[w];
+    sums[tid + 1] = run;
+    if (tid == 0) sums[0] = 0;
+    __syncthreads();
+    u.total = sums[THREADS];
+    return u;
+}
+// Item of unit x (of one head; x < total) and the units before it.
+template <int THREADS>
+__device__ int find_item(const Kv8Args& a, const int64_t* sums, const Units& u, int64_t x, int64_t& before) {
+    int lo = 0, hi = THREADS - 1;  // last chunk whose sum is <= x
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (sums[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    int b = lo * u.per;
+    before = sums[lo];
+    for (;; ++b) {
+        int s, c, l;
+        const int n = item_units(a, b, s, c, l);
+        if (x < before + n || b == a.items - 1) return b;
+        before += n;
+    }
+}
+// Units of a warp's run.
+__device__ __forceinline__ int64_t run_length(int64_t units, int64_t warps) { return max((units + warps - 1) / warps, (int64_t)1); }
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(32 * DECODE_WARPS, 2) kv8_decode_kernel(AttnArgs a) {
+    __shared__ int64_t sums[32 * DECODE_WARPS + 1];
+    __shared__ uint2 queries[NT == 1 ? 1 : DECODE_WARPS][NT == 1 ? 1 : NT * 8 * 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, Hk = a.kv.c.kv_heads;
+    pdl_wait();
+    pdl_trigger();
+    const Units units = count_units<32 * DECODE_WARPS>(a.kv, sums);
+    const int64_t all = units.total * Hk, per = run_length(all, (int64_t)gridDim.x * DECODE_WARPS);
+    const int64_t w = (int64_t)blockIdx.x * DECODE_WARPS + warp, begin = w * per, end = min(begin + per, all);
+    // units run (item, head, block): the items before x units of one head take x Hk units
+    int64_t u = begin;
+    while (u < end) {
+        int64_t before;
+        const int b = find_item<32 * DECODE_WARPS>(a.kv, sums, units, u / Hk, before);
+        int start, count, len;
+        const int n = item_blocks(a.kv, b, start, count, len);
+        const int64_t inner = u - before * Hk;
+        int h = (int)(inner / (n + TILE_COST)), at_unit = (int)(inner % (n + TILE_COST));
+        // the heads of this item, as far as the run goes
+        for (; h < Hk && u < end; ++h, at_unit = 0) {
+            const int until = (int)min((int64_t)n + TILE_COST, at_unit + (end - u));
+            const int first = max(at_unit - TILE_COST, 0), last = max(until - TILE_COST, 0);
+            u += until - at_unit;
+            if (first == last) continue;  // of this tile the run has only its cost
+            int i = first;
+            Tile<T, NT> tile;
+            tile.open(queries[NT == 1 ? 0 : warp], static_cast<const T*>(a.q) + (int64_t)start * a.ldq + (int64_t)h * a.group * D, a.ldq, 0,
+                      count * a.group, len, a.group, a.factor);
+            const int whole = (len + count) / BLK;
+            // pages one block ahead, keys from the block before (a block without a page breaks the chain)
+            const int stop = min(last, whole);
+            const auto keys_of = [&](int p) { return a.kv.c.k_codes + ((int64_t)p * Hk + h) * BLK * D; };
+            int page = i < stop ? page_of(a.kv, b, i) : -1;
+            int next = i + 1 < stop ? page_of(a.kv, b, i + 1) : -1;
+            uint4 kc[4][2][2];
+            if (page >= 0) tile.load_keys(kc, keys_of(page));
+            for (; i < stop; ++i) {
+                const int later = i + 2 < stop ? page_of(a.kv, b, i + 2) : -1;
+                if (page >= 0) {
+                    const int64_t ph = (int64_t)page * Hk + h;
+                    tile.block(kc, a.kv.c.v_codes + ph * BLK * D, a.kv.c.k_scales[ph], a.kv.c.v_scales[ph], i * BLK,
+                               next >= 0 ? keys_of(next) : nullptr);
+                } else if (next >= 0) {
+                    tile.load_keys(kc, keys_of(next));
+                }
+                page = next, next = later;
+            }
+            if (last > stop) {
+                const int64_t at = ((int64_t)b * Hk + h) * BLK * D;
+                tile.tail(static_cast<const T*>(a.kv.c.k_tail) + at, static_cast<const T*>(a.kv.c.v_tail) + at,
+                          len + count - whole * BLK, whole * BLK);
+            }
+            tile.close();
+            if (first == 0 && last == n) {
+                tile.write(static_cast<T*>(a.out) + (int64_t)start * a.ldo + (int64_t)h * a.group * D, a.ldo);
+                continue;
+            }
+            float* part = a.parts + (2 * w + (first == 0 ? 1 : 0)) * part_floats(NT) + lane;
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) part[((k * 8 + d) * 4 + j) * 32] = tile.O[d][k][j];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    part[(32 * NT + 4 * k + j) * 32] = tile.m[k][j];
+                    part[(32 * NT + 4 * k + 2 + j) * 32] = tile.l[k][j];
+                }
             }
         }
-    __syncthreads();
-    for (int e = tid; e < ROWS * D; e += 32 * WARPS) {
-        const int r = e / D, c = e % D;
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < WARPS; ++i) m = fmaxf(m, part_m[i * ROWS + r]);
-        const float at = m == -INFINITY ? 0.f : m;
-        float o = 0.f, l = 0.f;
-#pragma unroll
-        for (int i = 0; i < WARPS; ++i) {
-            const float f = exp2f(part_m[i * ROWS + r] - at);
-            o = fmaf(part_o[(i * ROWS + r) * (D + 4) + c], f, o);
-            l = fmaf(part_l[i * ROWS + r], f, l);
-        }
-        part_o[r * (D + 4) + c] = o;  // (this thread alone reads column c of row r)
-        if (c == 0) cta_m[r] = m, cta_l[r] = l;
     }
-    cluster.sync();
-    for (int e = split * 32 * WARPS + tid; e < ROWS * D; e += splits * 32 * WARPS) {
-        const int r = e / D, c = e % D, row = row0 + r;
-        if (row >= rows) continue;
-        float m = -INFINITY;
-        for (int i = 0; i < splits; ++i) m = fmaxf(m, cluster.map_shared_rank(cta_m, i)[r]);
-        const float at = m == -INFINITY ? 0.f : m;
-        float o = 0.f, l = 0.f;
-        for (int i = 0; i < splits; ++i) {
-            const float f = exp2f(cluster.map_shared_rank(cta_m, i)[r] - at);
-            o = fmaf(cluster.map_shared_rank(part_o, i)[r * (D + 4) + c], f, o);
-            l = fmaf(cluster.map_shared_rank(cta_l, i)[r], f, l);
-        }
-        T y;
-        from_f32(l == 0.f ? 0.f : o / l, y);  // l = 0: no key could be read
-        static_cast<T*>(a.out)[(int64_t)(start + row / a.group) * a.ldo + ((int64_t)h * a.group + row % a.group) * D + c] = y;
-    }
-    cluster.sync();
 }
 
-template <typename T, int NT, int WARPS>
-cudaError_t launch_attention(const AttnArgs& a, int tiles, int splits, cudaStream_t stream) {
-    constexpr int ROWS = 8 * NT;
-    constexpr int JOIN = WARPS * ROWS * (D + 4) * 4 + 2 * WARPS * ROWS * 4 + 2 * ROWS * 4;
-    constexpr int FRAG = NT * 8 * 32 * 8 + ROWS * 4;
-    constexpr int SMEM = JOIN > FRAG ? JOIN : FRAG;
-    auto kernel = kv8_attention_kernel<T, NT, WARPS>;
-    static thread_local int ready = -1;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (ready != dev) {
-        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        ready = dev;
+// Adds up the slots of a tile that several warps shared, in order: a CTA per kv head, item and quarter of the
+// tile (value features 32 x .. + 31), a thread per value of the context in the slots' own layout.  Latency
+// bound: the slots' maxima and sums are turned into weights first, then all loads are independent.
+constexpr int JOIN_SLOTS = 64;  // slots at a time
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(256 * NT) kv8_join_kernel(AttnArgs a, int64_t warps) {
+    constexpr int ROWS = 8 * NT, THREADS = 256 * NT;
+    __shared__ int64_t sums[THREADS + 1];
+    __shared__ float weight[JOIN_SLOTS][ROWS], top[ROWS], total[ROWS], scale[ROWS];
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int quarter = blockIdx.x & 3, h = blockIdx.x >> 2, b = blockIdx.y, Hk = a.kv.c.kv_heads;
+    pdl_wait();
+    pdl_trigger();
+    const Units units = count_units<THREADS>(a.kv, sums);
+    const int64_t per = run_length(units.total * Hk, warps);
+    int start, count, len;
+    const int n = item_blocks(a.kv, b, start, count, len);
+    if (n == 0) return;
+    int64_t before = sums[b / units.per];
+    for (int i = b / units.per * units.per; i < b; ++i) {
+        int s, c, l;
+        before += item_units(a.kv, i, s, c, l);
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tiles * splits, a.kv.c.kv_heads, a.kv.items);
-    cfg.blockDim = dim3(32 * WARPS);
-    cfg.dynamicSmemBytes = SMEM;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {(unsigned)splits, 1, 1};
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
+    const int64_t u0 = before * Hk + (int64_t)h * (n + TILE_COST) + TILE_COST, w0 = u0 / per, w1 = (u0 + n - 1) / per;
+    if (w0 == w1) return;  // one warp had it all
+    // the tile's first warp left it in slot 1, the others in slot 0
+    auto slot = [&](int64_t w) { return a.parts + (2 * w + (w == w0 ? 1 : 0)) * part_floats(NT); };
+    // thread: n tile, feature group 2 quarter + (0, 1), value j of the fragment, lane; its row is 8 k + 2 t + (j & 1)
+    const int k = tid / 256, in = tid % 256, d = 2 * quarter + in / 128, j = in / 32 % 4;
+    const int row = 8 * k + 2 * (lane & 3) + (j & 1);
+    if (tid < ROWS) top[tid] = -INFINITY, total[tid] = 0.f;
+    float o = 0.f;
+    for (int64_t from = w0; from <= w1; from += JOIN_SLOTS) {
+        const int m = (int)min((int64_t)JOIN_SLOTS, w1 - from + 1);
+        __syncthreads();
+        for (int e = tid; e < m * ROWS; e += THREADS) {
+            const int r = e % ROWS, i = e / ROWS;
+            weight[i][r] = slot(from + i)[(32 * NT + 4 * (r / 8) + (r & 1)) * 32 + (r % 8) / 2];
+        }
+        __syncthreads();
+        if (tid < ROWS) {
+            float now = top[tid];
+            for (int i = 0; i < m; ++i) now = fmaxf(now, weight[i][tid]);
+            scale[tid] = now == -INFINITY ? 0.f : ex2(top[tid] - now);
+            top[tid] = now;
+        }
+        __syncthreads();
+        for (int e = tid; e < m * ROWS; e += THREADS) {
+            const int r = e % ROWS, i = e / ROWS;
+            weight[i][r] = top[r] == -INFINITY ? 0.f : ex2(weight[i][r] - top[r]);
+        }
+        __syncthreads();
+        if (tid < ROWS) {
+            float l = total[tid] * scale[tid];
+#pragma unroll 8
+            for (int i = 0; i < m; ++i) l = fmaf(slot(from + i)[(32 * NT + 4 * (tid / 8) + 2 + (tid & 1)) * 32 + (tid % 8) / 2], weight[i][tid], l);
+            total[tid] = l;
+        }
+        o *= scale[row];
+#pragma unroll 16
+        for (int i = 0; i < m; ++i) o = fmaf(slot(from + i)[((k * 8 + d) * 4 + j) * 32 + lane], weight[i][row], o);
+    }
+    __syncthreads();
+    // value feature 16 d + 8 (j >> 1) + g of the row
+    const float l = total[row];
+    if (row < count * a.group) {
+        T y;
+        const float x = l == 0.f ? 0.f : o / l;
+        const uint32_t two = pack2<T>(x, x);
+        y = *reinterpret_cast<const T*>(&two);
+        T* out = static_cast<T*>(a.out) + (int64_t)(start + row / a.group) * a.ldo + ((int64_t)h * a.group + row % a.group) * D;
+        out[16 * d + 8 * (j >> 1) + (lane >> 2)] = y;
+    }
+}
+
+// ------------------------------------------------------------------ many rows
+// One warp per tile of 32 query rows; the tiles of a CTA are neighbours and read the same blocks, from L1.
+constexpr int MANY_NT = 4, MANY_WARPS = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * MANY_WARPS, 2) kv8_rows_kernel(AttnArgs a) {
+    const int warp = threadIdx.x >> 5, h = blockIdx.y, b = blockIdx.z, Hk = a.kv.c.kv_heads;
+    pdl_wait();
+    pdl_trigger();
+    int start, count, len;
+    item_of(a.kv, b, start, count, len);
+    // the last tiles see the most keys: they start first
+    const int rows = count * a.group, row0 = ((int)(gridDim.x - 1 - blockIdx.x) * MANY_WARPS + warp) * 8 * MANY_NT;
+    if (row0 >= rows) return;
+    __shared__ uint2 queries[MANY_WARPS][MANY_NT * 8 * 32];
+    Tile<T, MANY_NT> tile;
+    tile.open(queries[warp], static_cast<const T*>(a.q) + (int64_t)start * a.ldq + (int64_t)h * a.group * D, a.ldq, row0, rows, len, a.group,
+              a.factor);
+    const int whole = (len + count) / BLK, blocks = (len + (min(row0 + 8 * MANY_NT, rows) - 1) / a.group) / BLK + 1;
+    for (int i = 0; i < blocks; ++i) {
+        if (i >= whole) {
+            const int64_t at = ((int64_t)b * Hk + h) * BLK * D;
+            tile.tail(static_cast<const T*>(a.kv.c.k_tail) + at, static_cast<const T*>(a.kv.c.v_tail) + at,
+                      len + count - i * BLK, i * BLK);
+            continue;
+        }
+        const int page = page_of(a.kv, b, i);
+        if (page < 0) continue;
+        const int64_t ph = (int64_t)page * Hk + h;
+        uint4 kc[4][2][2];
+        tile.load_keys(kc, a.kv.c.k_codes + ph * BLK * D);
+        tile.block(kc, a.kv.c.v_codes + ph * BLK * D, a.kv.c.k_scales[ph], a.kv.c.v_scales[ph], i * BLK, nullptr);
+    }
+    tile.close();
+    tile.write(static_cast<T*>(a.out) + (int64_t)start * a.ldo + (int64_t)h * a.group * D, a.ldo);
+}
+
+// ------------------------------------------------------------------ launches
+// n tiles of 8 rows for the dealt-out form; 0: many rows
+int decode_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 0; }
+// CTAs of the dealt-out form: as many as are resident at once, fewer when there are not that many blocks
+int64_t decode_ctas(int nt, int64_t items, int64_t heads, int64_t max_keys) {
+    (void)nt;
+    const int64_t most = (int64_t)db_num_sms() * 2;
+    const int64_t blocks = items * heads * ((max_keys + BLK - 1) / BLK + TILE_COST);
+    return std::max<int64_t>(1, std::min(most, (blocks + DECODE_WARPS - 1) / DECODE_WARPS));
+}
+
+template <typename T, int NT>
+cudaError_t launch_decode(const AttnArgs& a, int64_t max_keys, cudaStream_t stream) {
+    const int64_t ctas = decode_ctas(NT, a.kv.items, a.kv.c.kv_heads, max_keys);
+    cudaError_t e = db_launch_pdl(kv8_decode_kernel<T, NT>, dim3((unsigned)ctas), dim3(32 * DECODE_WARPS), 0, stream, a);
+    if (e != cudaSuccess) return e;
+    return db_launch_pdl(kv8_join_kernel<T, NT>, dim3(4 * a.kv.c.kv_heads, a.kv.items), dim3(256 * NT), 0, stream, a,
+                         ctas * DECODE_WARPS);
 }
 
 template <typename T>
 cudaError_t attention(const AttnArgs& a, int64_t max_keys, cudaStream_t stream) {
     const int64_t rows = (int64_t)a.kv.max_rows * a.group;
-    const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    const int64_t tiles = (rows + 8 * nt - 1) / (8 * nt);
-    const int64_t work = tiles * a.kv.c.kv_heads * a.kv.items, blocks = (max_keys + BLK - 1) / BLK;
-    // split a tile's keys while that still finds idle SMs and every warp keeps a block
-    int splits = 1;
-    while (splits < 16 && work * splits < 2 * db_num_sms() && blocks > splits * 4) splits *= 2;
-    if (tiles * splits > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    if (nt == 1) return launch_attention<T, 1, 4>(a, (int)tiles, splits, stream);
-    if (nt == 2) return launch_attention<T, 2, 4>(a, (int)tiles, splits, stream);
-    return launch_attention<T, 4, 4>(a, (int)tiles, splits, stream);
+    const int nt = decode_tiles(rows);
+    if (nt == 1) return launch_decode<T, 1>(a, max_keys, stream);
+    if (nt == 2) return launch_decode<T, 2>(a, max_keys, stream);
+    const int64_t tiles = (rows + 8 * MANY_NT * MANY_WARPS - 1) / (8 * MANY_NT * MANY_WARPS);
+    return db_launch_pdl(kv8_rows_kernel<T>, dim3((unsigned)tiles, a.kv.c.kv_heads, a.kv.items), dim3(32 * MANY_WARPS), 0,
+                         stream, a);
 }
 
 // What every call on a cache checks; fills the arguments that they share.
@@ -782,25 +1084,33 @@ int db_kv8_read(const db_kv8_cache* cache, const int32_t* lengths, int64_t items
     db::Kv8Args a{};
     const int rc = db::cache_args(cache, lengths, nullptr, items, 0, 0, "kv8 read", &a);
     if (rc) return rc;
-    if (max_keys < 0 || max_keys >= ((int64_t)1 << 31) - db::BLK || (items && max_keys && (!k || !v)))
+    if (max_keys < 0 || max_keys >= ((int64_t)1 << 31) - db::BLK || (items && max_keys && (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 15))))
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "kv8 read: bad shape");
     if (items == 0 || max_keys == 0) return DB_OK;
-    const dim3 grid((unsigned)((max_keys + db::BLK - 1) / db::BLK), cache->kv_heads, (unsigned)items);
+    const dim3 grid((unsigned)((max_keys + db::BLK - 1) / db::BLK * 2), cache->kv_heads, (unsigned)items);
+    const dim3 block(db::READ_THREADS);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cache->dtype == DB_DTYPE_F16)
-        db::kv8_read_kernel<__half><<<grid, 256, 0, s>>>(a, max_keys, k, v);
-    else
-        db::kv8_read_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, max_keys, k, v);
-    return db_cuda_status((int)cudaGetLastError(), "kv8 read");
+    const cudaError_t e = cache->dtype == DB_DTYPE_F16
+                              ? db_launch_pdl(db::kv8_read_kernel<__half>, grid, block, 0, s, a, max_keys, k, v)
+                              : db_launch_pdl(db::kv8_read_kernel<__nv_bfloat16>, grid, block, 0, s, a, max_keys, k, v);
+    return db_cuda_status((int)e, "kv8 read");
+}
+
+size_t db_kv8_attention_workspace_bytes(int64_t items, int64_t max_rows, int64_t max_keys, int64_t kv_heads,
+                                        int64_t q_heads) {
+    if (items <= 0 || max_rows <= 0 || max_keys <= 0 || kv_heads <= 0 || q_heads <= 0) return 0;
+    const int nt = db::decode_tiles(max_rows * (q_heads / kv_heads));
+    if (!nt) return 0;
+    return (size_t)db::decode_ctas(nt, items, kv_heads, max_keys) * db::DECODE_WARPS * 2 * db::part_floats(nt) * sizeof(float);
 }
 
 int db_kv8_attention(const db_kv8_cache* cache, const void* q, int64_t ldq, const int32_t* lengths,
                      const int32_t* cu_seqlens, int64_t items, int64_t rows, int64_t max_rows, int64_t max_keys,
-                     int64_t q_heads, float scale, void* out, int64_t ldo, void* stream) {
+                     int64_t q_heads, float scale, void* out, int64_t ldo, void* workspace, void* stream) {
     db::AttnArgs a{};
     const int rc = db::cache_args(cache, lengths, cu_seqlens, items, rows, max_rows, "kv8 attention", &a.kv);
     if (rc) return rc;
-    if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > 65535 || max_keys < 0)
+    if (q_heads <= 0 || q_heads % cache->kv_heads || q_heads > 65535 || max_keys <= 0)
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "kv8 attention: bad shape");
     if (items == 0 || max_rows == 0) return DB_OK;
     if (!db::rows_ok(q, ldq, q_heads * db::D) || !db::rows_ok(out, ldo, q_heads * db::D))
@@ -810,10 +1120,12 @@ int db_kv8_attention(const db_kv8_cache* cache, const void* q, int64_t ldq, cons
     a.factor = scale * 1.4426950408889634f;
     if ((int64_t)max_rows * a.group >= ((int64_t)1 << 31))
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "kv8 attention: bad shape");
-    const int64_t most = (int64_t)cache->table_width * db::BLK;
+    if (!workspace && db_kv8_attention_workspace_bytes(items, max_rows, max_keys, cache->kv_heads, q_heads))
+        return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "kv8 attention: a workspace is needed");
+    a.parts = static_cast<float*>(workspace);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = cache->dtype == DB_DTYPE_F16 ? db::attention<__half>(a, max_keys ? max_keys : most, s)
-                                                       : db::attention<__nv_bfloat16>(a, max_keys ? max_keys : most, s);
+    const cudaError_t e = cache->dtype == DB_DTYPE_F16 ? db::attention<__half>(a, max_keys, s)
+                                                       : db::attention<__nv_bfloat16>(a, max_keys, s);
     return db_cuda_status((int)e, "kv8 attention");
 }
 

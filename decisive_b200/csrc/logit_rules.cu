@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <utility>
+
 #include "../../include/decisive_b200.h"
 #include "capi_internal.h"
 #include "common.cuh"
@@ -15,6 +17,7 @@ namespace db {
 namespace {
 
 constexpr int RULE_THREADS = 512, RULE_MAX_CTAS = 16, RULE_MAX_BIASES = 1024;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr int RULE_MAX_SLICE = 49152;  // tokens of one CTA: their counters take 192 KB
 
 struct RuleArgs {
@@ -35,6 +38,7 @@ struct RuleArgs {
     int64_t ldo;
     int32_t* best;
     float* lse;
+    int narrow;  // 16-bit counters
 };
 
 // Running (largest value, its lowest index, sum of e^(value - largest)) of a set of tokens.
@@ -59,151 +63,236 @@ __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// One row per cluster, a slice of the vocabulary per CTA; HBM bound: logits in, values out.  A
-// token is looked up in detail only where a bit says that the history or a bias names it, so the
-// stream itself costs a load, a mask test, an exponential and a store.  Counters live in shared
-// memory and only those that the history names are ever touched (cleared, then counted): nothing of
-// the vocabulary's size is initialised.  The CTAs' statistics meet in the first one's shared memory.
-// VEC: logits per load (16 bytes), 1 where rows are not 16-byte aligned.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(RULE_THREADS) logit_rules_kernel(RuleArgs a) {
+// 2^x on the special-function unit
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The statistics of a warp's lanes, in every lane.
+__device__ __forceinline__ Stat join_lanes(Stat mine) {
+    Stat r;
+    r.top = mine.top;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) r.top = fmaxf(r.top, __shfl_xor_sync(0xffffffffu, r.top, o));
+    // equal tops (both infinities among them) keep their sums as they are
+    r.sum = mine.sum * (mine.top == r.top ? 1.f : ex2((mine.top - r.top) * LOG2E));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
+    r.at = (int)__reduce_min_sync(0xffffffffu, (unsigned)(mine.top == r.top ? mine.at : 0x7fffffff));
+    return r;
+}
+
+// One row per cluster, every n-th stripe of 4096 tokens per CTA (common tokens have low ids: whole slices would
+// leave the first CTA most of the history); HBM bound: logits in, values out.  The stream itself
+// costs a load, a mask test, an exponential and a store, for 8 tokens of a lane at a time; the tokens that the
+// history or a bias names are left out of it and taken afterwards from a list in the order of their ids, one
+// to a lane (handled inside the stream, a few lanes of nearly every warp would hold up the others).
+// Counters live in shared memory, 16 bits each while the history has fewer tokens than that.  The CTAs'
+// statistics meet in the first one's shared memory.
+// VEC: rows start on 16-byte boundaries.
+constexpr int RULE_STEP = 8;                         // tokens of a lane at a time
+constexpr int STRIPE = RULE_THREADS * RULE_STEP;     // tokens of a CTA at a time
+
+// x added to a running statistic; -inf adds nothing
+__device__ __forceinline__ void add_one(Stat& s, float x, int id) {
+    Stat one;
+    one.top = x == x ? x : -INFINITY;
+    one.sum = x != x ? x : x == -INFINITY ? 0.f : 1.f;
+    one.at = one.top == -INFINITY ? 0x7fffffff : id;
+    s = join(s, one);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(RULE_THREADS, 3) logit_rules_kernel(RuleArgs a) {
     extern __shared__ __align__(16) uint32_t rule_smem[];
     __shared__ Stat warp_stat[RULE_THREADS / 32];
     __shared__ Stat cta_stat[RULE_MAX_CTAS];
+    __shared__ int warp_count[RULE_THREADS / 32];
+    constexpr int WARPS = RULE_THREADS / 32;
     cg::cluster_group cluster = cg::this_cluster();
+    auto started = cluster.barrier_arrive();  // waited for before another CTA's shared memory is written
     pdl_wait();
     pdl_trigger();
-    const int tid = threadIdx.x, row = blockIdx.y;
-    const int lo = blockIdx.x * a.slice, n = min(a.slice, a.vocab - lo);  // n may be <= 0 in the last CTAs
+    const int tid = threadIdx.x, lane = tid & 31, row = blockIdx.y;
+    const int rank = blockIdx.x, ctas = gridDim.x;
+    // local token c is token id_of(c); stripes past the vocabulary are empty
+    auto id_of = [&](int c) { return ((c / STRIPE) * ctas + rank) * STRIPE + c % STRIPE; };
     const int words = a.slice / 32;
-    uint32_t* seen = rule_smem;             // tokens of the slice that the history names
+    uint32_t* seen = rule_smem;             // the CTA's tokens that the history names
     uint32_t* biased = seen + words;        // ... that a bias names
-    uint32_t* count = biased + words;       // [slice], valid where seen
-    int32_t* ids = reinterpret_cast<int32_t*>(count + a.slice);
+    uint32_t* count = biased + words;       // counters, two to a word where they have 16 bits
+    const int two = a.narrow, counters = a.slice >> two;
+    int32_t* ids = reinterpret_cast<int32_t*>(count + counters);
     float* values = reinterpret_cast<float*>(ids + a.biases);
-    for (int i = tid; i < 2 * words; i += RULE_THREADS) seen[i] = 0;
-    __syncthreads();
+    // a step's logits are on their way while the one before is worked on, the first while the history is counted
+    constexpr int LOADS = RULE_STEP * sizeof(T) / 16, EACH = 16 / sizeof(T);
+    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.ld;
+    uint4 ahead[LOADS];
+    auto load = [&](int c) {
+        if (VEC && c + RULE_STEP <= a.vocab)
+#pragma unroll
+            for (int k = 0; k < LOADS; ++k) ahead[k] = __ldcs(reinterpret_cast<const uint4*>(in + c) + k);
+    };
+    load(rank * STRIPE + tid * RULE_STEP);
+    for (int i = tid; i < (2 * words + counters) / 4; i += RULE_THREADS) reinterpret_cast<uint4*>(seen)[i] = make_uint4(0, 0, 0, 0);
     const int32_t* history = a.history + (int64_t)row * a.ldh;
     const int length = a.history ? min(max(a.history_lens ? a.history_lens[row] : a.history_cols, 0), a.history_cols) : 0;
+    __syncthreads();
     for (int i = tid; i < length; i += RULE_THREADS) {
-        const int c = (int)((unsigned)history[i] - (unsigned)lo);
-        if ((unsigned)history[i] < (unsigned)a.vocab && (unsigned)c < (unsigned)a.slice) {
-            count[c] = 0;
+        const int32_t id = history[i];
+        const unsigned stripe = (unsigned)id / STRIPE, c = stripe / ctas * STRIPE + (unsigned)id % STRIPE;
+        if ((unsigned)id < (unsigned)a.vocab && stripe % ctas == rank) {
+            atomicAdd(&count[c >> two], two && (c & 1) ? 65536u : 1u);
             atomicOr(&seen[c >> 5], 1u << (c & 31));
         }
     }
     for (int i = tid; i < a.biases; i += RULE_THREADS) {
         const int32_t id = a.bias_ids[(int64_t)row * a.biases + i];
-        const int c = (unsigned)id < (unsigned)a.vocab ? id - lo : -1;
+        const unsigned stripe = (unsigned)id / STRIPE;
+        const int c = (unsigned)id < (unsigned)a.vocab && stripe % ctas == rank ? (int)(stripe / ctas * STRIPE + (unsigned)id % STRIPE) : -1;
         ids[i] = c;
         values[i] = a.bias_values[(int64_t)row * a.biases + i];
-        if ((unsigned)c < (unsigned)a.slice) atomicOr(&biased[c >> 5], 1u << (c & 31));
-    }
-    __syncthreads();
-    for (int i = tid; i < length; i += RULE_THREADS) {
-        const int c = (int)((unsigned)history[i] - (unsigned)lo);
-        if ((unsigned)history[i] < (unsigned)a.vocab && (unsigned)c < (unsigned)a.slice) atomicAdd(&count[c], 1u);
+        if (c >= 0) atomicOr(&biased[c >> 5], 1u << (c & 31));
     }
     __syncthreads();
 
-    const float rho = a.repetition ? a.repetition[row] : 1.f;
-    const float presence = a.presence ? a.presence[row] : 0.f, frequency = a.frequency ? a.frequency[row] : 0.f;
-    const T* in = static_cast<const T*>(a.logits) + (int64_t)row * a.ld + lo;
-    float* out = a.out + (int64_t)row * a.ldo + lo;
-    const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.ldm + lo / 32 : nullptr;
+    float* out = a.out + (int64_t)row * a.ldo;
+    const uint32_t* mask = a.mask ? a.mask + (int64_t)row * a.ldm : nullptr;
     Stat mine = {-INFINITY, 0.f, 0x7fffffff};
-    for (int c0 = tid * VEC; c0 < n; c0 += RULE_THREADS * VEC) {
-        float x[VEC];
-        if (VEC > 1 && c0 + VEC <= n) {
-            const uint4 r = __ldcs(reinterpret_cast<const uint4*>(in + c0));
-            const T* p = reinterpret_cast<const T*>(&r);
+    for (int c0 = tid * RULE_STEP, v0 = rank * STRIPE + c0; v0 < a.vocab; c0 += STRIPE, v0 += ctas * STRIPE) {
+        const bool whole = VEC && v0 + RULE_STEP <= a.vocab;
+        float x[RULE_STEP];
+        if (whole) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[i] = to_f32(p[i]);
+            for (int k = 0; k < LOADS; ++k) {
+                const T* p = reinterpret_cast<const T*>(&ahead[k]);
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) x[k * EACH + i] = to_f32(p[i]);
+            }
+            load(v0 + ctas * STRIPE);
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) x[i] = c0 + i < n ? to_f32(in[c0 + i]) : -INFINITY;
+            for (int i = 0; i < RULE_STEP; ++i) x[i] = v0 + i < a.vocab ? to_f32(in[v0 + i]) : -INFINITY;
         }
-        const int shift = c0 & 31;
-        const uint32_t bits = VEC == 32 ? 0xffffffffu : (1u << VEC) - 1;
-        const uint32_t allowed = mask ? (mask[c0 >> 5] >> shift) & bits : bits;
-        const uint32_t h = (seen[c0 >> 5] >> shift) & bits, w = (biased[c0 >> 5] >> shift) & bits;
-        if (h | w) {
+        const int word = c0 >> 5, shift = c0 & 31;
+        const uint32_t named = seen[word] | biased[word];
+        const uint32_t allowed = (mask ? mask[v0 >> 5] & ~named : ~named) >> shift;
+        const uint32_t left = (named >> shift) & 0xffu;
+        float top = -INFINITY;
+        if (!left && whole) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (h >> i & 1) {
-                    x[i] = x[i] > 0.f ? __fdiv_rn(x[i], rho) : __fmul_rn(x[i], rho);
-                    x[i] = __fsub_rn(x[i], __fadd_rn(presence, __fmul_rn(frequency, (float)count[c0 + i])));
-                }
-                if (w >> i & 1)
-                    for (int j = 0; j < a.biases; ++j)
-                        if (ids[j] == c0 + i) x[i] = __fadd_rn(x[i], values[j]);
+            for (int i = 0; i < RULE_STEP; ++i) x[i] = (allowed >> i & 1) ? x[i] : -INFINITY;
+#pragma unroll
+            for (int i = 0; i < RULE_STEP; i += 4)
+                __stcs(reinterpret_cast<float4*>(out + v0 + i), make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < RULE_STEP; ++i) {
+                x[i] = (allowed >> i & 1) ? x[i] : -INFINITY;
+                if (!(left >> i & 1) && v0 + i < a.vocab) out[v0 + i] = x[i];
             }
         }
-        float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            if (!(allowed >> i & 1)) x[i] = -INFINITY;
-            top = fmaxf(top, x[i]);
+        for (int i = 0; i < RULE_STEP; ++i) top = fmaxf(top, x[i]);
+        if (top > mine.top) {
+            mine.sum = top == INFINITY ? mine.sum * 0.f : mine.sum * ex2((mine.top - top) * LOG2E);
+            mine.top = top;
+            int at = 0;
+#pragma unroll
+            for (int i = RULE_STEP - 1; i >= 0; --i) at = x[i] == top ? i : at;
+            mine.at = v0 + at;
         }
-        if (VEC > 1 && c0 + VEC <= n) {
+        if (fabsf(mine.top) < 1e4f) {
+            const float base = mine.top * LOG2E;  // its rounding is a common factor: 1e4 x 2^-24 at most
 #pragma unroll
-            for (int i = 0; i < VEC; i += 4)
-                __stcs(reinterpret_cast<float4*>(out + c0 + i), make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
+            for (int i = 0; i < RULE_STEP; ++i) mine.sum += ex2(fmaf(x[i], LOG2E, -base));
         } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (c0 + i < n) out[c0 + i] = x[i];
-        }
-        if (top > mine.top) {
-            mine.sum = top == INFINITY ? mine.sum * 0.f : mine.sum * exp2f((mine.top - top) * 1.4426950408889634f);
-            mine.top = top;
-#pragma unroll
-            for (int i = VEC - 1; i >= 0; --i)
-                if (x[i] == top) mine.at = lo + c0 + i;
-        }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            // the largest value counts 1 (+inf too), a token that is out 0, a NaN itself
-            const float e = exp2f((x[i] - mine.top) * 1.4426950408889634f);
-            mine.sum += x[i] == -INFINITY ? 0.f : x[i] == mine.top ? 1.f : e;
+            for (int i = 0; i < RULE_STEP; ++i)
+                mine.sum += x[i] != x[i] ? x[i] : x[i] == mine.top ? (mine.top == -INFINITY ? 0.f : 1.f) : ex2((x[i] - mine.top) * LOG2E);
         }
     }
+
+    // the named tokens: their places in the order of ids by a scan over the words' bit counts, then one to a lane
+    int bits = 0;
+    const int each = (words + RULE_THREADS - 1) / RULE_THREADS, w0 = tid * each, w1 = min(w0 + each, words);
+    for (int i = w0; i < w1; ++i) bits += __popc(seen[i] | biased[i]);
+    int place = bits;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        Stat other;
-        other.top = __shfl_xor_sync(0xffffffffu, mine.top, o);
-        other.sum = __shfl_xor_sync(0xffffffffu, mine.sum, o);
-        other.at = __shfl_xor_sync(0xffffffffu, mine.at, o);
-        // lower lane first on both sides, so the two halves of a pair agree to the bit
-        mine = (tid & o) ? join(other, mine) : join(mine, other);
+    for (int o = 1; o < 32; o *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, place, o);
+        if (lane >= o) place += y;
     }
-    if ((tid & 31) == 0) warp_stat[tid >> 5] = mine;
-    cluster.sync();  // also: the first CTA's shared memory is there to be written
-    if (tid == 0) {
-        Stat all = warp_stat[0];
-        for (int i = 1; i < RULE_THREADS / 32; ++i) all = join(all, warp_stat[i]);
-        *cluster.map_shared_rank(&cta_stat[cluster.block_rank()], 0) = all;
+    if (lane == 31) warp_count[tid >> 5] = place;
+    __syncthreads();
+    int total = 0;
+    for (int i = 0; i < WARPS; ++i) {
+        if (i == (tid >> 5)) place += total;
+        total += warp_count[i];
     }
-    cluster.sync();
-    if (cluster.block_rank() == 0 && tid == 0) {
-        Stat all = cta_stat[0];
-        for (int i = 1; i < (int)cluster.num_blocks(); ++i) all = join(all, cta_stat[i]);
-        if (a.best) a.best[row] = all.top == -INFINITY ? -1 : all.at;
-        // nothing allowed: log 0 = -inf (and NaN where a NaN was allowed)
-        if (a.lse) a.lse[row] = all.top == -INFINITY ? (all.sum == 0.f ? -INFINITY : all.sum) : all.top + logf(all.sum);
+    place -= bits;
+    int32_t* list = reinterpret_cast<int32_t*>(values + a.biases);  // RULE_THREADS entries at a time
+    const float rho = a.repetition ? a.repetition[row] : 1.f;
+    const float presence = a.presence ? a.presence[row] : 0.f, frequency = a.frequency ? a.frequency[row] : 0.f;
+    for (int from = 0; from < total; from += RULE_THREADS) {
+        if (from) __syncthreads();  // the list has been read
+        int at = place;
+        if (place < from + RULE_THREADS && place + bits > from)
+            for (int i = w0; i < w1; ++i)
+                for (uint32_t rest = seen[i] | biased[i]; rest; rest &= rest - 1, ++at)
+                    if (at >= from && at < from + RULE_THREADS) list[at - from] = 32 * i + __ffs(rest) - 1;
+        __syncthreads();
+        if (from + tid >= total) continue;
+        const int c = list[tid], id = id_of(c);
+        float y = to_f32(in[id]);
+        if (seen[c >> 5] >> (c & 31) & 1) {
+            const uint32_t pair = count[c >> two], times = two ? (c & 1 ? pair >> 16 : pair & 0xffffu) : pair;
+            y = y > 0.f ? __fdiv_rn(y, rho) : __fmul_rn(y, rho);
+            y = __fsub_rn(y, __fadd_rn(presence, __fmul_rn(frequency, (float)times)));
+        }
+        if (biased[c >> 5] >> (c & 31) & 1)
+            for (int j = 0; j < a.biases; ++j)
+                if (ids[j] == c) y = __fadd_rn(y, values[j]);
+        if (mask && !(mask[id >> 5] >> (id & 31) & 1)) y = -INFINITY;
+        out[id] = y;
+        add_one(mine, y, id);
+    }
+    mine = join_lanes(mine);
+    if (lane == 0) warp_stat[tid >> 5] = mine;
+    __syncthreads();
+    cluster.barrier_wait(std::move(started));
+    const Stat none = {-INFINITY, 0.f, 0x7fffffff};
+    if (tid < 32) {
+        const Stat all = join_lanes(lane < WARPS ? warp_stat[lane] : none);
+        if (lane == 0) *cluster.map_shared_rank(&cta_stat[cluster.block_rank()], 0) = all;
+    }
+    // the others are done once theirs is on its way; the first one waits for all
+    auto written = cluster.barrier_arrive();
+    if (cluster.block_rank() != 0) return;
+    cluster.barrier_wait(std::move(written));
+    if (tid < 32) {
+        const Stat all = join_lanes(lane < (int)cluster.num_blocks() ? cta_stat[lane] : none);
+        if (lane == 0) {
+            if (a.best) a.best[row] = all.top == -INFINITY ? -1 : all.at;
+            // nothing allowed: log 0 = -inf (and NaN where a NaN was allowed)
+            if (a.lse) a.lse[row] = all.top == -INFINITY ? (all.sum == 0.f ? -INFINITY : all.sum) : all.top + logf(all.sum);
+        }
     }
 }
 
 template <typename T>
 cudaError_t launch(RuleArgs a, int rows, cudaStream_t stream) {
-    constexpr int VEC = 16 / sizeof(T);
     const bool vec = !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15) && !((a.ld * sizeof(T)) & 15) && !((a.ldo * 4) & 15);
-    // CTAs per row: at least 2048 tokens each, all 16 for a vocabulary of 32 K tokens and more
+    // CTAs per row: for few rows one per stripe, up to 16; for many only as many as fill the SMs with three
+    // each, so that a CTA's fixed work is spread over more tokens
+    const int stripes = (a.vocab + STRIPE - 1) / STRIPE, fill = 3 * db_num_sms();
     int ctas = 1;
-    while (ctas < RULE_MAX_CTAS && (a.vocab + ctas - 1) / ctas > 2048) ctas *= 2;
-    a.slice = ((a.vocab + ctas - 1) / ctas + 31) / 32 * 32;
-    const size_t smem = (size_t)a.slice / 32 * 8 + (size_t)a.slice * 4 + (size_t)a.biases * 8;
-    auto kernel = vec ? logit_rules_kernel<T, VEC> : logit_rules_kernel<T, 1>;
+    while (ctas < RULE_MAX_CTAS && ctas < stripes && (stripes > ctas * (RULE_MAX_SLICE / 2 / STRIPE) || rows * ctas < fill)) ctas *= 2;
+    a.slice = (stripes + ctas - 1) / ctas * STRIPE;
+    a.narrow = a.history_cols < 65536;
+    const size_t smem = (size_t)a.slice / 32 * 8 + (size_t)(a.slice >> a.narrow) * 4 + (size_t)a.biases * 8 + RULE_THREADS * 4;
+    auto kernel = vec ? logit_rules_kernel<T, true> : logit_rules_kernel<T, false>;
     static thread_local int ready_device[2] = {-1, -1};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);

@@ -260,7 +260,7 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
 
 /* ---- generation operators.  Packed rows: `items` sequences' rows lie one after another; cu_seqlens
  * (device, int32 [items + 1]) gives their offsets, NULL means equal items (rows = items * max_len).
- * max_len / max_rows is the longest item's rows (longer items are cut to it; it sizes the launch).
+ * max_len / max_rows is the longest item's rows; it sizes the launch (the cache entries cut longer items to it).
  * Row strides are in elements; rows of 16-bit tensors start on 16-byte boundaries (stride % 8 == 0).
  * head_dim is 128; other values give DB_ERR_UNSUPPORTED.  Device-side offsets, lengths and page numbers outside
  * their tensors are brought back inside or skipped; the cache entries note them in the error word
@@ -311,12 +311,15 @@ int db_kv8_append(const db_kv8_cache *cache, const void *k, int64_t ldk, const v
                   void *stream);
 /* Attention over the cache after an append: row i of item b (position p = lengths[b] + i, the same
  * lengths as the append's) sees the cached keys 0 .. p: out = softmax(scale q.k) v.  q, out
- * [rows, q_heads, 128]; query head h uses kv head h / (q_heads / kv_heads).  max_keys: an upper bound on
- * lengths + rows over the items, which sizes the split of the keys (0: the table's width).  A row that
- * can read no key (its pages are missing) is 0. */
+ * [rows, q_heads, 128]; query head h uses kv head h / (q_heads / kv_heads).  max_keys > 0: the caller's
+ * estimate of the longest item's keys (table_width * 64 when nothing better is known); it sizes the launch
+ * and the workspace and changes no result's meaning.  A row that can read no key (its pages are missing) is
+ * 0.  workspace: device bytes from db_kv8_attention_workspace_bytes (may be NULL where that is 0). */
+size_t db_kv8_attention_workspace_bytes(int64_t items, int64_t max_rows, int64_t max_keys, int64_t kv_heads,
+                                        int64_t q_heads);
 int db_kv8_attention(const db_kv8_cache *cache, const void *q, int64_t ldq, const int32_t *lengths,
                      const int32_t *cu_seqlens, int64_t items, int64_t rows, int64_t max_rows, int64_t max_keys,
-                     int64_t q_heads, float scale, void *out, int64_t ldo, void *stream);
+                     int64_t q_heads, float scale, void *out, int64_t ldo, void *workspace, void *stream);
 /* The cached values of tokens 0 .. max_keys - 1 (0 from lengths[b] on): k, v f32 [items, max_keys,
  * kv_heads, 128]. */
 int db_kv8_read(const db_kv8_cache *cache, const int32_t *lengths, int64_t items, int64_t max_keys, float *k, float *v,
