@@ -264,30 +264,44 @@ def attention_decoder(q16, k16, v16, items: int, q_heads: int, kv_heads: int, kp
 
 
 # ------------------------------------------------------------------ generation operators
-def _heads(name, x, dtype=None, device=None):
-    """A packed tensor [rows, heads, 128] whose rows may be strided (a view of a wider projection); returns
-    its row stride."""
-    if x.dim() != 3 or x.shape[2] != 128 or x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != 128):
+# A decode step spends microseconds in these wrappers, so their checks read each tensor's shape and
+# strides once.
+def _heads(name, x, dtype, device: int):
+    """A packed tensor [rows, heads, 128] whose rows may be strided (a view of a wider projection) ->
+    (rows, heads, row stride)."""
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != 128:
+        raise ValueError(f"{name}: a tensor [rows, heads, 128] is wanted")
+    rows, heads, _ = shape
+    ld, sh, sd = x.stride()
+    if sd != 1 or (sh != 128 and heads > 1):
         raise ValueError(f"{name}: a tensor [rows, heads, 128] with dense rows is wanted")
-    if (dtype is not None and x.dtype != dtype) or (device is not None and x.device != device) or not x.is_cuda:
+    if x.dtype != dtype or x.get_device() != device:
         raise ValueError(f"{name}: type or device differs from the other tensors'")
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1] * 128
+    return rows, heads, ld if rows > 1 else heads * 128
 
 
-def _array(name, x, dtype, shape, device):
-    """A dense device tensor of one type and shape; None passes."""
-    if x is not None and (x.dtype != dtype or tuple(x.shape) != tuple(shape) or not x.is_contiguous() or
-                          x.device != device):
-        raise ValueError(f"{name}: a dense {dtype} tensor {list(shape)} on {device} is wanted")
-    return x.data_ptr() if x is not None else None
+def _array(name, x, dtype, shape, device: int):
+    """The address of a dense device tensor of one type and shape; None passes."""
+    if x is None:
+        return None
+    if x.dtype != dtype or x.shape != shape or not x.is_contiguous() or x.get_device() != device:
+        raise ValueError(f"{name}: a dense {dtype} tensor {list(shape)} on device {device} is wanted")
+    return x.data_ptr()
 
 
-def _raw_stream(device):
+def _device(name, x) -> int:
+    if not x.is_cuda:
+        raise ValueError(f"{name}: a tensor on a device is wanted")
+    return x.get_device()
+
+
+def _raw_stream(device: int):
     import torch
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
-def _code(dtype, name):
+def _code16(dtype, name):
     import torch
     if dtype == torch.bfloat16:
         return 2
@@ -296,8 +310,11 @@ def _code(dtype, name):
     raise ValueError(f"{name}: float16 or bfloat16 is wanted")
 
 
+DELTA_STEP_TOKENS = 16  # DB_DELTA_STEP_TOKENS: up to here items need no workspace
+
+
 def gated_delta(q, k, v, g, beta, items: int = 1, cu_seqlens=None, max_len: int | None = None, state=None,
-                scale: float | None = None, norm_eps: float | None = 1e-6, state_out=None, out=None):
+                scale: float = 128 ** -0.5, norm_eps: float | None = 1e-6, state_out=None, out=None):
     """The gated delta rule over packed sequences -> (out [rows, v_heads, 128], states after the last rows
     f32 [items, v_heads, 128 (value), 128 (key)]).
 
@@ -306,45 +323,53 @@ def gated_delta(q, k, v, g, beta, items: int = 1, cu_seqlens=None, max_len: int 
     device) the items are equal; with it max_len is the longest item's rows (default: all rows, which
     is only slower).  state: f32 [items, v_heads, 128, 128], or with one item in front a kept state that
     every item starts from; None: zeros.  state_out may be state itself.  q and k are divided by their
-    lengths unless norm_eps is None; scale defaults to 128^-0.5."""
+    lengths unless norm_eps is None.  A value that is not finite makes the outputs of its value feature (in
+    v) or head (elsewhere) NaN, from the start of its block of 64 tokens at the earliest."""
     import torch
-    dev, dt = v.device, v.dtype
-    code = _code(dt, "gated_delta")
-    ldq, ldk, ldv = _heads("q", q, dt, dev), _heads("k", k, dt, dev), _heads("v", v, dt, dev)
-    rows, hv, hk = v.shape[0], v.shape[1], k.shape[1]
-    if q.shape != k.shape or k.shape[0] != rows:
+    dt, dev = v.dtype, _device("v", v)
+    code = _code16(dt, "gated_delta")
+    rows, hv, ldv = _heads("v", v, dt, dev)
+    rows_k, hk, ldk = _heads("k", k, dt, dev)
+    rows_q, hq, ldq = _heads("q", q, dt, dev)
+    if rows_k != rows or rows_q != rows or hq != hk:
         raise ValueError("gated_delta: q, k and v differ in their rows or heads")
+    f32, ld = torch.float32, []
     for name, x in (("g", g), ("beta", beta)):
-        if x.shape != (rows, hv) or x.dtype != torch.float32 or x.stride(1) != 1 and hv > 1 or x.device != dev:
+        sr, sh = x.stride() if x.dim() == 2 else (0, 0)
+        if x.shape != (rows, hv) or x.dtype != f32 or (sh != 1 and hv > 1) or x.get_device() != dev:
             raise ValueError(f"{name}: a float32 tensor [rows, v_heads] with dense rows is wanted")
+        ld.append(sr if rows > 1 else hv)
+    cu = None
     if cu_seqlens is not None:
-        _array("cu_seqlens", cu_seqlens, torch.int32, (items + 1,), dev)
+        cu = _array("cu_seqlens", cu_seqlens, torch.int32, (items + 1,), dev)
         max_len = rows if max_len is None else min(max_len, rows)
     else:
         if items and rows % items:
             raise ValueError("gated_delta: rows do not divide into equal items")
         max_len = rows // items if items else 0
-    stride = 0
+    stride, si = 0, None
     if state is not None:
-        one = state.shape[0] == 1
-        _array("state", state, torch.float32, (1 if one else items, hv, 128, 128), dev)
+        one = len(state.shape) == 4 and state.shape[0] == 1
+        si = _array("state", state, f32, (1 if one else items, hv, 128, 128), dev)
         stride = 0 if one and items != 1 else hv * 128 * 128
     if state_out is None:
-        state_out = torch.empty((items, hv, 128, 128), dtype=torch.float32, device=dev)
-    so = _array("state_out", state_out, torch.float32, (items, hv, 128, 128), dev)
+        state_out = g.new_empty((items, hv, 128, 128))
+        so = state_out.data_ptr()
+    else:
+        so = _array("state_out", state_out, f32, (items, hv, 128, 128), dev)
     if out is None:
-        out = torch.empty((rows, hv, 128), dtype=dt, device=dev)
-    ldo = _heads("out", out, dt, dev)
-    if out.shape != (rows, hv, 128):
-        raise ValueError("gated_delta: out differs from v in its shape")
-    lib = load()
-    need = lib.db_gated_delta_workspace_bytes(items, rows, max_len, hk, hv, code)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        out, ldo = v.new_empty((rows, hv, 128)), hv * 128
+    else:
+        rows_o, ho, ldo = _heads("out", out, dt, dev)
+        if rows_o != rows or ho != hv:
+            raise ValueError("gated_delta: out differs from v in its shape")
+    lib, ws = load(), None
+    if max_len > DELTA_STEP_TOKENS:
+        need = lib.db_gated_delta_workspace_bytes(items, rows, max_len, hk, hv, code)
+        ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
     check(lib.db_gated_delta(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ldq, ldk, ldv, g.data_ptr(),
-                             beta.data_ptr(), g.stride(0) if rows > 1 else hv, beta.stride(0) if rows > 1 else hv,
-                             cu_seqlens.data_ptr() if cu_seqlens is not None else None, items, rows, max_len, hk, hv,
-                             128, 128 ** -0.5 if scale is None else scale, -1.0 if norm_eps is None else norm_eps,
-                             state.data_ptr() if state is not None else None, stride, so, out.data_ptr(), ldo,
+                             beta.data_ptr(), ld[0], ld[1], cu, items, rows, max_len, hk, hv, 128, scale,
+                             -1.0 if norm_eps is None else norm_eps, si, stride, so, out.data_ptr(), ldo,
                              ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
     return out, state_out
 
@@ -358,24 +383,29 @@ class KvCache8:
     bf16; page_table int32 [sequences, table_width]: the page of each block, the caller's to fill."""
 
     BLOCK = 64
+    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "page_table", "dtype", "device",
+                 "kv_heads", "table_width", "_c", "ref")
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, page_table):
         import torch
-        dev = k_tail.device
+        dev, dt, f32 = _device("k_tail", k_tail), k_tail.dtype, torch.float32
+        if len(k_scales.shape) != 2 or len(page_table.shape) != 2:
+            raise ValueError("KvCache8: k_scales [pages, kv_heads] and page_table [sequences, width] are wanted")
         pages, heads = k_scales.shape
         sequences, width = page_table.shape
-        code = _code(k_tail.dtype, "KvCache8")
+        code = _code16(dt, "KvCache8")
         self._c = _lib.KvCache8(
             _array("k_codes", k_codes, torch.int8, (pages, heads, 64, 128), dev),
-            _array("k_scales", k_scales, torch.float32, (pages, heads), dev),
+            _array("k_scales", k_scales, f32, (pages, heads), dev),
             _array("v_codes", v_codes, torch.int8, (pages, heads, 128, 64), dev),
-            _array("v_scales", v_scales, torch.float32, (pages, heads), dev),
-            _array("k_tail", k_tail, k_tail.dtype, (sequences, heads, 64, 128), dev),
-            _array("v_tail", v_tail, k_tail.dtype, (sequences, heads, 128, 64), dev),
+            _array("v_scales", v_scales, f32, (pages, heads), dev),
+            _array("k_tail", k_tail, dt, (sequences, heads, 64, 128), dev),
+            _array("v_tail", v_tail, dt, (sequences, heads, 128, 64), dev),
             _array("page_table", page_table, torch.int32, (sequences, width), dev),
             pages, width, sequences, heads, 128, code)
         self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
         self.k_tail, self.v_tail, self.page_table = k_tail, v_tail, page_table
+        self.dtype, self.device, self.kv_heads, self.table_width = dt, dev, heads, width
         self.ref = C.byref(self._c)
 
     @classmethod
@@ -394,52 +424,55 @@ class KvCache8:
                    z(dtype, sequences, kv_heads, 64, 128), z(dtype, sequences, kv_heads, 128, 64), table)
 
 
-def _kv8_rows(cache, x, lengths, cu_seqlens, max_rows):
+def _kv8_items(device: int, rows: int, lengths, cu_seqlens, max_rows):
+    """(items, their most rows, addresses of lengths and cu_seqlens)."""
     import torch
-    dev, rows, items = cache.k_tail.device, x.shape[0], lengths.shape[0]
-    _array("lengths", lengths, torch.int32, (items,), dev)
+    if len(lengths.shape) != 1:
+        raise ValueError("lengths: a tensor [items] is wanted")
+    items = lengths.shape[0]
+    ln = _array("lengths", lengths, torch.int32, (items,), device)
     if cu_seqlens is not None:
-        _array("cu_seqlens", cu_seqlens, torch.int32, (items + 1,), dev)
-        return items, rows, rows if max_rows is None else min(max_rows, rows), cu_seqlens.data_ptr()
+        cu = _array("cu_seqlens", cu_seqlens, torch.int32, (items + 1,), device)
+        return items, rows if max_rows is None else min(max_rows, rows), ln, cu
     if items and rows % items:
         raise ValueError("kv8: rows do not divide into equal items")
-    return items, rows, rows // items if items else 0, None
+    return items, rows // items if items else 0, ln, None
 
 
 def kv8_append(cache: KvCache8, k, v, lengths, cu_seqlens=None, max_rows: int | None = None) -> None:
     """Writes the items' new rows (k, v [rows, kv_heads, 128]) at positions lengths[b] (int32, device) on;
     blocks that fill up are quantised.  The lengths stay as they are: advance them once every layer has
     taken the step.  cu_seqlens and max_rows as in gated_delta."""
-    dt, dev = cache.k_tail.dtype, cache.k_tail.device
-    ldk, ldv = _heads("k", k, dt, dev), _heads("v", v, dt, dev)
-    if k.shape != v.shape or k.shape[1] != cache.k_tail.shape[1]:
+    dt, dev = cache.dtype, cache.device
+    rows, heads, ldk = _heads("k", k, dt, dev)
+    rows_v, heads_v, ldv = _heads("v", v, dt, dev)
+    if rows_v != rows or heads_v != heads or heads != cache.kv_heads:
         raise ValueError("kv8_append: k or v differs from the cache in its heads or rows")
-    items, rows, most, cu = _kv8_rows(cache, k, lengths, cu_seqlens, max_rows)
-    check(load().db_kv8_append(cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, lengths.data_ptr(), cu, items, rows,
-                               most, _raw_stream(dev)))
+    items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)
+    check(load().db_kv8_append(cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, ln, cu, items, rows, most,
+                               _raw_stream(dev)))
 
 
 def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | None = None,
-                  max_keys: int | None = None, scale: float | None = None, out=None):
+                  max_keys: int | None = None, scale: float = 128 ** -0.5, out=None):
     """Attention over the cache after the append of the same rows: row i of item b sees the cached keys
     0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: the longest item's keys, as far as the caller
     knows (default: the table's width); it only sizes the launch and the workspace."""
     import torch
-    dt, dev = cache.k_tail.dtype, cache.k_tail.device
-    ldq = _heads("q", q, dt, dev)
-    items, rows, most, cu = _kv8_rows(cache, q, lengths, cu_seqlens, max_rows)
+    dt, dev = cache.dtype, cache.device
+    rows, heads, ldq = _heads("q", q, dt, dev)
+    items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=dev)
-    ldo = _heads("out", out, dt, dev)
-    if out.shape != q.shape:
-        raise ValueError("kv8_attention: out differs from q in its shape")
-    lib, heads = load(), q.shape[1]
-    keys = max(1, max_keys or cache.page_table.shape[1] * 64)
-    need = lib.db_kv8_attention_workspace_bytes(items, most, keys, cache.k_tail.shape[1], heads)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(lib.db_kv8_attention(cache.ref, q.data_ptr(), ldq, lengths.data_ptr(), cu, items, rows, most, keys, heads,
-                               128 ** -0.5 if scale is None else scale, out.data_ptr(), ldo,
-                               ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
+        out, ldo = q.new_empty((rows, heads, 128)), heads * 128
+    else:
+        rows_o, heads_o, ldo = _heads("out", out, dt, dev)
+        if rows_o != rows or heads_o != heads:
+            raise ValueError("kv8_attention: out differs from q in its shape")
+    lib, keys = load(), max(1, max_keys or cache.table_width * 64)
+    need = lib.db_kv8_attention_workspace_bytes(items, most, keys, cache.kv_heads, heads)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    check(lib.db_kv8_attention(cache.ref, q.data_ptr(), ldq, ln, cu, items, rows, most, keys, heads, scale,
+                               out.data_ptr(), ldo, ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
     return out
 
 
@@ -447,12 +480,11 @@ def kv8_read(cache: KvCache8, lengths, max_keys: int):
     """The cached keys and values of tokens 0 .. max_keys - 1, f32 [items, max_keys, kv_heads, 128] each
     (0 from lengths[b] on)."""
     import torch
-    dev, items = cache.k_tail.device, lengths.shape[0]
-    _array("lengths", lengths, torch.int32, (items,), dev)
-    k, v = (torch.empty((items, max_keys, cache.k_tail.shape[1], 128), dtype=torch.float32, device=dev)
+    dev = cache.device
+    items, _, ln, _ = _kv8_items(dev, 0, lengths, None, None)
+    k, v = (torch.empty((items, max_keys, cache.kv_heads, 128), dtype=torch.float32, device=cache.k_tail.device)
             for _ in range(2))
-    check(load().db_kv8_read(cache.ref, lengths.data_ptr(), items, max_keys, k.data_ptr(), v.data_ptr(),
-                             _raw_stream(dev)))
+    check(load().db_kv8_read(cache.ref, ln, items, max_keys, k.data_ptr(), v.data_ptr(), _raw_stream(dev)))
     return k, v
 
 
@@ -466,33 +498,34 @@ def logit_rules(logits, history=None, history_lengths=None, repetition=None, pre
     bit id % 32 of word id / 32 set where a token is allowed.  A row with nothing allowed has best -1
     and lse -inf.  out may be f32 logits themselves."""
     import torch
+    f32, i32, dt = torch.float32, torch.int32, logits.dtype
+    if len(logits.shape) != 2:
+        raise ValueError("logit_rules: logits [rows, vocab] are wanted")
     rows, vocab = logits.shape
-    dev = logits.device
-    if vocab > 1 and logits.stride(1) != 1 or not logits.is_cuda:
-        raise ValueError("logit_rules: logits with dense rows on a device are wanted")
-    if str(logits.dtype).split(".")[1] not in DTYPES:
+    ld, step = logits.stride()
+    dev = _device("logits", logits)
+    if vocab > 1 and step != 1:
+        raise ValueError("logit_rules: logits with dense rows are wanted")
+    if dt != f32 and dt != torch.float16 and dt != torch.bfloat16:
         raise ValueError("logit_rules: logits are float32, float16 or bfloat16")
-    f32, i32 = torch.float32, torch.int32
     cols = history.shape[1] if history is not None else 0
-    hist = _array("history", history, i32, (rows, cols), dev)
-    lens = _array("history_lengths", history_lengths, i32, (rows,), dev)
-    pen = [_array(n, x, f32, (rows,), dev)
-           for n, x in (("repetition", repetition), ("presence", presence), ("frequency", frequency))]
     biases = bias_ids.shape[1] if bias_ids is not None else 0
-    ids = _array("bias_ids", bias_ids, i32, (rows, biases), dev)
-    vals = _array("bias_values", bias_values, f32, (rows, biases), dev)
-    words = (vocab + 31) // 32
-    bits = _array("mask", mask, i32, (rows, words), dev)
+    words, one = (vocab + 31) // 32, (rows,)
     if out is None:
-        out = torch.empty((rows, vocab), dtype=f32, device=dev)
-    elif out.shape != logits.shape or out.dtype != f32 or vocab > 1 and out.stride(1) != 1 or out.device != dev:
-        raise ValueError("logit_rules: out is f32 with dense rows, of the logits' shape")
-    best = torch.empty(rows, dtype=i32, device=dev)
-    lse = torch.empty(rows, dtype=f32, device=dev)
-    check(load().db_logit_rules(logits.data_ptr(), DTYPES[str(logits.dtype).split(".")[1]],
-                                logits.stride(0) if rows > 1 else vocab, rows, vocab, hist, cols, lens, cols, *pen, ids,
-                                vals, biases, bits, words, out.data_ptr(), out.stride(0) if rows > 1 else vocab,
-                                best.data_ptr(), lse.data_ptr(), _raw_stream(dev)))
+        out, ldo = torch.empty((rows, vocab), dtype=f32, device=logits.device), vocab
+    else:
+        ldo, step = out.stride() if len(out.shape) == 2 else (0, 0)
+        if out.shape != logits.shape or out.dtype != f32 or (vocab > 1 and step != 1) or out.get_device() != dev:
+            raise ValueError("logit_rules: out is f32 with dense rows, of the logits' shape")
+    best, lse = out.new_empty(one, dtype=i32), out.new_empty(one)
+    check(load().db_logit_rules(
+        logits.data_ptr(), 0 if dt == f32 else 1 if dt == torch.float16 else 2, ld if rows > 1 else vocab, rows, vocab,
+        _array("history", history, i32, (rows, cols), dev), cols,
+        _array("history_lengths", history_lengths, i32, one, dev), cols, _array("repetition", repetition, f32, one, dev),
+        _array("presence", presence, f32, one, dev), _array("frequency", frequency, f32, one, dev),
+        _array("bias_ids", bias_ids, i32, (rows, biases), dev),
+        _array("bias_values", bias_values, f32, (rows, biases), dev), biases, _array("mask", mask, i32, (rows, words), dev),
+        words, out.data_ptr(), ldo if rows > 1 else vocab, best.data_ptr(), lse.data_ptr(), _raw_stream(dev)))
     return out, best, lse
 
 

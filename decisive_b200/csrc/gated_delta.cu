@@ -789,7 +789,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1) delta_chunk_kernel(DeltaArgs a,
 }
 
 // Up to this many tokens per item the recurrence is faster than a chunk.
-constexpr int STEP_TOKENS = 16;
+constexpr int STEP_TOKENS = DB_DELTA_STEP_TOKENS;
 
 template <typename T, int WARPS>
 cudaError_t launch_chunks(const DeltaArgs& a, const ChunkSpace& w, cudaStream_t stream) {

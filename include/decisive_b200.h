@@ -276,7 +276,9 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
  * per item, state_stride floats apart (0: one kept prefix state for all items; NULL: zeros); state_out
  * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own).
  * An item without rows passes its state on.  out [rows, v_heads, 128] in v's type.  workspace: device
- * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0). */
+ * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0; it is 0 up to max_len =
+ * DB_DELTA_STEP_TOKENS). */
+#define DB_DELTA_STEP_TOKENS 16
 size_t db_gated_delta_workspace_bytes(int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads,
                                       int dtype);
 int db_gated_delta(const void *q, const void *k, const void *v, int dtype, int64_t ldq, int64_t ldk, int64_t ldv,
