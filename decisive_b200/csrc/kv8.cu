@@ -18,55 +18,12 @@
 #include "capi_internal.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "kv8.cuh"
 
 namespace db {
 namespace {
 
-constexpr int D = 128, BLK = DB_KV8_BLOCK;
-
-struct Kv8Args {
-    db_kv8_cache c;
-    const int32_t* lengths;  // [items] tokens cached before this call's rows
-    const int32_t* cu;       // [items + 1] rows of the items, or null: max_rows each
-    int items, rows, max_rows;
-    int* error;
-};
-
-// Item b: rows [start, start + count) of this call, `len` tokens cached before them.  Offsets and
-// lengths outside the tensors are brought back inside and noted in the error word.
-__device__ __forceinline__ void item_of(const Kv8Args& a, int b, int& start, int& count, int& len) {
-    if (a.cu) {
-        start = min(max(a.cu[b], 0), a.rows);
-        count = min(min(max(a.cu[b + 1], start), a.rows) - start, a.max_rows);
-    } else {
-        start = b * a.max_rows;
-        count = a.max_rows;
-    }
-    const int64_t most = (int64_t)a.c.table_width * BLK;
-    const int given = a.lengths[b];
-    len = given;
-    if (given < 0 || (int64_t)given + count > most) {
-        len = given < 0 ? 0 : (int)min((int64_t)given, most);
-        count = (int)min((int64_t)count, most - len);
-        if (a.error && threadIdx.x == 0) atomicOr(a.error, DB_DEV_ERR_SHAPE);
-    }
-}
-
-// The page that holds block i of item b, or -1 (noted in the error word) where the table names none.
-__device__ __forceinline__ int page_of(const Kv8Args& a, int b, int i) {
-    const int p = i < a.c.table_width ? a.c.page_table[(int64_t)b * a.c.table_width + i] : -1;
-    if ((unsigned)p < (unsigned)a.c.pages) return p;
-    if (a.error && (threadIdx.x & 31) == 0) atomicOr(a.error, DB_DEV_ERR_SHAPE);
-    return -1;
-}
-
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ float from_bits(uint32_t b) {
-    const unsigned short h = (unsigned short)b;
-    return to_f32(*reinterpret_cast<const T*>(&h));
-}
+constexpr int D = KV8_D, BLK = KV8_BLK;
 
 // ------------------------------------------------------------------ append
 constexpr int APPEND_THREADS = 256;
@@ -298,52 +255,12 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 2^x on the special-function unit
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // The 8 x 8 matrix of 16-bit values that a warp holds, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// Four int8 codes as two pairs of f16, exactly: the bytes become the low bits of 1024 + (code + 128).
-__device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t& hi) {
-    c ^= 0x80808080u;
-    const uint32_t l = __byte_perm(c, 0x64646464u, 0x4140), h = __byte_perm(c, 0x64646464u, 0x4342);
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&l), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&h), off);
-    lo = *reinterpret_cast<const uint32_t*>(&x);
-    hi = *reinterpret_cast<const uint32_t*>(&y);
-}
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-struct AttnArgs {
-    Kv8Args kv;
-    const void* q;
-    int64_t ldq;
-    void* out;
-    int64_t ldo;
-    int group;     // query heads per kv head
-    float factor;  // scale * log2 e
-    float* parts;  // decode: partial results, see kv8_decode_kernel
-};
-
 // Scores and the context are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that the codes are
 // the wide operand (16 keys or 16 value features of an MMA) and 8 query rows the narrow one: a single
 // token's 4 or 8 heads fill it.  Row n of a kv head's tile is query (token n / group, head n % group).
@@ -955,45 +872,8 @@ __global__ void __launch_bounds__(256 * NT) kv8_join_kernel(AttnArgs a, int64_t 
     }
 }
 
-// ------------------------------------------------------------------ many rows
-// One warp per tile of 32 query rows; the tiles of a CTA are neighbours and read the same blocks, from L1.
-constexpr int MANY_NT = 4, MANY_WARPS = 4;
-
-template <typename T>
-__global__ void __launch_bounds__(32 * MANY_WARPS, 2) kv8_rows_kernel(AttnArgs a) {
-    const int warp = threadIdx.x >> 5, h = blockIdx.y, b = blockIdx.z, Hk = a.kv.c.kv_heads;
-    pdl_wait();
-    pdl_trigger();
-    int start, count, len;
-    item_of(a.kv, b, start, count, len);
-    // the last tiles see the most keys: they start first
-    const int rows = count * a.group, row0 = ((int)(gridDim.x - 1 - blockIdx.x) * MANY_WARPS + warp) * 8 * MANY_NT;
-    if (row0 >= rows) return;
-    __shared__ uint2 queries[MANY_WARPS][MANY_NT * 8 * 32];
-    Tile<T, MANY_NT> tile;
-    tile.open(queries[warp], static_cast<const T*>(a.q) + (int64_t)start * a.ldq + (int64_t)h * a.group * D, a.ldq, row0, rows, len, a.group,
-              a.factor);
-    const int whole = (len + count) / BLK, blocks = (len + (min(row0 + 8 * MANY_NT, rows) - 1) / a.group) / BLK + 1;
-    for (int i = 0; i < blocks; ++i) {
-        if (i >= whole) {
-            const int64_t at = ((int64_t)b * Hk + h) * BLK * D;
-            tile.tail(static_cast<const T*>(a.kv.c.k_tail) + at, static_cast<const T*>(a.kv.c.v_tail) + at,
-                      len + count - i * BLK, i * BLK);
-            continue;
-        }
-        const int page = page_of(a.kv, b, i);
-        if (page < 0) continue;
-        const int64_t ph = (int64_t)page * Hk + h;
-        uint4 kc[4][2][2];
-        tile.load_keys(kc, a.kv.c.k_codes + ph * BLK * D);
-        tile.block(kc, a.kv.c.v_codes + ph * BLK * D, a.kv.c.k_scales[ph], a.kv.c.v_scales[ph], i * BLK, nullptr);
-    }
-    tile.close();
-    tile.write(static_cast<T*>(a.out) + (int64_t)start * a.ldo + (int64_t)h * a.group * D, a.ldo);
-}
-
 // ------------------------------------------------------------------ launches
-// n tiles of 8 rows for the dealt-out form; 0: many rows
+// n tiles of 8 rows for the dealt-out form; 0: many rows (kv8_rows.cu)
 int decode_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 0; }
 // CTAs of the dealt-out form: as many as are resident at once, fewer when there are not that many blocks
 int64_t decode_ctas(int nt, int64_t items, int64_t heads, int64_t max_keys) {
@@ -1018,9 +898,7 @@ cudaError_t attention(const AttnArgs& a, int64_t max_keys, cudaStream_t stream) 
     const int nt = decode_tiles(rows);
     if (nt == 1) return launch_decode<T, 1>(a, max_keys, stream);
     if (nt == 2) return launch_decode<T, 2>(a, max_keys, stream);
-    const int64_t tiles = (rows + 8 * MANY_NT * MANY_WARPS - 1) / (8 * MANY_NT * MANY_WARPS);
-    return db_launch_pdl(kv8_rows_kernel<T>, dim3((unsigned)tiles, a.kv.c.kv_heads, a.kv.items), dim3(32 * MANY_WARPS), 0,
-                         stream, a);
+    return kv8_rows_attention<T>(a, stream);
 }
 
 // What every call on a cache checks; fills the arguments that they share.

@@ -1,0 +1,517 @@
+// Attention over the 8-bit cache for many query rows (a chunk of a prompt), on the tcgen05 tensor cores.
+//
+// One CTA = 128 query rows of one kv head (token n / group, head n % group: neighbouring tokens share every key
+// tile), one row per lane of tensor memory; keys in tiles of one block (64), one pass.  Even and odd tiles go to two
+// softmax warpgroups, each with its own running maximum, sum and accumulator, joined at the end, so the tensor
+// pipe always holds two independent chains.  Per tile
+//   S = Q K^T (codes as exact f16),  P = 2^(S c - m),  O += P V (codes as exact f16)
+// Four warps turn codes into f16 tiles in shared memory, in the order in which the MMAs take them; a value page is
+// stored [128][64 tokens], which is already the K-major operand.  P stays in tensor memory: it overwrites S
+// and is the A operand of the second product, as one f16 for bf16 outputs, as two for f16 ones.  Where scales go: a
+// key block's into the exponent's factor, a value block's into P, relative to the largest value scale of the
+// keys that the CTA reads (blocks below 2^-24 of that count as 2^-24), the row sum taken back by its inverse.  The
+// maximum moves only when a tile raises it by more than 8 (log2), so accumulators are rarely rescaled.
+//
+// Warps: 0-3 conversion, 4-7 softmax of even tiles, 8-11 of odd tiles, 12 MMA issue and tensor memory.
+// Tensor memory (512 columns): S / P of (parity, slot) at 128 parity + 64 slot, O even 256-383, O odd 384-511.
+#include "kv8.cuh"
+#include "capi_internal.h"
+#include "kernels.h"
+#include "tc_chain.cuh"
+
+namespace db {
+namespace {
+
+using chain::tie32;
+using chain::warp_wait;
+
+constexpr int D = KV8_D, BLK = KV8_BLK;
+constexpr int ROWS = 128, THREADS = 416;
+constexpr int STAGES = 10, STAGE = BLK * D * 2;  // f16 tiles of one block's keys or values
+constexpr int Q_BYTES = ROWS * D * 2, Q_HALF = Q_BYTES / 2, K_HALF = STAGE / 2;
+constexpr int INFO = 16;                         // tiles whose scales are kept at a time
+constexpr uint32_t TM_O = 256;
+constexpr uint64_t DRAIN_NS = 100000000ull;
+
+enum Bar { FULL = 0, EMPTY = FULL + STAGES, S_FULL = EMPTY + STAGES, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
+           JOIN = PV_DONE + 4, MMA_DONE, END, BARS };
+
+struct Info {
+    float ks;     // key scale
+    float shift;  // 7 + log2 (value scale / reference)
+    float undo;   // 2^-shift
+    int there;
+};
+struct Shared {
+    uint64_t bars[BARS];
+    Info info[INFO];
+    float row_factor[ROWS];
+    float join_m[2][ROWS], join_l[2][ROWS];
+    uint32_t tmem;
+    int abort;
+    uint32_t vref, tail_k, tail_v;  // largest value scale (bits); the open block's largest magnitudes (16-bit bits)
+    int odd;                        // the open block has values that are not finite
+};
+constexpr int SMEM = 1024 + Q_BYTES + STAGES * STAGE + sizeof(Shared);
+static_assert(SMEM <= 232448, "shared memory");
+
+// 2^e that brings a largest magnitude m to [2^7, 2^8), the codes' own size (1 for 0); back = 2^-e.
+__device__ __forceinline__ float code_power(float m, float& back) {
+    const int e = (int)((__float_as_uint(m) >> 23) & 0xff) - 127;
+    const int k = m > 0.f ? min(max(7 - e, -126), 126) : 0;
+    back = __uint_as_float((uint32_t)(127 - k) << 23);
+    return __uint_as_float((uint32_t)(127 + k) << 23);
+}
+__device__ __forceinline__ void sts128u(uint8_t* base, uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    *reinterpret_cast<uint4*>(base + at) = make_uint4(a, b, c, d);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
+    constexpr bool TWO = std::is_same<T, __half>::value;
+    constexpr uint32_t INF = TWO ? 0x7c00u : 0x7f80u;
+    extern __shared__ uint8_t rows_smem[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rows_smem) + 1023) & ~uintptr_t(1023));
+    uint8_t* ring = smem + Q_BYTES;
+    Shared& sh = *reinterpret_cast<Shared*>(ring + STAGES * STAGE);
+    volatile int* abort_flag = &sh.abort;
+    int* err = a.kv.error;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int h = blockIdx.y, b = blockIdx.z, Hk = a.kv.c.kv_heads;
+    pdl_wait();
+    pdl_trigger();
+    int start, count, len;
+    item_of(a.kv, b, start, count, len);
+    // the last tiles see the most keys: they start first
+    const int rows = count * a.group, row0 = (int)(gridDim.x - 1 - blockIdx.x) * ROWS;
+    if (row0 >= rows) return;
+    const int last = len + (min(row0 + ROWS, rows) - 1) / a.group;  // last key that a row sees
+    const int whole = (len + count) / BLK, blocks = last / BLK + 1;
+    const int tiles = (blocks + 1) & ~1, pairs = tiles / 2;  // (an odd count is filled up by a tile without keys)
+    const int inside = blocks > whole ? len + count - whole * BLK : 0;  // tokens of the open block, where it is read
+    const int64_t tail_at = ((int64_t)b * Hk + h) * BLK * D;
+    const T* kt = static_cast<const T*>(a.kv.c.k_tail) + tail_at;
+    const T* vt = static_cast<const T*>(a.kv.c.v_tail) + tail_at;
+
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(&sh.bars[FULL + i], 1);
+            mbar_init(&sh.bars[EMPTY + i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&sh.bars[S_FULL + i], 1);
+            mbar_init(&sh.bars[P_FULL + i], 4);
+            mbar_init(&sh.bars[PV_DONE + i], 1);
+        }
+        mbar_init(&sh.bars[JOIN], 8);
+        mbar_init(&sh.bars[MMA_DONE], 1);
+        mbar_init(&sh.bars[END], THREADS / 32);
+        sh.abort = 0;
+        sh.vref = sh.tail_k = sh.tail_v = 0;
+        sh.odd = 0;
+        fence_barrier_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(&sh.tmem, 512);
+        tmem_relinquish();
+    }
+    // queries to [2^7, 2^8) per row, K-major and 128-byte swizzled: two columns of 64 dims x 128 rows
+    const float sign = a.factor < 0.f ? -1.f : 1.f;
+    for (int r = warp; r < ROWS; r += THREADS / 32) {
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        const int row = row0 + r;
+        if (row < rows) {
+            const T* q = static_cast<const T*>(a.q) + (int64_t)(start + row / a.group) * a.ldq +
+                         ((int64_t)h * a.group + row % a.group) * D + 4 * lane;
+            const uint2 w = *reinterpret_cast<const uint2*>(q);
+            x[0] = from_bits<T>(w.x & 0xffffu), x[1] = from_bits<T>(w.x >> 16);
+            x[2] = from_bits<T>(w.y & 0xffffu), x[3] = from_bits<T>(w.y >> 16);
+        }
+        float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+        top = warp_max(top);
+        float back = 1.f;
+        const float up = sign * (top < INFINITY ? code_power(top, back) : 1.f);
+        if (lane == 0) sh.row_factor[r] = fabsf(a.factor) * back;
+        const uint32_t at = (lane >> 4) * Q_HALF + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + 8 * (lane & 1);
+        *reinterpret_cast<uint2*>(smem + at) = make_uint2(pack2<__half>(x[0] * up, x[1] * up), pack2<__half>(x[2] * up, x[3] * up));
+    }
+    __syncthreads();
+    // the largest value scale that is read, and the open block's magnitudes
+    {
+        float top = 0.f;
+        for (int i = tid; i < min(blocks, whole); i += THREADS) {
+            const int p = i < a.kv.c.table_width ? a.kv.c.page_table[(int64_t)b * a.kv.c.table_width + i] : -1;
+            if ((unsigned)p < (unsigned)a.kv.c.pages) {
+                const float s = a.kv.c.v_scales[(int64_t)p * Hk + h];
+                if (s < INFINITY) top = fmaxf(top, s);
+            }
+        }
+        top = warp_max(top);
+        if (lane == 0 && top > 0.f) atomicMax(&sh.vref, __float_as_uint(top));
+        uint32_t km = 0, vm = 0;
+        bool odd = false;
+        for (int e = tid; inside && e < BLK * D / 8; e += THREADS) {
+            const uint4 k = *reinterpret_cast<const uint4*>(kt + 8 * e), v = *reinterpret_cast<const uint4*>(vt + 8 * e);
+            const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
+            const bool key_there = e / (D / 8) < inside;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t x = kw[j >> 1] >> (16 * (j & 1)) & 0x7fffu, y = vw[j >> 1] >> (16 * (j & 1)) & 0x7fffu;
+                if (key_there && x < INF) km = max(km, x);
+                if (8 * e % BLK + j < inside) {
+                    if (y < INF) vm = max(vm, y); else odd = true;
+                }
+            }
+        }
+        if (inside) {
+            km = __reduce_max_sync(0xffffffffu, km);
+            vm = __reduce_max_sync(0xffffffffu, vm);
+            if (lane == 0) {
+                atomicMax(&sh.tail_k, km);
+                atomicMax(&sh.tail_v, vm);
+            }
+            if (__any_sync(0xffffffffu, odd) && lane == 0) sh.odd = 1;
+        }
+    }
+    fence_proxy_async_smem();  // the query tile
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    float kt_back, vt_back;
+    const float kt_up = code_power(from_bits<T>(sh.tail_k), kt_back), vt_up = code_power(from_bits<T>(sh.tail_v), vt_back);
+    const float vref0 = fmaxf(__uint_as_float(sh.vref), inside ? vt_back : 0.f), vref = vref0 > 0.f ? vref0 : 1.f;
+
+    if (warp < 4) {
+        // ---------------------------------------------------------------- codes -> f16 tiles
+        // load i, in the order of use: K 0, K 1, then per pair p: K 2p+2, K 2p+3 (while there are), V 2p, V 2p+1
+        const int loads = 2 * tiles;
+        auto what = [&](int i, bool& is_v) {
+            is_v = false;
+            if (i < 2) return i;
+            int p = (i - 2) >> 2, r = (i - 2) & 3;
+            if (p == pairs - 1) r += 2;
+            is_v = r >= 2;
+            return is_v ? 2 * p + r - 2 : 2 * p + 2 + r;
+        };
+        // Each warp takes every 4th load whole: what a load costs once (its page, its barriers, the proxy fence) is
+        // then paid by four at a time.  A lane holds 16 pieces of 16 codes; a piece's place is refilled with the
+        // warp's next load as soon as it is converted.  Page numbers are read one load further ahead.
+        const int known = min(blocks, whole);
+        auto table = [&](int i) {
+            bool is_v;
+            const int j = i < loads ? what(i, is_v) : known;
+            return j < known && j < a.kv.c.table_width ? a.kv.c.page_table[(int64_t)b * a.kv.c.table_width + j] : -1;
+        };
+        auto codes_of = [&](int i, int p) -> const uint4* {
+            bool is_v;
+            if (i < loads) what(i, is_v);
+            if (i >= loads || (unsigned)p >= (unsigned)a.kv.c.pages) return nullptr;
+            return reinterpret_cast<const uint4*>((is_v ? a.kv.c.v_codes : a.kv.c.k_codes) + ((int64_t)p * Hk + h) * BLK * D) + lane;
+        };
+        uint4 raw[16];
+        int page = table(warp), next_page = table(warp + 4);
+        {
+            const uint4* src = codes_of(warp, page);
+            if (src)
+#pragma unroll
+                for (int c = 0; c < 16; ++c) raw[c] = src[32 * c];
+        }
+        for (int i = warp; i < loads; i += 4) {
+            bool is_v;
+            const int j = what(i, is_v), st = i % STAGES;
+            const bool tail = j == whole && inside, paged = (unsigned)page < (unsigned)a.kv.c.pages;
+            if (j < known && !paged && lane == 0 && err) atomicOr(err, DB_DEV_ERR_SHAPE);
+            Info n;
+            n.ks = kt_back;
+            float vs = vt_back;
+            if (!is_v && paged) {
+                n.ks = a.kv.c.k_scales[(int64_t)page * Hk + h];
+                vs = a.kv.c.v_scales[(int64_t)page * Hk + h];
+            }
+            const uint4* src = codes_of(i + 4, next_page);
+            if (!warp_wait(&sh.bars[EMPTY + st], ((i / STAGES) & 1) ^ 1u, abort_flag, err, DB_DEV_ERR_TIMEOUT_CVT)) break;
+            uint8_t* dst = ring + st * STAGE;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const int q = lane + 32 * c;  // 16 codes: of key q / 8, or of value feature q / 4
+                uint32_t f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (paged) {
+                    codes_to_f16(raw[c].x, f[0], f[1]);
+                    codes_to_f16(raw[c].y, f[2], f[3]);
+                    codes_to_f16(raw[c].z, f[4], f[5]);
+                    codes_to_f16(raw[c].w, f[6], f[7]);
+                }
+                if (src) raw[c] = src[32 * c];
+                // rows of 128 bytes: a key's 64 dims, a value feature's 64 tokens
+                const int r = is_v ? q >> 2 : q >> 3, half = is_v ? 0 : (q >> 2) & 1, p0 = 2 * (q & 3);
+                const uint32_t row = half * K_HALF + r * 128;
+                // (the two halves of a key start with different pieces: one bank each)
+                const uint32_t first = row + (((p0 + half) ^ (r & 7)) << 4), second = row + (((p0 + 1 - half) ^ (r & 7)) << 4);
+                sts128u(dst, first, half ? f[4] : f[0], half ? f[5] : f[1], half ? f[6] : f[2], half ? f[7] : f[3]);
+                sts128u(dst, second, half ? f[0] : f[4], half ? f[1] : f[5], half ? f[2] : f[6], half ? f[3] : f[7]);
+            }
+            if (tail) {
+#pragma unroll 1
+                for (int c = 0; c < 16; ++c) {
+                    const int q = lane + 32 * c;
+                    const uint4* from = reinterpret_cast<const uint4*>((is_v ? vt : kt) + 16 * q);
+                    const uint4 x = from[0], y = from[1];
+                    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    const float up = is_v ? vt_up : kt_up;
+                    uint32_t f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        uint32_t l = w[e] & 0xffffu, g = w[e] >> 16;
+                        const int key = is_v ? 16 * (q & 3) + 2 * e : q >> 3;
+                        // slots without a token, and values (not keys) that are not finite, stay out of the products
+                        if (key >= inside || (is_v && (l & INF) == INF)) l = 0;
+                        if (key + (is_v ? 1 : 0) >= inside || (is_v && (g & INF) == INF)) g = 0;
+                        f[e] = pack2<__half>(from_bits<T>(l) * up, from_bits<T>(g) * up);
+                    }
+                    const int r = is_v ? q >> 2 : q >> 3, half = is_v ? 0 : (q >> 2) & 1, p0 = 2 * (q & 3);
+                    const uint32_t row = half * K_HALF + r * 128;
+                    sts128u(dst, row + ((p0 ^ (r & 7)) << 4), f[0], f[1], f[2], f[3]);
+                    sts128u(dst, row + (((p0 + 1) ^ (r & 7)) << 4), f[4], f[5], f[6], f[7]);
+                }
+            }
+            if (!is_v && lane == 0) {
+                float ratio = vs / vref;
+                ratio = ratio < 5.9604645e-8f ? 5.9604645e-8f : ratio;  // (a NaN stays)
+                n.shift = 7.f + log2f(ratio);
+                n.undo = 0.0078125f / ratio;
+                n.there = paged || tail;
+                sh.info[j & (INFO - 1)] = n;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[FULL + st]);
+            page = next_page;
+            next_page = table(i + 8);
+        }
+    } else if (warp == 12) {
+        // ---------------------------------------------------------------- MMA issue
+        constexpr uint32_t IDESC_S = idesc_f16_f32(ROWS, BLK), IDESC_O = idesc_f16_f32(ROWS, D);
+        const uint64_t dQ = sw128_desc(smem_u32(smem)), dR = sw128_desc(smem_u32(ring));
+        int st = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        auto next_stage = [&]() -> int {
+            const int s = st;
+            ok = ok && warp_wait(&sh.bars[FULL + s], ph, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+            if (++st == STAGES) st = 0, ph ^= 1u;
+            return s;
+        };
+        // S of pair p: slot p & 1 of both parities; free once the P V of pair p - 2 is done
+        auto scores = [&](int p) {
+            const int slot = p & 1;
+            for (int t = 0; t < 2 && ok; ++t) {
+                if (p >= 2) ok = warp_wait(&sh.bars[PV_DONE + 2 * t + slot], ((p >> 1) & 1) ^ 1u, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+                const int s = next_stage();
+                if (!ok) return;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t dK = dR + (uint64_t)((s * STAGE) >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        umma_f16(tmem + 128u * t + 64u * slot, dQ + (uint64_t)(((kk >> 2) * Q_HALF + (kk & 3) * 32) >> 4),
+                                 dK + (uint64_t)(((kk >> 2) * K_HALF + (kk & 3) * 32) >> 4), IDESC_S, kk > 0);
+                    umma_commit(&sh.bars[EMPTY + s]);
+                    umma_commit(&sh.bars[S_FULL + 2 * t + slot]);
+                }
+                __syncwarp();
+            }
+        };
+        auto context = [&](int p) {
+            const int slot = p & 1;
+            for (int t = 0; t < 2 && ok; ++t) {
+                const int s = next_stage();
+                ok = ok && warp_wait(&sh.bars[P_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+                if (!ok) return;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t dV = dR + (uint64_t)((s * STAGE) >> 4);
+                    const uint32_t p_tm = tmem + 128u * t + 64u * slot;
+#pragma unroll
+                    for (int kk = 0; kk < BLK / 16; ++kk) {
+                        // 32 keys lie in 32 columns: 16 of the first parts, 16 of the second
+                        const uint32_t at = p_tm + 32u * (kk >> 1) + 8u * (kk & 1);
+                        if (TWO) chain::umma_f16_ts(tmem + TM_O + 128u * t, at + 16u, dV + (uint64_t)(kk * 2), IDESC_O, p > 0 || kk > 0);
+                        chain::umma_f16_ts(tmem + TM_O + 128u * t, at, dV + (uint64_t)(kk * 2), IDESC_O, TWO || p > 0 || kk > 0);
+                    }
+                    umma_commit(&sh.bars[EMPTY + s]);
+                    umma_commit(&sh.bars[PV_DONE + 2 * t + slot]);
+                }
+                __syncwarp();
+            }
+        };
+        scores(0);
+        for (int p = 0; p < pairs && ok; ++p) {
+            if (p + 1 < pairs) scores(p + 1);
+            if (ok) context(p);
+        }
+        // every MMA issued has completed before tensor memory is released
+        if (lane == 0) {
+            umma_commit(&sh.bars[MMA_DONE]);
+            mbar_wait_drain(&sh.bars[MMA_DONE], 0, DRAIN_NS);
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- softmax
+        const int t = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t o_tm = tmem + lanes + TM_O + 128u * t;
+        const int limit = row0 + row < rows ? len + (row0 + row) / a.group : -1;
+        const float factor = sh.row_factor[row];
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int p = 0; p < pairs; ++p) {
+            const int slot = p & 1, base = (2 * p + t) * BLK;
+            const uint32_t s_tm = tmem + lanes + 128u * t + 64u * slot;
+            if (!(ok = warp_wait(&sh.bars[S_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI))) break;
+            tc_fence_after();
+            const Info n = sh.info[(2 * p + t) & (INFO - 1)];
+            uint32_t r[2][32];
+            tmem_ld_32x32b_x32(s_tm, r[0]);
+            tmem_ld_32x32b_x32(s_tm + 32u, r[1]);
+            tmem_wait_ld(r[0]);
+            tie32(r[1]);
+            const int seen = n.there ? limit - base : -1;  // keys 0 .. seen of the tile
+            const bool masked = __any_sync(0xffffffffu, seen < BLK - 1);
+            if (masked) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * c + i > seen) r[c][i] = __float_as_uint(-INFINITY);
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(r[c][i]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale = factor * n.ks;
+            const float mt = top == -INFINITY ? top : top * scale;
+            float move = 1.f;
+            if (mt > m + 8.f) {  // (the first keys: from -inf)
+                move = ex2(m - mt);
+                m = mt;
+                l *= move;
+            }
+            const float add = n.shift - (m == -INFINITY ? 0.f : m);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            // the previous P V of this parity is done: O is stable
+            const bool rescale = p > 0 && __any_sync(0xffffffffu, move != 1.f);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float x = ex2(fmaf(__uint_as_float(r[c][2 * i]), scale, add));
+                    float y = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), scale, add));
+                    if (masked) {  // (a factor of 0 or NaN must not reach what is masked)
+                        if (32 * c + 2 * i > seen) x = 0.f;
+                        if (32 * c + 2 * i + 1 > seen) y = 0.f;
+                    }
+                    sum[2 * (i & 1)] += x;
+                    sum[2 * (i & 1) + 1] += y;
+                    pk[i] = pack2<__half>(x, y);
+                    if (TWO) pk[16 + i] = pack2<__half>(x - from_bits<__half>(pk[i] & 0xffffu), y - from_bits<__half>(pk[i] >> 16));
+                }
+                if (TWO)
+                    chain::tmem_st32(s_tm + 32u * c, pk);
+                else
+                    chain::tmem_st16(s_tm + 32u * c, pk);
+            }
+            const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if (all != 0.f) l = fmaf(all, n.undo, l);
+            if (rescale) {
+                if (!(ok = warp_wait(&sh.bars[PV_DONE + 2 * t + (slot ^ 1)], ((p - 1) >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_32x32b_x32(o_tm + 32u * c, r[0]);
+                    tmem_wait_ld(r[0]);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) r[0][i] = __float_as_uint(__uint_as_float(r[0][i]) * move);
+                    chain::tmem_st32(o_tm + 32u * c, r[0]);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[P_FULL + 2 * t + slot]);
+        }
+        // the last P V of both parities, then the two halves together: this warpgroup writes 64 features
+        for (int x = 0; x < 2 && ok; ++x)
+            ok = warp_wait(&sh.bars[PV_DONE + 2 * x + ((pairs - 1) & 1)], ((pairs - 1) >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
+        if (ok) {
+            tc_fence_after();
+            sh.join_m[t][row] = m;
+            sh.join_l[t][row] = l;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[JOIN]);
+            ok = warp_wait(&sh.bars[JOIN], 0, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
+        }
+        if (ok) {
+            const float m0 = sh.join_m[0][row], m1 = sh.join_m[1][row], mm = fmaxf(m0, m1), at = mm == -INFINITY ? 0.f : mm;
+            const float f0 = ex2(m0 - at), f1 = ex2(m1 - at), sum = sh.join_l[0][row] * f0 + sh.join_l[1][row] * f1;
+            const float norm = sum == 0.f ? 0.f : vref * 0.0078125f / sum;  // no key could be read: 0
+            const float g0 = f0, g1 = f1;
+            const int n = row0 + row;
+            T* out = static_cast<T*>(a.out) + (int64_t)(start + n / a.group) * a.ldo + ((int64_t)h * a.group + n % a.group) * D + 64 * t;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t e[32], o[32];
+                const uint32_t from = tmem + lanes + TM_O + 64u * t + 32u * c;
+                tmem_ld_32x32b_x32(from, e);
+                tmem_ld_32x32b_x32(from + 128u, o);
+                tmem_wait_ld(e);
+                tie32(o);
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = (__uint_as_float(e[i]) * g0 + __uint_as_float(o[i]) * g1) * norm;
+                if (sh.odd) {
+                    // values of the open block that are not finite reach the rows that see their tokens
+                    for (int key = 0; key < min(inside, limit - whole * BLK + 1); ++key)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float x = to_f32(vt[(64 * t + 32 * c + i) * BLK + key]);
+                            if (!isfinite(x)) v[i] += x;
+                        }
+                }
+                if (n < rows) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) =
+                            make_uint4(pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+                                       pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+                }
+            }
+        }
+    }
+    // through an mbarrier: every role is done with tensor memory before it is released
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.bars[END]);
+    if (warp == 12) {
+        if (lane == 0) mbar_wait_drain(&sh.bars[END], 0, DB_WAIT_LIMIT_NS);
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace
+
+template <typename T>
+cudaError_t kv8_rows_attention(const AttnArgs& a, cudaStream_t stream) {
+    const cudaError_t e = db_set_max_smem(reinterpret_cast<const void*>(kv8_rows_kernel<T>), SMEM);
+    if (e != cudaSuccess) return e;
+    const int64_t tiles = ((int64_t)a.kv.max_rows * a.group + ROWS - 1) / ROWS;
+    return db_launch_pdl(kv8_rows_kernel<T>, dim3((unsigned)tiles, a.kv.c.kv_heads, a.kv.items), dim3(THREADS), SMEM, stream, a);
+}
+template cudaError_t kv8_rows_attention<__half>(const AttnArgs&, cudaStream_t);
+template cudaError_t kv8_rows_attention<__nv_bfloat16>(const AttnArgs&, cudaStream_t);
+
+}  // namespace db
