@@ -5,14 +5,15 @@
 // softmax warpgroups, each with its own running maximum, sum and accumulator, joined at the end, so the tensor
 // pipe always holds two independent chains.  Per tile
 //   S = Q K^T (codes as exact f16),  P = 2^(S c - m),  O += P V (codes as exact f16)
-// Four warps turn codes into f16 tiles in shared memory, in the order in which the MMAs take them; a value page is
+// Six warps turn codes into f16 tiles in shared memory, in the order in which the MMAs take them; a value page is
 // stored [128][64 tokens], which is already the K-major operand.  P stays in tensor memory: it overwrites S
 // and is the A operand of the second product, as one f16 for bf16 outputs, as two for f16 ones.  Where scales go: a
 // key block's into the exponent's factor, a value block's into P, relative to the largest value scale of the
 // keys that the CTA reads (blocks below 2^-24 of that count as 2^-24), the row sum taken back by its inverse.  The
 // maximum moves only when a tile raises it by more than 8 (log2), so accumulators are rarely rescaled.
 //
-// Warps: 0-3 conversion, 4-7 softmax of even tiles, 8-11 of odd tiles, 12 MMA issue and tensor memory.
+// Warps: 0-3, 14 and 15 conversion, 4-7 softmax of even tiles, 8-11 of odd tiles, 12 and 13 MMA issue for even and odd
+// tiles (one issuer for both was the kernel's bound: 3600 of 6600 cycles per pair of tiles), 12 tensor memory.
 // Tensor memory (512 columns): S / P of (parity, slot) at 128 parity + 64 slot, O even 256-383, O odd 384-511.
 #include "kv8.cuh"
 #include "capi_internal.h"
@@ -26,7 +27,7 @@ using chain::tie32;
 using chain::warp_wait;
 
 constexpr int D = KV8_D, BLK = KV8_BLK;
-constexpr int ROWS = 128, THREADS = 416;
+constexpr int ROWS = 128, THREADS = 512, CONVERTERS = 6;
 constexpr int STAGES = 10, STAGE = BLK * D * 2;  // f16 tiles of one block's keys or values
 constexpr int Q_BYTES = ROWS * D * 2, Q_HALF = Q_BYTES / 2, K_HALF = STAGE / 2;
 constexpr int INFO = 16;                         // tiles whose scales are kept at a time
@@ -34,7 +35,7 @@ constexpr uint32_t TM_O = 256;
 constexpr uint64_t DRAIN_NS = 100000000ull;
 
 enum Bar { FULL = 0, EMPTY = FULL + STAGES, S_FULL = EMPTY + STAGES, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
-           JOIN = PV_DONE + 4, MMA_DONE, END, BARS };
+           JOIN = PV_DONE + 4, MMA_DONE, END = MMA_DONE + 2, BARS };
 
 struct Info {
     float ks;     // key scale
@@ -64,6 +65,73 @@ __device__ __forceinline__ float code_power(float m, float& back) {
 }
 __device__ __forceinline__ void sts128u(uint8_t* base, uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     *reinterpret_cast<uint4*>(base + at) = make_uint4(a, b, c, d);
+}
+
+// One row's softmax step on a tile's 64 scores: moves the maximum m (and l) if the tile raises it by more than 8, writes
+// P = 2^(S scale + shift - m) over S as the f16 operand (32 keys to 32 columns: 16 of first parts, 16 of second), returns
+// its sum.  MASKED: only keys 0 .. seen count; a scale of 0 or NaN must not reach the others.
+template <bool TWO, bool MASKED>
+__device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float scale, float shift, float& m, float& l, float& move,
+                                        uint32_t s_tm) {
+    if (MASKED) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (32 * c + i > seen) r[c][i] = __float_as_uint(-INFINITY);
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(r[c][i]));
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    const float mt = top == -INFINITY ? top : top * scale;
+    if (mt > m + 8.f) {  // (the first keys: from -inf)
+        move = ex2(m - mt);
+        m = mt;
+        l *= move;
+    }
+    const float add = shift - (m == -INFINITY ? 0.f : m);
+    const uint64_t scale2 = f2_pack(__float_as_uint(scale), __float_as_uint(scale)), add2 = f2_pack(__float_as_uint(add), __float_as_uint(add));
+    const uint64_t minus = f2_pack(0xbf800000u, 0xbf800000u);
+    uint64_t sum[2] = {0, 0};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        uint32_t pk[32];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint64_t e = f2_fma(f2_pack(r[c][2 * i], r[c][2 * i + 1]), scale2, add2);
+            float x = ex2(f2_lo(e)), y = ex2(f2_hi(e));
+            if (MASKED) {
+                if (32 * c + 2 * i > seen) x = 0.f;
+                if (32 * c + 2 * i + 1 > seen) y = 0.f;
+            }
+            const uint64_t xy = f2_pack(__float_as_uint(x), __float_as_uint(y));
+            sum[i & 1] = f2_add(sum[i & 1], xy);
+            pk[i] = pack2<__half>(x, y);
+            if (TWO) {
+                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pk[i]));
+                const uint64_t left = f2_fma(f2_pack(__float_as_uint(h.x), __float_as_uint(h.y)), minus, xy);
+                pk[16 + i] = pack2<__half>(f2_lo(left), f2_hi(left));
+            }
+        }
+        if (TWO)
+            chain::tmem_st32(s_tm + 32u * c, pk);
+        else
+            chain::tmem_st16(s_tm + 32u * c, pk);
+    }
+    const uint64_t both = f2_add(sum[0], sum[1]);
+    return f2_lo(both) + f2_hi(both);
+}
+
+// A bounded wait for roles that run ahead: the thread sleeps between its looks.
+__device__ __forceinline__ bool warp_wait_idle(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    int ok = 1;
+    if ((threadIdx.x & 31) == 0) ok = mbar_wait_backoff(bar, parity, abort_flag, err, DB_DEV_ERR_TIMEOUT_CVT);
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();
+    return ok != 0;
 }
 
 template <typename T>
@@ -105,6 +173,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         }
         mbar_init(&sh.bars[JOIN], 8);
         mbar_init(&sh.bars[MMA_DONE], 1);
+        mbar_init(&sh.bars[MMA_DONE + 1], 1);
         mbar_init(&sh.bars[END], THREADS / 32);
         sh.abort = 0;
         sh.vref = sh.tail_k = sh.tail_v = 0;
@@ -182,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
     const float kt_up = code_power(from_bits<T>(sh.tail_k), kt_back), vt_up = code_power(from_bits<T>(sh.tail_v), vt_back);
     const float vref0 = fmaxf(__uint_as_float(sh.vref), inside ? vt_back : 0.f), vref = vref0 > 0.f ? vref0 : 1.f;
 
-    if (warp < 4) {
+    if (warp < 4 || warp > 13) {
         // ---------------------------------------------------------------- codes -> f16 tiles
         // load i, in the order of use: K 0, K 1, then per pair p: K 2p+2, K 2p+3 (while there are), V 2p, V 2p+1
         const int loads = 2 * tiles;
@@ -194,8 +263,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             is_v = r >= 2;
             return is_v ? 2 * p + r - 2 : 2 * p + 2 + r;
         };
-        // Each warp takes every 4th load whole: what a load costs once (its page, its barriers, the proxy fence) is
-        // then paid by four at a time.  A lane holds 16 pieces of 16 codes; a piece's place is refilled with the
+        // Each warp takes every 6th load whole: what a load costs once (its page, its barriers, the proxy fence) is
+        // then paid by six at a time.  A lane holds 16 pieces of 16 codes; a piece's place is refilled with the
         // warp's next load as soon as it is converted.  Page numbers are read one load further ahead.
         const int known = min(blocks, whole);
         auto table = [&](int i) {
@@ -207,34 +276,53 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             bool is_v;
             if (i < loads) what(i, is_v);
             if (i >= loads || (unsigned)p >= (unsigned)a.kv.c.pages) return nullptr;
-            return reinterpret_cast<const uint4*>((is_v ? a.kv.c.v_codes : a.kv.c.k_codes) + ((int64_t)p * Hk + h) * BLK * D) + lane;
+            return reinterpret_cast<const uint4*>((is_v ? a.kv.c.v_codes : a.kv.c.k_codes) + ((int64_t)p * Hk + h) * BLK * D);
+        };
+        // piece c of this lane: 8 lanes that store together take four pieces of one half of two rows (of keys), or of two
+        // rows (of values): eight different banks
+        auto piece = [&](int c, bool is_v) {
+            return is_v ? lane + 32 * c : (4 * c + 2 * (lane >> 4) + ((lane >> 2) & 1)) * 8 + ((lane >> 3) & 1) * 4 + (lane & 3);
+        };
+        auto first_is_v = [&](int i) {
+            bool is_v = false;
+            if (i < loads) what(i, is_v);
+            return is_v;
         };
         uint4 raw[16];
-        int page = table(warp), next_page = table(warp + 4);
+        const int mine = warp < 4 ? warp : warp - 10;
+        int page = table(mine), next_page = table(mine + CONVERTERS);
+        float ks = 0.f, vs = 0.f;  // the block's scales, with its codes
+        auto scales_of = [&](int i, int p) {
+            if (i < loads && !first_is_v(i) && (unsigned)p < (unsigned)a.kv.c.pages) {
+                ks = a.kv.c.k_scales[(int64_t)p * Hk + h];
+                vs = a.kv.c.v_scales[(int64_t)p * Hk + h];
+            }
+        };
         {
-            const uint4* src = codes_of(warp, page);
+            const uint4* src = codes_of(mine, page);
             if (src)
 #pragma unroll
-                for (int c = 0; c < 16; ++c) raw[c] = src[32 * c];
+                for (int c = 0; c < 16; ++c) raw[c] = src[piece(c, first_is_v(mine))];
+            scales_of(mine, page);
         }
-        for (int i = warp; i < loads; i += 4) {
+        for (int i = mine; i < loads; i += CONVERTERS) {
             bool is_v;
             const int j = what(i, is_v), st = i % STAGES;
             const bool tail = j == whole && inside, paged = (unsigned)page < (unsigned)a.kv.c.pages;
             if (j < known && !paged && lane == 0 && err) atomicOr(err, DB_DEV_ERR_SHAPE);
             Info n;
-            n.ks = kt_back;
-            float vs = vt_back;
-            if (!is_v && paged) {
-                n.ks = a.kv.c.k_scales[(int64_t)page * Hk + h];
-                vs = a.kv.c.v_scales[(int64_t)page * Hk + h];
-            }
-            const uint4* src = codes_of(i + 4, next_page);
-            if (!warp_wait(&sh.bars[EMPTY + st], ((i / STAGES) & 1) ^ 1u, abort_flag, err, DB_DEV_ERR_TIMEOUT_CVT)) break;
+            n.ks = paged ? ks : kt_back;
+            const float v_scale = paged ? vs : vt_back;
+            scales_of(i + CONVERTERS, next_page);
+            const uint4* src = codes_of(i + CONVERTERS, next_page);
+            const bool next_v = first_is_v(i + CONVERTERS);
+            if (!warp_wait_idle(&sh.bars[EMPTY + st], ((i / STAGES) & 1) ^ 1u, abort_flag, err)) break;
             uint8_t* dst = ring + st * STAGE;
+            // rows of 128 bytes: a key's 64 dims, a value feature's 64 tokens; piece 0's row and first half of 16 bytes
+            const int q0 = piece(0, is_v), r0 = is_v ? q0 >> 2 : q0 >> 3, half = is_v ? 0 : (q0 >> 2) & 1, p0 = 2 * (q0 & 3);
+            const int n0 = piece(0, next_v), step = is_v ? 8 : 4;
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
-                const int q = lane + 32 * c;  // 16 codes: of key q / 8, or of value feature q / 4
                 uint32_t f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
                 if (paged) {
                     codes_to_f16(raw[c].x, f[0], f[1]);
@@ -242,19 +330,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                     codes_to_f16(raw[c].z, f[4], f[5]);
                     codes_to_f16(raw[c].w, f[6], f[7]);
                 }
-                if (src) raw[c] = src[32 * c];
-                // rows of 128 bytes: a key's 64 dims, a value feature's 64 tokens
-                const int r = is_v ? q >> 2 : q >> 3, half = is_v ? 0 : (q >> 2) & 1, p0 = 2 * (q & 3);
-                const uint32_t row = half * K_HALF + r * 128;
-                // (the two halves of a key start with different pieces: one bank each)
-                const uint32_t first = row + (((p0 + half) ^ (r & 7)) << 4), second = row + (((p0 + 1 - half) ^ (r & 7)) << 4);
-                sts128u(dst, first, half ? f[4] : f[0], half ? f[5] : f[1], half ? f[6] : f[2], half ? f[7] : f[3]);
-                sts128u(dst, second, half ? f[0] : f[4], half ? f[1] : f[5], half ? f[2] : f[6], half ? f[3] : f[7]);
+                if (src) raw[c] = src[n0 + 32 * c];
+                const int r = r0 + step * c;
+                uint8_t* row = dst + half * K_HALF + r * 128;
+                sts128u(row, (p0 ^ (r & 7)) << 4, f[0], f[1], f[2], f[3]);
+                sts128u(row, ((p0 + 1) ^ (r & 7)) << 4, f[4], f[5], f[6], f[7]);
             }
             if (tail) {
 #pragma unroll 1
                 for (int c = 0; c < 16; ++c) {
-                    const int q = lane + 32 * c;
+                    const int q = piece(c, is_v);
                     const uint4* from = reinterpret_cast<const uint4*>((is_v ? vt : kt) + 16 * q);
                     const uint4 x = from[0], y = from[1];
                     const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
@@ -276,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                 }
             }
             if (!is_v && lane == 0) {
-                float ratio = vs / vref;
+                float ratio = v_scale / vref;
                 ratio = ratio < 5.9604645e-8f ? 5.9604645e-8f : ratio;  // (a NaN stays)
                 n.shift = 7.f + log2f(ratio);
                 n.undo = 0.0078125f / ratio;
@@ -287,73 +372,67 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[FULL + st]);
             page = next_page;
-            next_page = table(i + 8);
+            next_page = table(i + 2 * CONVERTERS);
         }
-    } else if (warp == 12) {
-        // ---------------------------------------------------------------- MMA issue
+    } else if (warp >= 12) {
+        // ---------------------------------------------------------------- MMA issue, one parity of tiles
         constexpr uint32_t IDESC_S = idesc_f16_f32(ROWS, BLK), IDESC_O = idesc_f16_f32(ROWS, D);
+        const int t = warp - 12;
         const uint64_t dQ = sw128_desc(smem_u32(smem)), dR = sw128_desc(smem_u32(ring));
-        int st = 0;
-        uint32_t ph = 0;
+        const uint32_t s_tm = tmem + 128u * t, o_tm = tmem + TM_O + 128u * t;
         bool ok = true;
-        auto next_stage = [&]() -> int {
-            const int s = st;
-            ok = ok && warp_wait(&sh.bars[FULL + s], ph, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
-            if (++st == STAGES) st = 0, ph ^= 1u;
-            return s;
+        auto loaded = [&](int i) -> int {  // the stage of load i, once it is there
+            const int st = i % STAGES;
+            ok = ok && warp_wait(&sh.bars[FULL + st], (i / STAGES) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+            return st;
         };
-        // S of pair p: slot p & 1 of both parities; free once the P V of pair p - 2 is done
+        // S of pair p goes where the P of pair p - 2 was: after its P V
         auto scores = [&](int p) {
             const int slot = p & 1;
-            for (int t = 0; t < 2 && ok; ++t) {
-                if (p >= 2) ok = warp_wait(&sh.bars[PV_DONE + 2 * t + slot], ((p >> 1) & 1) ^ 1u, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
-                const int s = next_stage();
-                if (!ok) return;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t dK = dR + (uint64_t)((s * STAGE) >> 4);
+            if (p >= 2) ok = warp_wait(&sh.bars[PV_DONE + 2 * t + slot], ((p >> 1) & 1) ^ 1u, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+            const int st = loaded(p ? 4 * p - 2 + t : t);
+            if (!ok) return;
+            tc_fence_after();
+            if (lane == 0) {
+                const uint64_t dK = dR + (uint64_t)((st * STAGE) >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        umma_f16(tmem + 128u * t + 64u * slot, dQ + (uint64_t)(((kk >> 2) * Q_HALF + (kk & 3) * 32) >> 4),
-                                 dK + (uint64_t)(((kk >> 2) * K_HALF + (kk & 3) * 32) >> 4), IDESC_S, kk > 0);
-                    umma_commit(&sh.bars[EMPTY + s]);
-                    umma_commit(&sh.bars[S_FULL + 2 * t + slot]);
-                }
-                __syncwarp();
+                for (int kk = 0; kk < D / 16; ++kk)
+                    umma_f16(s_tm + 64u * slot, dQ + (uint64_t)(((kk >> 2) * Q_HALF + (kk & 3) * 32) >> 4),
+                             dK + (uint64_t)(((kk >> 2) * K_HALF + (kk & 3) * 32) >> 4), IDESC_S, kk > 0);
+                umma_commit(&sh.bars[EMPTY + st]);
+                umma_commit(&sh.bars[S_FULL + 2 * t + slot]);
             }
+            __syncwarp();
         };
         auto context = [&](int p) {
-            const int slot = p & 1;
-            for (int t = 0; t < 2 && ok; ++t) {
-                const int s = next_stage();
-                ok = ok && warp_wait(&sh.bars[P_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
-                if (!ok) return;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t dV = dR + (uint64_t)((s * STAGE) >> 4);
-                    const uint32_t p_tm = tmem + 128u * t + 64u * slot;
+            const int slot = p & 1, st = loaded(4 * p + (p == pairs - 1 ? 2 : 4) + t);
+            ok = ok && warp_wait(&sh.bars[P_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+            if (!ok) return;
+            tc_fence_after();
+            if (lane == 0) {
+                const uint64_t dV = dR + (uint64_t)((st * STAGE) >> 4);
 #pragma unroll
-                    for (int kk = 0; kk < BLK / 16; ++kk) {
-                        // 32 keys lie in 32 columns: 16 of the first parts, 16 of the second
-                        const uint32_t at = p_tm + 32u * (kk >> 1) + 8u * (kk & 1);
-                        if (TWO) chain::umma_f16_ts(tmem + TM_O + 128u * t, at + 16u, dV + (uint64_t)(kk * 2), IDESC_O, p > 0 || kk > 0);
-                        chain::umma_f16_ts(tmem + TM_O + 128u * t, at, dV + (uint64_t)(kk * 2), IDESC_O, TWO || p > 0 || kk > 0);
-                    }
-                    umma_commit(&sh.bars[EMPTY + s]);
-                    umma_commit(&sh.bars[PV_DONE + 2 * t + slot]);
+                for (int kk = 0; kk < BLK / 16; ++kk) {
+                    // 32 keys lie in 32 columns: 16 of the first parts, 16 of the second
+                    const uint32_t at = s_tm + 64u * slot + 32u * (kk >> 1) + 8u * (kk & 1);
+                    if (TWO) chain::umma_f16_ts(o_tm, at + 16u, dV + (uint64_t)(kk * 2), IDESC_O, p > 0 || kk > 0);
+                    chain::umma_f16_ts(o_tm, at, dV + (uint64_t)(kk * 2), IDESC_O, TWO || p > 0 || kk > 0);
                 }
-                __syncwarp();
+                umma_commit(&sh.bars[EMPTY + st]);
+                umma_commit(&sh.bars[PV_DONE + 2 * t + slot]);
             }
+            __syncwarp();
         };
         scores(0);
+        if (pairs > 1 && ok) scores(1);
         for (int p = 0; p < pairs && ok; ++p) {
-            if (p + 1 < pairs) scores(p + 1);
-            if (ok) context(p);
+            context(p);
+            if (p + 2 < pairs && ok) scores(p + 2);
         }
         // every MMA issued has completed before tensor memory is released
         if (lane == 0) {
-            umma_commit(&sh.bars[MMA_DONE]);
-            mbar_wait_drain(&sh.bars[MMA_DONE], 0, DRAIN_NS);
+            umma_commit(&sh.bars[MMA_DONE + t]);
+            mbar_wait_drain(&sh.bars[MMA_DONE + t], 0, DRAIN_NS);
         }
         __syncwarp();
     } else {
@@ -377,54 +456,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             tmem_wait_ld(r[0]);
             tie32(r[1]);
             const int seen = n.there ? limit - base : -1;  // keys 0 .. seen of the tile
-            const bool masked = __any_sync(0xffffffffu, seen < BLK - 1);
-            if (masked) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (32 * c + i > seen) r[c][i] = __float_as_uint(-INFINITY);
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(r[c][i]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), scale = factor * n.ks;
-            const float mt = top == -INFINITY ? top : top * scale;
-            float move = 1.f;
-            if (mt > m + 8.f) {  // (the first keys: from -inf)
-                move = ex2(m - mt);
-                m = mt;
-                l *= move;
-            }
-            const float add = n.shift - (m == -INFINITY ? 0.f : m);
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-            // the previous P V of this parity is done: O is stable
-            const bool rescale = p > 0 && __any_sync(0xffffffffu, move != 1.f);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t pk[32];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float x = ex2(fmaf(__uint_as_float(r[c][2 * i]), scale, add));
-                    float y = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), scale, add));
-                    if (masked) {  // (a factor of 0 or NaN must not reach what is masked)
-                        if (32 * c + 2 * i > seen) x = 0.f;
-                        if (32 * c + 2 * i + 1 > seen) y = 0.f;
-                    }
-                    sum[2 * (i & 1)] += x;
-                    sum[2 * (i & 1) + 1] += y;
-                    pk[i] = pack2<__half>(x, y);
-                    if (TWO) pk[16 + i] = pack2<__half>(x - from_bits<__half>(pk[i] & 0xffffu), y - from_bits<__half>(pk[i] >> 16));
-                }
-                if (TWO)
-                    chain::tmem_st32(s_tm + 32u * c, pk);
-                else
-                    chain::tmem_st16(s_tm + 32u * c, pk);
-            }
-            const float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const float scale = factor * n.ks;
+            float move = 1.f, all;
+            if (__any_sync(0xffffffffu, seen < BLK - 1))
+                all = soften<TWO, true>(r, seen, scale, n.shift, m, l, move, s_tm);
+            else
+                all = soften<TWO, false>(r, seen, scale, n.shift, m, l, move, s_tm);
             if (all != 0.f) l = fmaf(all, n.undo, l);
+            // O is stable once the previous P V of this parity is done
+            const bool rescale = p > 0 && __any_sync(0xffffffffu, move != 1.f);
             if (rescale) {
                 if (!(ok = warp_wait(&sh.bars[PV_DONE + 2 * t + (slot ^ 1)], ((p - 1) >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI))) break;
                 tc_fence_after();
