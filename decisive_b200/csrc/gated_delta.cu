@@ -10,6 +10,7 @@
 #include "capi_internal.h"
 #include "common.cuh"
 #include "kernels.h"
+#include "tc_chain.cuh"
 
 namespace db {
 namespace {
@@ -163,14 +164,14 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) delta_step_kernel(DeltaArgs a
 // Numerics.  The state has to keep f32's accuracy through f16 tensor products: k and q enter them exactly
 // (bf16 rows as f16 after a power of two per row, which loses nothing within 2^-24 of the row's largest
 // value; their lengths are applied afterwards as factors per token), and every f32 operand (S, R, U, T, P) as
-// the sum of two f16 parts after a power of two per row: 22 bits.  lo x lo products are left out (2^-22).
-// Decay sums are taken in f64: differences of f32 sums would lose what a slow decay has left.
+// the sum of two f16 parts after a power of two: per row of the state for S and R, per chunk for T and P, so that
+// 22 bits remain of what matters.  lo x lo products are left out (2^-22).  Decay sums are taken in f64: differences
+// of f32 sums would lose what a slow decay has left.
 constexpr int C = 64;                    // tokens per chunk
-constexpr int BLOCKS = 10;               // 16 x 16 blocks of a lower triangle of 64
-constexpr int TRI = BLOCKS * 256;        // halves of one triangle, in fragment order
-constexpr int FACTORS = 5 * C + 4;       // floats per chunk and head: see Factor
-// factors per token: R (times S k), O (times S q), U' (times U), rows of T, rows of P; then e^G_C
-enum Factor { F_R = 0, F_O = C, F_U = 2 * C, F_T = 3 * C, F_P = 4 * C, F_END = 5 * C };
+constexpr int BLOCKS = 10;               // 16 x 16 blocks of a lower triangle of 64, 512 bytes each, row-major
+constexpr int TRI = BLOCKS * 256;        // halves of one triangle
+// floats per chunk and head: factors per token of R (times S k), O (times S q) and U' (times U), then numbers of the chunk
+enum Factor { F_R = 0, F_O = C, F_U = 2 * C, F_DECAY = 3 * C, F_T, F_P, F_OMEGA, F_REACH, F_GROW, FACTORS = 3 * C + 8 };
 
 struct ChunkSpace {
     __half *k16, *q16;  // bf16 inputs: the rows as f16, [chunk ids][C][k_heads][D]; null for f16 inputs
@@ -212,15 +213,20 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-__device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(addr)
-                 : "memory");
-}
 // Byte offset of 16-byte piece c of row r in a tile of 256-byte rows (pieces permuted per row so that eight
 // rows of one column of pieces lie on different banks).
 __device__ __forceinline__ uint32_t tile_at(int r, int c) { return (uint32_t)(r * 256 + ((c ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T>
+__device__ __forceinline__ float lane16(uint32_t bits) {
+    const unsigned short u = (unsigned short)bits;
+    return to_f32(*reinterpret_cast<const T*>(&u));
+}
 
 // 2^e that brings a largest magnitude m into [2^14, 2^15) (1 for 0, infinities and NaN), and 2^-e.
 __device__ __forceinline__ float row_power(float m, float& back) {
@@ -228,10 +234,6 @@ __device__ __forceinline__ float row_power(float m, float& back) {
     const int k = m > 0.f && e < 128 ? min(max(14 - e, -126), 126) : 0;
     back = __uint_as_float((uint32_t)(127 - k) << 23);
     return __uint_as_float((uint32_t)(127 + k) << 23);
-}
-__device__ __forceinline__ float quad_max(float x) {
-    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
 // x, y as f16 pairs hi + lo
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -246,15 +248,23 @@ constexpr int PREP_THREADS = 128;
 constexpr int AP = 68;  // row pitch of the f32 triangles, floats (rows stay 16-byte aligned)
 
 struct PrepShared {
-    uint8_t k[C * 256], q[C * 256];  // f16 tiles
-    float A[C * AP], T[C * AP], tmp[32 * 36];
-    double G[C];
-    float beta[C], rk[C], rq[C];
+    union {
+        struct {
+            uint8_t k[C * 256], q[C * 256];  // f16 tiles
+        };
+        struct {
+            float A[C * AP], T[C * AP];      // once the products are in registers
+        };
+    };
+    float tmp[32 * 36];
+    float Gh[C], Gl[C];  // decay sums (log2) in two parts: their differences keep what one would round away
+    float beta[C], rk[C], rq[C], nk[C];
+    float top[2][PREP_THREADS / 32];
 };
 
-// T, P and the factors of one chunk, for one key head and the value heads that share it.
+// T, P and the factors of one chunk, for one key head and `heads` of the value heads that share it.
 template <typename T>
-__global__ void __launch_bounds__(PREP_THREADS) delta_prepare_kernel(DeltaArgs a, ChunkSpace w) {
+__global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArgs a, ChunkSpace w, int heads) {
     extern __shared__ __align__(16) uint8_t prep_smem[];
     PrepShared& sh = *reinterpret_cast<PrepShared*>(prep_smem);
     pdl_wait();
@@ -321,7 +331,12 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prepare_kernel(DeltaArgs a
                 *reinterpret_cast<uint4*>(dst) = y;
             }
             *reinterpret_cast<uint4*>((which ? sh.q : sh.k) + tile_at(r, c)) = y;
-            if (c == 0) (which ? sh.rq : sh.rk)[r] = (a.eps >= 0.f ? rsqrtf(ss + a.eps) : 1.f) * (which ? a.scale : 1.f) * back;
+            if (c == 0) {
+                // (a row of zeros, past the end or given, takes no part: its 1 / sqrt(eps) must not set the others' scale)
+                const float inverse = ss == 0.f ? 0.f : a.eps >= 0.f ? rsqrtf(ss + a.eps) : 1.f;
+                (which ? sh.rq : sh.rk)[r] = inverse * (which ? a.scale : 1.f) * back;
+                if (!which) sh.nk[r] = sqrtf(ss) * inverse;
+            }
         }
     }
     __syncthreads();
@@ -351,11 +366,11 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prepare_kernel(DeltaArgs a
             }
     }
 
-    const int group = a.v_heads / a.k_heads;
-    for (int hv = hk * group; hv < (hk + 1) * group; ++hv) {
+    const int group = a.v_heads / a.k_heads, first = hk * group + blockIdx.z * heads;
+    for (int hv = first; hv < min(first + heads, (hk + 1) * group); ++hv) {
         __half* tri = w.tri + ((int64_t)id * a.v_heads + hv) * 4 * TRI;
         float* factor = w.factor + ((int64_t)id * a.v_heads + hv) * FACTORS;
-        __syncthreads();  // the previous head's triangles have been read
+        __syncthreads();  // the tiles, or the previous head's triangles, have been read
         if (warp == 0) {
             double x[2];
 #pragma unroll
@@ -372,57 +387,72 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prepare_kernel(DeltaArgs a
                 if (lane >= o) sum += y;
             }
             const double all = __shfl_sync(0xffffffffu, sum, 31);
-            sh.G[2 * lane] = sum - x[1];
-            sh.G[2 * lane + 1] = sum;
+            float fu[2], reach = 0.f, largest = 0.f, grow = 0.f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int i = 2 * lane + j;
-                const double G = j ? sum : sum - x[1];
+                const double G = j ? sum : sum - x[1], two = G * 1.4426950408889634;
+                sh.Gh[i] = (float)two;
+                sh.Gl[i] = (float)(two - (double)sh.Gh[i]);
                 const float e = expf((float)G);
                 factor[F_R + i] = e * sh.rk[i];
                 factor[F_O + i] = e * sh.rq[i];
-                factor[F_U + i] = expf((float)(all - G)) * sh.rk[i];
+                const float left = expf((float)(all - G));
+                fu[j] = left * sh.rk[i];
+                grow += left * sh.nk[i];
+                reach = fmaxf(reach, e * sh.nk[i]);
+                largest = fmaxf(largest, fabsf(fu[j]));
             }
-            if (lane == 0) factor[F_END] = expf((float)all);
+            reach = warp_max(reach);
+            largest = warp_max(largest);
+            grow = warp_sum(grow);
+            float back;
+            const float omega = row_power(largest, back) * (1.f / 65536.f);  // factors of U' to at most 1/2
+            factor[F_U + 2 * lane] = fu[0] * omega;
+            factor[F_U + 2 * lane + 1] = fu[1] * omega;
+            if (lane == 0) {
+                factor[F_DECAY] = expf((float)all);
+                factor[F_OMEGA] = back * 65536.f;
+                factor[F_REACH] = 11.4f * reach;  // |S k| <= sqrt(128) |k| max |S|
+                factor[F_GROW] = omega * grow;    // |sum U'_i k_i| <= max |U| sum of the weights
+            }
         }
         __syncthreads();
-        // A into shared memory, P to its place (the fragment of the block that a lane holds is what a lane of
-        // the product P U takes)
-        float p[8][4], ptop[2] = {0.f, 0.f};
+        // A into shared memory, P to its place
+        float p[8][4], largest = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < 2 * warp + 2) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int r = warp * 16 + g + 8 * (i >> 1), c = 8 * j + 2 * t + (i & 1);
-                    const float d = c <= r ? expf((float)(sh.G[r] - sh.G[c])) * sh.rk[c] : 0.f;
+                    const float d = c <= r ? ex2((sh.Gh[r] - sh.Gh[c]) + (sh.Gl[r] - sh.Gl[c])) * sh.rk[c] : 0.f;
                     sh.A[r * AP + c] = c < r ? kk[j][i] * d * sh.rk[r] * sh.beta[r] : 0.f;
                     p[j][i] = c <= r ? qk[j][i] * d * sh.rq[r] : 0.f;
-                    ptop[i >> 1] = fmaxf(ptop[i >> 1], fabsf(p[j][i]));
+                    largest = fmaxf(largest, fabsf(p[j][i]));
                 }
             }
-        auto store = [&](float (&x)[8][4], float top0, float top1, int which, int f) {
-            float back[2];
-            const float up[2] = {row_power(quad_max(top0), back[0]), row_power(quad_max(top1), back[1])};
-            if (t == 0) {
-                factor[f + warp * 16 + g] = back[0];
-                factor[f + warp * 16 + 8 + g] = back[1];
-            }
+        largest = warp_max(largest);
+        if (lane == 0) sh.top[0][warp] = largest;
+        // two f16 parts after one power of two for the whole triangle; rows of 16 x 16 blocks
+        auto store = [&](float (&x)[8][4], const float (&top)[PREP_THREADS / 32], int which, int f) {
+            float back;
+            const float up = row_power(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), back);
+            if (tid == 0) factor[f] = back;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j <= warp) {
-                    uint4 h, l;
-                    split2(x[2 * j][0] * up[0], x[2 * j][1] * up[0], h.x, l.x);
-                    split2(x[2 * j + 1][0] * up[0], x[2 * j + 1][1] * up[0], h.y, l.y);
-                    split2(x[2 * j][2] * up[1], x[2 * j][3] * up[1], h.z, l.z);
-                    split2(x[2 * j + 1][2] * up[1], x[2 * j + 1][3] * up[1], h.w, l.w);
-                    const int at = (warp * (warp + 1) / 2 + j) * 256 + lane * 8;
-                    *reinterpret_cast<uint4*>(tri + which * TRI + at) = h;
-                    *reinterpret_cast<uint4*>(tri + (which + 1) * TRI + at) = l;
-                }
+            for (int j = 0; j < 8; ++j)
+                if (j < 2 * warp + 2)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t h, l;
+                        split2(x[j][2 * i] * up, x[j][2 * i + 1] * up, h, l);
+                        const int at = (warp * (warp + 1) / 2 + (j >> 1)) * 256 + (g + 8 * i) * 16 + 8 * (j & 1) + 2 * t;
+                        *reinterpret_cast<uint32_t*>(tri + which * TRI + at) = h;
+                        *reinterpret_cast<uint32_t*>(tri + (which + 1) * TRI + at) = l;
+                    }
         };
-        store(p, ptop[0], ptop[1], 2, F_P);
         __syncthreads();
+        store(p, sh.top[0], 2, F_P);
         // (I + A)^-1, 16 x 16 blocks on the diagonal: lane c < 16 of warp b solves for column c of block b
         if (lane < 16) {
             const float* Ab = sh.A + (16 * warp) * AP + 16 * warp;
@@ -500,7 +530,7 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prepare_kernel(DeltaArgs a
             for (int i = 0; i < 8; ++i) sh.T[(32 + r0 + i) * AP + c] = -z[i];
         }
         __syncthreads();
-        float top[2] = {0.f, 0.f};
+        largest = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < 2 * warp + 2) {
@@ -508,297 +538,473 @@ __global__ void __launch_bounds__(PREP_THREADS) delta_prepare_kernel(DeltaArgs a
                 for (int i = 0; i < 4; ++i) {
                     const int r = warp * 16 + g + 8 * (i >> 1), c = 8 * j + 2 * t + (i & 1);
                     p[j][i] = c <= r ? sh.T[r * AP + c] * sh.beta[c] : 0.f;
-                    top[i >> 1] = fmaxf(top[i >> 1], fabsf(p[j][i]));
+                    largest = fmaxf(largest, fabsf(p[j][i]));
                 }
             }
-        store(p, top[0], top[1], 0, F_T);
+        largest = warp_max(largest);
+        if (lane == 0) sh.top[1][warp] = largest;
+        __syncthreads();
+        store(p, sh.top[1], 0, F_T);
     }
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
-// One buffered chunk of delta_chunk_kernel.
-template <int WARPS>
-struct Stage {
-    uint8_t k[C * 256], q[C * 256];
-    __half tri[4 * TRI];
-    float factor[FACTORS];
-    uint8_t v[C * WARPS * 32];  // this CTA's value features, 16 per warp
+// Walks the chunks of one item and value head.  Latency bound: four products follow one another per chunk, each taking
+// f16 parts of what the one before left, so the state's 128 value rows are the 128 lanes of tensor memory, every product
+// has them as its rows (A from tensor memory, B from shared memory), and nothing of the chain passes through shared
+// memory:
+//   X = S [K; Q]^T,  R = V - e^G X_k,  U = R T^T,  S <- e^G_C S + U' K,  O = e^G X_q + U P^T
+// The state stays in tensor memory as its two parts (together f32's 24 bits); tensor-core sums enter it by one f32
+// fma, because the cores' own accumulation truncates.  The powers of two that keep parts in range come from bounds,
+// max |S k| <= sqrt(128) |k| max |S| for R, e^G_C max |S| + max |U| sum e^(G_C-G_i) |k_i| for the next S; the slack of a
+// bound (2^6) costs nothing, because f16 parts of a row scaled to 2^15 reach down to 2^-40 of it.
+// The code is kept small: what the warps of an SM run between two products has to stay in its instruction cache.
+//
+// Warps 0-7: the rows' arithmetic (thread: row 32 (w & 3) + lane; half w >> 2 of the keys, or of the tokens);
+// 8: MMA issue and tensor memory; 9-11: loads of the next chunk.
+// Tensor memory columns: S parts 0-127, U' K 128-255, U 256-319 (then U' parts in its place), P U 320-383, X_k 384-447
+// (then R parts, then U parts), X_q 448-511.  Parts of 32 values lie in 32 columns: 16 of first parts (two values to a
+// column), 16 of second parts.
+constexpr int CHAIN_THREADS = 384, LOADERS = 96;
+constexpr uint64_t DRAIN_NS = 100000000ull;
+constexpr int KQ_BYTES = 2 * C * D * 2, KQ_HALF = KQ_BYTES / 2, TRI_BYTES = C * C * 2;
+
+struct ChainStage {
+    uint8_t kq[KQ_BYTES];       // rows 0-63 K, 64-127 Q; two columns of 64 keys x 128 rows, 128-byte swizzle
+    uint8_t tri[4][TRI_BYTES];  // T hi, T lo, P hi, P lo: 64 rows of 128 bytes, 128-byte swizzle
+    uint8_t v[C * D * 2];
 };
+enum ChainBar { CB_FULL = 0, CB_EMPTY = 2, CB_S = 4, CB_X, CB_R, CB_U, CB_W, CB_UU, CB_D, CB_PU, CB_DONE, CB_END, CHAIN_BARS };
+struct ChainShared {
+    uint64_t bars[CHAIN_BARS];
+    float factor[2][FACTORS];
+    float top[3][2][D];  // largest magnitudes of S, U and the next chunk's V: [half][row]
+    uint32_t tmem;
+    int abort;
+};
+constexpr int CHAIN_SMEM = 1024 + 2 * sizeof(ChainStage) + sizeof(ChainShared);
+static_assert(sizeof(ChainStage) % 1024 == 0 && CHAIN_SMEM <= 232448, "shared memory");
 
-// Walks the chunks of one item and value head for 16 WARPS of the state's 128 value rows.  All products are
-// formed transposed (rows = value features), so a warp keeps its 16 rows of the state in its accumulators,
-// feeds them to the next product as they are, and never waits for another warp; what the rows share (k, q,
-// T, P) is read from shared memory, the next chunk's while this one is worked on.
-template <typename T, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, 1) delta_chunk_kernel(DeltaArgs a, ChunkSpace w) {
-    extern __shared__ __align__(16) uint8_t chunk_smem[];
-    Stage<WARPS>* stage = reinterpret_cast<Stage<WARPS>*>(chunk_smem);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int hv = blockIdx.y, b = blockIdx.z, hk = hv / (a.v_heads / a.k_heads);
-    const int slice = blockIdx.x * 16 * WARPS, d0 = slice + 16 * warp;  // first value row of the CTA, the warp
+// B operand with N contiguous (MN-major), 128-byte swizzle: rows of 128 bytes hold 64 values of N for one K; 8-row atoms
+// are 1024 bytes apart, the next 64 values of N KQ_HALF bytes.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (uint64_t)((KQ_HALF >> 4) & 0x3FFFu) << 16 |
+           (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 | (uint64_t)2u << 61;
+}
+// 32 values (16 pairs) as f16 parts: 16 columns of first parts, 16 of second ones.
+__device__ __forceinline__ void parts32(const uint64_t (&x)[16], uint32_t (&r)[32]) {
+    const uint64_t minus = f2_pack(0xbf800000u, 0xbf800000u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const __half2 h = __floats2half2_rn(f2_lo(x[i]), f2_hi(x[i]));
+        const float2 f = __half22float2(h);
+        const uint64_t left = f2_fma(f2_pack(__float_as_uint(f.x), __float_as_uint(f.y)), minus, x[i]);
+        const __half2 l = __floats2half2_rn(f2_lo(left), f2_hi(left));
+        r[i] = *reinterpret_cast<const uint32_t*>(&h);
+        r[16 + i] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+}
+__device__ __forceinline__ uint64_t both(float x) { return f2_pack(__float_as_uint(x), __float_as_uint(x)); }
+// Two factors of neighbouring tokens from shared memory.
+__device__ __forceinline__ uint64_t pair_at(const float* f) { return *reinterpret_cast<const uint64_t*>(f); }
+// The larger magnitude of a pair.
+__device__ __forceinline__ float pair_top(uint64_t x, float top) { return fmaxf(top, fmaxf(fabsf(f2_lo(x)), fabsf(f2_hi(x)))); }
+
+template <typename T>
+__global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs a, ChunkSpace w, int* err) {
+    extern __shared__ uint8_t chain_smem[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(chain_smem) + 1023) & ~uintptr_t(1023));
+    ChainStage* stages = reinterpret_cast<ChainStage*>(smem);
+    ChainShared& sh = *reinterpret_cast<ChainShared*>(smem + 2 * sizeof(ChainStage));
+    volatile int* abort_flag = &sh.abort;
+    const int tid = threadIdx.x, lane = tid & 31, warp = chain::warp_index();
+    const int hv = blockIdx.x, b = blockIdx.y, hk = hv / (a.v_heads / a.k_heads);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.bars[CB_FULL + i], LOADERS / 32);
+            mbar_init(&sh.bars[CB_EMPTY + i], 1 + 8);
+        }
+        for (int i : {CB_S, CB_R, CB_W, CB_UU}) mbar_init(&sh.bars[i], 8);
+        for (int i : {CB_X, CB_U, CB_D, CB_PU, CB_DONE}) mbar_init(&sh.bars[i], 1);
+        mbar_init(&sh.bars[CB_END], CHAIN_THREADS / 32);
+        sh.abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(&sh.tmem, 512);
+        tmem_relinquish();
+    }
     pdl_wait();
     pdl_trigger();
     int start, end;
     item_rows(a, b, start, end);
     const int chunks = (end - start + C - 1) / C;
     const int64_t id0 = start / C + b;
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
 
-    float S[16][4];  // tile j: keys 8 j + 2 t, + 1 of value rows g (0, 1) and g + 8 (2, 3)
-    const int64_t at = ((int64_t)hv * D + d0 + g) * D + 2 * t;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        float2 x = make_float2(0.f, 0.f), y = x;
-        if (a.state_in) {
-            const float* s = a.state_in + (int64_t)b * a.state_stride + at + 8 * j;
-            x = *reinterpret_cast<const float2*>(s);
-            y = *reinterpret_cast<const float2*>(s + 8 * D);
-        }
-        S[j][0] = x.x, S[j][1] = x.y, S[j][2] = y.x, S[j][3] = y.y;
-    }
-
-    constexpr int NT = 32 * WARPS;
-    auto fetch = [&](int c) {
-        Stage<WARPS>& st = stage[c & 1];
-        const int row0 = start + c * C, n = min(C, end - row0);
-        const int64_t id = id0 + c;
-        const __half* k16 = w.k16 ? w.k16 + (id * C * a.k_heads + hk) * D
-                                  : static_cast<const __half*>(a.k) + (int64_t)row0 * a.ldk + (int64_t)hk * D;
-        const __half* q16 = w.q16 ? w.q16 + (id * C * a.k_heads + hk) * D
-                                  : static_cast<const __half*>(a.q) + (int64_t)row0 * a.ldq + (int64_t)hk * D;
-        const int64_t ldk = w.k16 ? (int64_t)a.k_heads * D : a.ldk, ldq = w.q16 ? (int64_t)a.k_heads * D : a.ldq;
-        const uint32_t sk = smem_u32(st.k), sq = smem_u32(st.q), sv = smem_u32(st.v);
-        for (int e = tid; e < C * 16; e += NT) {
-            const int r = e >> 4, p = e & 15;
-            const bool there = r < n;
-            const int rr = there ? r : 0;
-            cp_async16(sk + tile_at(r, p), k16 + rr * ldk + 8 * p, there);
-            cp_async16(sq + tile_at(r, p), q16 + rr * ldq + 8 * p, there);
-        }
-        const T* v = static_cast<const T*>(a.v) + (int64_t)row0 * a.ldv + (int64_t)hv * D + slice;
-        for (int e = tid; e < C * 2 * WARPS; e += NT) {
-            const int r = e / (2 * WARPS), p = e % (2 * WARPS);
-            const bool there = r < n;
-            cp_async16(sv + r * WARPS * 32 + ((p ^ (r & (2 * WARPS - 1) & 7)) << 4), v + (there ? r : 0) * a.ldv + 8 * p, there);
-        }
-        const uint8_t* tri = reinterpret_cast<const uint8_t*>(w.tri + (id * a.v_heads + hv) * 4 * TRI);
-        const uint32_t stri = smem_u32(st.tri);
-        for (int e = tid; e < 4 * TRI * 2 / 16; e += NT) cp_async16(stri + 16 * e, tri + 16 * e, true);
-        const uint8_t* f = reinterpret_cast<const uint8_t*>(w.factor + (id * a.v_heads + hv) * FACTORS);
-        const uint32_t sf = smem_u32(st.factor);
-        for (int e = tid; e < FACTORS / 4; e += NT) cp_async16(sf + 16 * e, f + 16 * e, true);
-        cp_async_commit();
-    };
-    if (chunks > 0) fetch(0);
-    for (int c = 0; c < chunks; ++c) {
-        if (c + 1 < chunks) {
-            fetch(c + 1);
-            cp_async_wait<1>();
-        } else {
-            cp_async_wait<0>();
-        }
-        __syncthreads();
-        const Stage<WARPS>& st = stage[c & 1];
-        const uint32_t sk = smem_u32(st.k), sq = smem_u32(st.q), sv = smem_u32(st.v);
-        const float* f = st.factor;
-
-        // X = S [K; Q]^T: tiles 0-7 tokens of K, 8-15 of Q
-        float X[16][4];
-        float up[2], back[2];
-        {
-            float top[2] = {0.f, 0.f};
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                top[0] = fmaxf(top[0], fmaxf(fabsf(S[j][0]), fabsf(S[j][1])));
-                top[1] = fmaxf(top[1], fmaxf(fabsf(S[j][2]), fabsf(S[j][3])));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) X[j][i] = 0.f;
+    if (warp >= 9) {
+        // ---------------------------------------------------------------- loads
+        const int lt = tid - 9 * 32;
+        bool ok = true;
+        for (int c = 0; c <= chunks && ok; ++c) {
+            if (c > 0) {
+                // the chunk before has landed: to the tensor core's view, then on
+                cp_async_wait<0>();
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.bars[CB_FULL + ((c - 1) & 1)]);
             }
-            up[0] = row_power(quad_max(top[0]), back[0]);
-            up[1] = row_power(quad_max(top[1]), back[1]);
-        }
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            uint32_t h[4], l[4];
-            split2(S[2 * s][0] * up[0], S[2 * s][1] * up[0], h[0], l[0]);
-            split2(S[2 * s][2] * up[1], S[2 * s][3] * up[1], h[1], l[1]);
-            split2(S[2 * s + 1][0] * up[0], S[2 * s + 1][1] * up[0], h[2], l[2]);
-            split2(S[2 * s + 1][2] * up[1], S[2 * s + 1][3] * up[1], h[3], l[3]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                uint32_t bb[4];
-                ldmatrix4(bb, (j < 4 ? sk : sq) +
-                                  tile_at(16 * (j & 3) + ((lane >> 4) << 3) + (lane & 7), 2 * s + ((lane >> 3) & 1)));
-                mma16816(X[2 * j], l, bb[0], bb[1]);
-                mma16816(X[2 * j + 1], l, bb[2], bb[3]);
-                mma16816(X[2 * j], h, bb[0], bb[1]);
-                mma16816(X[2 * j + 1], h, bb[2], bb[3]);
-            }
-        }
-        // R = V - e^G S k, in place of the K half
-        float top[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            // V^T fragments of tokens 16 j .. + 15: value rows 0-7, 8-15 of tokens 0-7, then of 8-15
-            uint32_t vv[4];
-            const int r = 16 * j + ((lane >> 4) << 3) + (lane & 7), p = 2 * warp + ((lane >> 3) & 1);
-            ldmatrix4t(vv, sv + r * WARPS * 32 + ((p ^ (r & (2 * WARPS - 1) & 7)) << 4));
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                const float2 ff = *reinterpret_cast<const float2*>(&f[F_R + 16 * j + 8 * hh + 2 * t]);
-                float (&x)[4] = X[2 * j + hh];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t word = vv[2 * hh + (i >> 1)];
-                    const unsigned short u = (unsigned short)(i & 1 ? word >> 16 : word & 0xffffu);
-                    x[i] = fmaf(-((i & 1) ? ff.y : ff.x), x[i] * back[i >> 1], to_f32(*reinterpret_cast<const T*>(&u)));
-                    top[i >> 1] = fmaxf(top[i >> 1], fabsf(x[i]));
+            if (c < chunks) {
+                const int s = c & 1;
+                ok = chain::warp_wait(&sh.bars[CB_EMPTY + s], ((c >> 1) & 1) ^ 1u, abort_flag, err, DB_DEV_ERR_TIMEOUT_TMA);
+                if (!ok) break;
+                ChainStage& st = stages[s];
+                const int row0 = start + c * C, n = min(C, end - row0);
+                const int64_t id = id0 + c;
+                const __half* k16 = w.k16 ? w.k16 + (id * C * a.k_heads + hk) * D
+                                          : static_cast<const __half*>(a.k) + (int64_t)row0 * a.ldk + (int64_t)hk * D;
+                const __half* q16 = w.q16 ? w.q16 + (id * C * a.k_heads + hk) * D
+                                          : static_cast<const __half*>(a.q) + (int64_t)row0 * a.ldq + (int64_t)hk * D;
+                const int64_t ldk = w.k16 ? (int64_t)a.k_heads * D : a.ldk, ldq = w.q16 ? (int64_t)a.k_heads * D : a.ldq;
+                const uint32_t skq = smem_u32(st.kq), sv = smem_u32(st.v), stri = smem_u32(st.tri);
+                // 16-byte piece p of row r: column p / 8, place p % 8 ^ r % 8
+                const int p16 = lt & 15, r16 = lt >> 4;
+                for (int r = r16; r < C; r += LOADERS / 16) {
+                    const bool there = r < n;
+                    const int rr = there ? r : 0;
+                    const uint32_t to = skq + (p16 >> 3) * KQ_HALF + r * 128 + (((p16 & 7) ^ (r & 7)) << 4);
+                    cp_async16_if(to, k16 + rr * ldk + 8 * p16, there);
+                    cp_async16_if(to + C * 128, q16 + rr * ldq + 8 * p16, there);
+                    cp_async16_if(sv + r * (D * 2) + 16 * p16,
+                                  static_cast<const T*>(a.v) + (int64_t)(row0 + rr) * a.ldv + (int64_t)hv * D + 8 * p16, there);
                 }
+                // the triangles' blocks: 32 pieces each, row x of the block, half y
+                const __half* tri = w.tri + (id * a.v_heads + hv) * 4 * TRI;
+                const int x = lane >> 1, y = lane & 1;
+                for (int e = warp - 9; e < 4 * BLOCKS; e += LOADERS / 32) {
+                    const int which = e / BLOCKS, blk = e % BLOCKS;
+                    const int I = blk >= 6 ? 3 : blk >= 3 ? 2 : blk >= 1 ? 1 : 0, J = blk - I * (I + 1) / 2;
+                    cp_async16_if(stri + which * TRI_BYTES + (16 * I + x) * 128 + (((2 * J + y) ^ (x & 7)) << 4),
+                                  tri + which * TRI + blk * 256 + x * 16 + y * 8, true);
+                }
+                const float* f = w.factor + (id * a.v_heads + hv) * FACTORS;
+                for (int e = lt; e < FACTORS / 4; e += LOADERS) cp_async16_if(smem_u32(&sh.factor[s][4 * e]), f + 4 * e, true);
+                cp_async_commit();
             }
         }
-        float ru[2], rb[2];
-        ru[0] = row_power(quad_max(top[0]), rb[0]);
-        ru[1] = row_power(quad_max(top[1]), rb[1]);
-        uint32_t ah[4][4], al[4][4];
-        auto split_rows = [&](const float (&x0)[4], const float (&x1)[4], float u0, float u1, uint32_t (&h)[4], uint32_t (&l)[4]) {
-            split2(x0[0] * u0, x0[1] * u0, h[0], l[0]);
-            split2(x0[2] * u1, x0[3] * u1, h[1], l[1]);
-            split2(x1[0] * u0, x1[1] * u0, h[2], l[2]);
-            split2(x1[2] * u1, x1[3] * u1, h[3], l[3]);
+        cp_async_wait<0>();
+    } else if (warp == 8) {
+        // ---------------------------------------------------------------- MMA issue
+        bool ok = true;
+        auto wait = [&](int bar, uint32_t parity) {
+            ok = ok && chain::warp_wait(&sh.bars[bar], parity, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
+            tc_fence_after();
+            return ok;
         };
+        constexpr uint32_t ID_X = idesc_f16_f32(128, 128), ID_D = idesc_f16_f32(128, 128) | (1u << 16);  // (B MN-major)
+        for (int c = 0; c < chunks && ok; ++c) {
+            const int s = c & 1;
+            const uint32_t ph = c & 1;
+            const uint64_t dKQ = sw128_desc(smem_u32(stages[s].kq)), dK = mn_desc(smem_u32(stages[s].kq)),
+                           dT = sw128_desc(smem_u32(stages[s].tri));
+            // D (128 x 64) = (parts at a_tm) x (a triangle)^T: keys 16 s.. of the sum meet rows 16 s.. only
+            auto triangle = [&](uint32_t d_tm, uint32_t a_tm, int which) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) split_rows(X[2 * s], X[2 * s + 1], ru[0], ru[1], ah[s], al[s]);
-        // Y += (a triangle of T or P) applied to the rows in ah, al
-        auto triangle = [&](float (&Y)[8][4], int which) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) Y[j][i] = 0.f;
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int j = s; j < 4; ++j) {
-                    const int blk = (j * (j + 1) / 2 + s) * 256 + lane * 8;
-                    const uint4 bh = *reinterpret_cast<const uint4*>(st.tri + which * TRI + blk);
-                    const uint4 bl = *reinterpret_cast<const uint4*>(st.tri + (which + 1) * TRI + blk);
-                    mma16816(Y[2 * j], al[s], bh.x, bh.y);
-                    mma16816(Y[2 * j + 1], al[s], bh.z, bh.w);
-                    mma16816(Y[2 * j], ah[s], bl.x, bl.y);
-                    mma16816(Y[2 * j + 1], ah[s], bl.z, bl.w);
-                    mma16816(Y[2 * j], ah[s], bh.x, bh.y);
-                    mma16816(Y[2 * j + 1], ah[s], bh.z, bh.w);
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t at = a_tm + 32u * (k >> 1) + 8u * (k & 1), id = idesc_f16_f32(128, 64 - 16 * k);
+                    const uint64_t hi = dT + (uint64_t)((which * TRI_BYTES + k * 2048 + k * 32) >> 4), lo = hi + (TRI_BYTES >> 4);
+                    chain::umma_f16_ts(d_tm + 16u * k, at + 16u, hi, id, k > 0);
+                    chain::umma_f16_ts(d_tm + 16u * k, at, lo, id, 1);
+                    chain::umma_f16_ts(d_tm + 16u * k, at, hi, id, 1);
                 }
+            };
+            if (c > 0) wait(CB_PU, ph ^ 1u);  // (X goes where its U parts were)
+            wait(CB_FULL + s, (c >> 1) & 1);
+            if (!wait(CB_S, ph)) break;
+            if (chain::elect()) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const uint32_t at = tmem + 32u * (k >> 1) + 8u * (k & 1);
+                    const uint64_t d = dKQ + (uint64_t)(((k >> 2) * KQ_HALF + (k & 3) * 32) >> 4);
+                    chain::umma_f16_ts(tmem + 384u, at + 16u, d, ID_X, k > 0);
+                    chain::umma_f16_ts(tmem + 384u, at, d, ID_X, 1);
+                }
+                umma_commit(&sh.bars[CB_X]);
+            }
+            __syncwarp();
+            if (!wait(CB_R, ph)) break;
+            if (chain::elect()) {
+                triangle(tmem + 256u, tmem + 384u, 0);
+                umma_commit(&sh.bars[CB_U]);
+            }
+            __syncwarp();
+            if (!wait(CB_W, ph)) break;
+            if (chain::elect()) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t at = tmem + 256u + 32u * (k >> 1) + 8u * (k & 1);
+                    const uint64_t d = dK + (uint64_t)((k * 2048) >> 4);
+                    chain::umma_f16_ts(tmem + 128u, at + 16u, d, ID_D, k > 0);
+                    chain::umma_f16_ts(tmem + 128u, at, d, ID_D, 1);
+                }
+                umma_commit(&sh.bars[CB_D]);
+            }
+            __syncwarp();
+            if (!wait(CB_UU, ph)) break;
+            if (chain::elect()) {
+                triangle(tmem + 320u, tmem + 384u, 2);
+                umma_commit(&sh.bars[CB_PU]);
+                umma_commit(&sh.bars[CB_EMPTY + s]);
+            }
+            __syncwarp();
+        }
+        // every MMA issued has completed before tensor memory is released
+        if (chain::elect()) {
+            umma_commit(&sh.bars[CB_DONE]);
+            mbar_wait_drain(&sh.bars[CB_DONE], 0, DRAIN_NS);
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------------- the rows' arithmetic
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        bool ok = true;
+        auto wait = [&](int bar, uint32_t parity) {
+            ok = ok && chain::warp_wait(&sh.bars[bar], parity, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
+            tc_fence_after();
+            return ok;
         };
-        float U[8][4];
-        triangle(U, 0);
-        float utop[2] = {0.f, 0.f}, wtop[2] = {0.f, 0.f};
+        auto ready = [&](int bar) {  // what this warp stored in tensor memory may be read
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[bar]);
+        };
+        // the halves' largest magnitudes meet in shared memory
+        float s_top, u_top = 0.f, v_top;
+        auto meet = [&](float s, float u, float v) {
+            sh.top[0][half][row] = s;
+            sh.top[1][half][row] = u;
+            sh.top[2][half][row] = v;
+            named_barrier_sync(1, 256);
+            s_top = fmaxf(s, sh.top[0][half ^ 1][row]);
+            u_top = fmaxf(u, sh.top[1][half ^ 1][row]);
+            v_top = fmaxf(v, sh.top[2][half ^ 1][row]);
+        };
+        auto values_top = [&](int s) {
+            const unsigned short* v = reinterpret_cast<const unsigned short*>(stages[s].v) + 32 * half * D + row;
+            uint32_t top = 0;
+#pragma unroll 8
+            for (int i = 0; i < 32; ++i) top = max(top, (uint32_t)v[i * D] & 0x7fffu);
+            return lane16<T>(top);
+        };
+        // a power of two 2^e (e of a float's exponent field) and the next one for a largest magnitude of `bound`
+        int up_e = 0;  // S parts hold S 2^up_e
+        auto power = [](int e) { return __uint_as_float((uint32_t)(127 + e) << 23); };
+        auto retarget = [&](float bound) {  // the step that brings bound to [2^14, 2^15)
+            const int e = (int)((__float_as_uint(bound) >> 23) & 0xff) - 127;
+            const int step = bound > 0.f && e < 128 ? 14 - e : 0;
+            return min(max(max(step, -100), -100 - up_e), min(100, 100 - up_e));
+        };
+        const int64_t at = ((int64_t)hv * D + row) * D + 64 * half;
+        if (chunks > 0) {
+            // the state that is given, looked at once for its largest value, then split
+            float top = 0.f;
+            const float* in = a.state_in ? a.state_in + (int64_t)b * a.state_stride + at : nullptr;
+            if (in)
+#pragma unroll 4
+                for (int i = 0; i < 16; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(in + 4 * i);
+                    top = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), top);
+                }
+            ok = chain::warp_wait(&sh.bars[CB_FULL], 0, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
+            meet(top, 0.f, ok ? values_top(0) : 0.f);
+            up_e = retarget(s_top);
+            s_top *= power(up_e);
+            const uint64_t up = both(power(up_e));
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+                uint64_t x[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 ft = *reinterpret_cast<const float2*>(&f[F_T + 8 * j + 2 * t]);
-            const float2 fu = *reinterpret_cast<const float2*>(&f[F_U + 8 * j + 2 * t]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                U[j][i] *= rb[i >> 1] * ((i & 1) ? ft.y : ft.x);
-                X[j][i] = U[j][i] * ((i & 1) ? fu.y : fu.x);  // what the state takes, over k
-                utop[i >> 1] = fmaxf(utop[i >> 1], fabsf(U[j][i]));
-                wtop[i >> 1] = fmaxf(wtop[i >> 1], fabsf(X[j][i]));
+                for (int i = 0; i < 16; ++i) x[i] = in ? f2_mul(*reinterpret_cast<const uint64_t*>(in + 32 * q + 2 * i), up) : 0ull;
+                uint32_t r[32];
+                parts32(x, r);
+                chain::tmem_st32(tm + 64u * half + 32u * q, r);
             }
         }
-        // the state: S <- e^G_C S + U'^T K, eight tiles of keys at a time
-        float wu[2], wb[2];
-        wu[0] = row_power(quad_max(wtop[0]), wb[0]);
-        wu[1] = row_power(quad_max(wtop[1]), wb[1]);
+        float Oq[32], o_scale = 0.f;
+        // chunk c's outputs: e^G S q is there, P U joins it
+        auto output = [&](int c) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(tm + 320u + 32u * half, r);
+            tmem_wait_ld(r);
+            const int row0 = start + c * C + 32 * half, n = end - row0;
+            T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.ldo + (int64_t)hv * D + row;
+            if (n >= 32) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) split_rows(X[2 * s], X[2 * s + 1], wu[0], wu[1], ah[s], al[s]);
-        const float decay = f[F_END];
+                for (int i = 0; i < 32; ++i, out += a.ldo) from_f32(fmaf(__uint_as_float(r[i]), o_scale, Oq[i]), *out);
+            } else {
 #pragma unroll
-        for (int part = 0; part < 4; ++part) {
-            float Y[4][4];
+                for (int i = 0; i < 32; ++i)
+                    if (i < n) from_f32(fmaf(__uint_as_float(r[i]), o_scale, Oq[i]), out[i * a.ldo]);
+            }
+        };
+        if (chunks > 0) ready(CB_S);
+        // (after an abort the waits return at once and the rest runs on: every warp meets the barriers as often as the others)
+        for (int c = 0; c < chunks; ++c) {
+            const int s = c & 1;
+            const uint32_t ph = c & 1;
+            const float* f = sh.factor[s];
+            // while X is formed: the chunk before goes out
+            if (c > 0) {
+                wait(CB_PU, ph ^ 1u);
+                output(c - 1);
+            }
+            // R = V - e^G S k
+            const float s_back = power(-up_e);
+            float r_back;
+            const float r_up = row_power(v_top + f[F_REACH] * (s_top * s_back), r_back);
+            wait(CB_X, ph);
+            uint32_t r[32];
+            uint64_t x[16];
+            tmem_ld_32x32b_x32(tm + 384u + 32u * half, r);
+            tmem_wait_ld(r);
+            {
+                const uint64_t k = both(-s_back * r_up), up = both(r_up);
+                const unsigned short* v = reinterpret_cast<const unsigned short*>(stages[s].v) + 32 * half * D + row;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int i = 0; i < 16; ++i) {
+                    const uint64_t vv = f2_pack(__float_as_uint(lane16<T>(v[2 * i * D])), __float_as_uint(lane16<T>(v[(2 * i + 1) * D])));
+                    x[i] = f2_fma(f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k), pair_at(f + F_R + 32 * half + 2 * i), f2_mul(vv, up));
+                }
+                parts32(x, r);
+            }
+            chain::tmem_st32(tm + 384u + 32u * half, r);
+            ready(CB_R);
+            // while U is formed: e^G S q
+            tmem_ld_32x32b_x32(tm + 448u + 32u * half, r);
+            tmem_wait_ld(r);
+            {
+                const uint64_t k = both(s_back);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) Y[j][i] = 0.f;
+                for (int i = 0; i < 16; ++i) {
+                    const uint64_t o = f2_mul(f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k), pair_at(f + F_O + 32 * half + 2 * i));
+                    Oq[2 * i] = f2_lo(o), Oq[2 * i + 1] = f2_hi(o);
+                }
+            }
+            // U in units of 2^22 / (r_up x T's power): at most 2^14 whatever R and T are
+            const float u_back = 4194304.f * r_back * f[F_T], grow = f[F_GROW];
+            o_scale = u_back * f[F_P];
+            const float s_scale = u_back * f[F_OMEGA] * power(up_e), decay = f[F_DECAY];
+            wait(CB_U, ph);
+            tmem_ld_32x32b_x32(tm + 256u + 32u * half, r);
+            tmem_wait_ld(r);
+            float top = 0.f;
+            {
+                const uint64_t k = both(2.3841858e-7f);
+                uint64_t y[16];
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k);
+                    y[i] = f2_mul(x[i], pair_at(f + F_U + 32 * half + 2 * i));
+                }
+                parts32(y, r);
+            }
+            chain::tmem_st32(tm + 256u + 32u * half, r);
+            ready(CB_W);
+            parts32(x, r);
+            chain::tmem_st32(tm + 384u + 32u * half, r);
+            ready(CB_UU);
+            // while U' K is formed: what the next chunk's powers of two need
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    // K^T: keys 32 part + 16 j .. + 15 of tokens 16 s .. + 15
-                    uint32_t bb[4];
-                    ldmatrix4t(bb, sk + tile_at(16 * s + ((lane >> 3) & 1) * 8 + (lane & 7), 4 * part + 2 * j + (lane >> 4)));
-                    mma16816(Y[2 * j], al[s], bb[0], bb[1]);
-                    mma16816(Y[2 * j + 1], al[s], bb[2], bb[3]);
-                    mma16816(Y[2 * j], ah[s], bb[0], bb[1]);
-                    mma16816(Y[2 * j + 1], ah[s], bb[2], bb[3]);
+            for (int i = 0; i < 16; ++i) top = pair_top(x[i], top);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[CB_EMPTY + s]);  // this warp is done with the chunk's values and factors
+            float v_next = 0.f;
+            if (c + 1 < chunks) {
+                wait(CB_FULL + (s ^ 1), ((c + 1) >> 1) & 1);
+                v_next = values_top(s ^ 1);
+            }
+            const float before = s_top;
+            meet(0.f, top, v_next);
+            const int step = retarget(decay * before + u_top * grow * fabsf(s_scale));
+            up_e += step;
+            const uint64_t keep = both(decay * power(step)), add = both(s_scale * power(step));
+            // S <- e^G_C S + U' K
+            wait(CB_D, ph);
+            top = 0.f;
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+                uint32_t d[32];
+                tmem_ld_32x32b_x32(tm + 64u * half + 32u * q, r);
+                tmem_ld_32x32b_x32(tm + 128u + 64u * half + 32u * q, d);
+                tmem_wait_ld(r);
+                chain::tie32(d);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r[i])), l = __half22float2(*reinterpret_cast<const __half2*>(&r[16 + i]));
+                    const uint64_t old = f2_add(f2_pack(__float_as_uint(h.x), __float_as_uint(h.y)), f2_pack(__float_as_uint(l.x), __float_as_uint(l.y)));
+                    x[i] = f2_fma(f2_pack(d[2 * i], d[2 * i + 1]), add, f2_mul(old, keep));
+                    top = pair_top(x[i], top);
+                }
+                parts32(x, r);
+                chain::tmem_st32(tm + 64u * half + 32u * q, r);
+            }
+            sh.top[0][half][row] = top;
+            if (c + 1 < chunks) {
+                ready(CB_S);
+            } else {
+                tmem_wait_st();
+            }
+            named_barrier_sync(1, 256);
+            s_top = fmaxf(top, sh.top[0][half ^ 1][row]);
+        }
+        if (ok && chunks > 0 && wait(CB_PU, (chunks - 1) & 1)) output(chunks - 1);
+        if (a.state_out && ok) {
+            float* o = a.state_out + (int64_t)b * a.v_heads * D * D + at;
+            const float back = power(-up_e);
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+                uint32_t r[32];
+                if (chunks > 0) {
+                    tmem_ld_32x32b_x32(tm + 64u * half + 32u * q, r);
+                    tmem_wait_ld(r);
                 }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[4 * part + j][i] = fmaf(S[4 * part + j][i], decay, Y[j][i] * wb[i >> 1]);
-        }
-        // O = e^G S0 q + P U
-        float uu[2], ub[2];
-        uu[0] = row_power(quad_max(utop[0]), ub[0]);
-        uu[1] = row_power(quad_max(utop[1]), ub[1]);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) split_rows(U[2 * s], U[2 * s + 1], uu[0], uu[1], ah[s], al[s]);
-        float O[8][4];
-        triangle(O, 2);
-        const int row0 = start + c * C, n = end - row0;
-        T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.ldo + (int64_t)hv * D + d0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 fo = *reinterpret_cast<const float2*>(&f[F_O + 8 * j + 2 * t]);
-            const float2 fp = *reinterpret_cast<const float2*>(&f[F_P + 8 * j + 2 * t]);
-            uint32_t word[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = fmaf((i & 1) ? fo.y : fo.x, X[8 + j][i] * back[i >> 1],
-                                     O[j][i] * (ub[i >> 1] * ((i & 1) ? fp.y : fp.x)));
-                T y;
-                from_f32(x, y);
-                const uint32_t u = *reinterpret_cast<const unsigned short*>(&y);
-                if (i & 1) word[i >> 1] |= u << 16; else word[i >> 1] = u;
-            }
-            // transposed: token g, value rows 2 t, 2 t + 1 of either half
-            uint32_t lo8, hi8;
-            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(lo8) : "r"(word[0]));
-            asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(hi8) : "r"(word[1]));
-            if (8 * j + g < n) {
-                T* dst = out + (int64_t)(8 * j + g) * a.ldo + 2 * t;
-                *reinterpret_cast<uint32_t*>(dst) = lo8;
-                *reinterpret_cast<uint32_t*>(dst + 8) = hi8;
+                for (int i = 0; i < 8; ++i) {
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (chunks > 0) {
+                        const float2 h0 = __half22float2(*reinterpret_cast<const __half2*>(&r[2 * i])), l0 = __half22float2(*reinterpret_cast<const __half2*>(&r[16 + 2 * i]));
+                        const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&r[2 * i + 1])), l1 = __half22float2(*reinterpret_cast<const __half2*>(&r[17 + 2 * i]));
+                        y = make_float4((h0.x + l0.x) * back, (h0.y + l0.y) * back, (h1.x + l1.x) * back, (h1.y + l1.y) * back);
+                    } else if (a.state_in) {
+                        y = *reinterpret_cast<const float4*>(a.state_in + (int64_t)b * a.state_stride + at + 32 * q + 4 * i);
+                    }
+                    *reinterpret_cast<float4*>(o + 32 * q + 4 * i) = y;
+                }
             }
         }
-        __syncthreads();  // the stage may be filled again
     }
-    if (a.state_out) {
-        float* s = a.state_out + (int64_t)b * a.v_heads * D * D + at;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            *reinterpret_cast<float2*>(s + 8 * j) = make_float2(S[j][0], S[j][1]);
-            *reinterpret_cast<float2*>(s + 8 * j + 8 * D) = make_float2(S[j][2], S[j][3]);
-        }
+    // through an mbarrier: every role is done with tensor memory before it is released
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.bars[CB_END]);
+    if (warp == 8) {
+        if (lane == 0) mbar_wait_drain(&sh.bars[CB_END], 0, DB_WAIT_LIMIT_NS);
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
     }
 }
 
 // Up to this many tokens per item the recurrence is faster than a chunk.
 constexpr int STEP_TOKENS = DB_DELTA_STEP_TOKENS;
-
-template <typename T, int WARPS>
-cudaError_t launch_chunks(const DeltaArgs& a, const ChunkSpace& w, cudaStream_t stream) {
-    auto kernel = delta_chunk_kernel<T, WARPS>;
-    const int smem = 2 * sizeof(Stage<WARPS>);
-    cudaError_t e = db_set_max_smem(reinterpret_cast<const void*>(kernel), smem);
-    if (e != cudaSuccess) return e;
-    return db_launch_pdl(kernel, dim3(D / (16 * WARPS), a.v_heads, a.items), dim3(32 * WARPS), smem, stream, a, w);
-}
 
 template <typename T>
 cudaError_t launch(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
@@ -810,11 +1016,16 @@ cudaError_t launch(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     chunk_space(a.items, a.rows, a.k_heads, a.v_heads, !std::is_same<T, __half>::value, static_cast<uint8_t*>(workspace), &w);
     cudaError_t e = db_set_max_smem(reinterpret_cast<const void*>(delta_prepare_kernel<T>), sizeof(PrepShared));
     if (e != cudaSuccess) return e;
-    e = db_launch_pdl(delta_prepare_kernel<T>, dim3((unsigned)chunk_ids(a.rows, a.items), a.k_heads), dim3(PREP_THREADS),
-                      sizeof(PrepShared), stream, a, w);
+    // a CTA per value head while that still finds idle SMs, else one for all that share a key head
+    const int64_t ids = chunk_ids(a.rows, a.items);
+    const int group = a.v_heads / a.k_heads, heads = ids * a.k_heads < 4 * db_num_sms() ? 1 : group;
+    e = db_launch_pdl(delta_prepare_kernel<T>, dim3((unsigned)ids, a.k_heads, (group + heads - 1) / heads), dim3(PREP_THREADS),
+                      sizeof(PrepShared), stream, a, w, heads);
     if (e != cudaSuccess) return e;
-    // a head per CTA where heads fill the SMs, else half a head
-    return a.v_heads * a.items >= db_num_sms() ? launch_chunks<T, 8>(a, w, stream) : launch_chunks<T, 4>(a, w, stream);
+    e = db_set_max_smem(reinterpret_cast<const void*>(delta_chain_kernel<T>), CHAIN_SMEM);
+    if (e != cudaSuccess) return e;
+    return db_launch_pdl(delta_chain_kernel<T>, dim3(a.v_heads, a.items), dim3(CHAIN_THREADS), CHAIN_SMEM, stream, a, w,
+                         db_device_error_ptr());
 }
 
 }  // namespace

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
     Shared& sh = *reinterpret_cast<Shared*>(ring + STAGES * STAGE);
     volatile int* abort_flag = &sh.abort;
     int* err = a.kv.error;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = chain::warp_index();
     const int h = blockIdx.y, b = blockIdx.z, Hk = a.kv.c.kv_heads;
     pdl_wait();
     pdl_trigger();
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             const int st = loaded(p ? 4 * p - 2 + t : t);
             if (!ok) return;
             tc_fence_after();
-            if (lane == 0) {
+            if (chain::elect()) {
                 const uint64_t dK = dR + (uint64_t)((st * STAGE) >> 4);
 #pragma unroll
                 for (int kk = 0; kk < D / 16; ++kk)
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             ok = ok && warp_wait(&sh.bars[P_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
             if (!ok) return;
             tc_fence_after();
-            if (lane == 0) {
+            if (chain::elect()) {
                 const uint64_t dV = dR + (uint64_t)((st * STAGE) >> 4);
 #pragma unroll
                 for (int kk = 0; kk < BLK / 16; ++kk) {
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             if (p + 2 < pairs && ok) scores(p + 2);
         }
         // every MMA issued has completed before tensor memory is released
-        if (lane == 0) {
+        if (chain::elect()) {
             umma_commit(&sh.bars[MMA_DONE + t]);
             mbar_wait_drain(&sh.bars[MMA_DONE + t], 0, DRAIN_NS);
         }
