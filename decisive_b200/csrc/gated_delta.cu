@@ -564,7 +564,7 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, boo
 // The code is kept small: what the warps of an SM run between two products has to stay in its instruction cache.
 //
 // Warps 0-7: the rows' arithmetic (thread: row 32 (w & 3) + lane; half w >> 2 of the keys, or of the tokens);
-// 8: MMA issue and tensor memory; 9-11: loads of the next chunk.
+// 8: MMA issue and tensor memory; 9-11: loads of the next chunk, outputs of the last.
 // Tensor memory columns: S parts 0-127, U' K 128-255, U 256-319 (then U' parts in its place), P U 320-383, X_k 384-447
 // (then R parts, then U parts), X_q 448-511.  Parts of 32 values lie in 32 columns: 16 of first parts (two values to a
 // column), 16 of second parts.
@@ -577,11 +577,12 @@ struct ChainStage {
     uint8_t tri[4][TRI_BYTES];  // T hi, T lo, P hi, P lo: 64 rows of 128 bytes, 128-byte swizzle
     uint8_t v[C * D * 2];
 };
-enum ChainBar { CB_FULL = 0, CB_EMPTY = 2, CB_S = 4, CB_X, CB_R, CB_U, CB_W, CB_UU, CB_D, CB_PU, CB_DONE, CB_END, CHAIN_BARS };
+enum ChainBar { CB_FULL = 0, CB_EMPTY = 2, CB_S = 4, CB_X, CB_R, CB_U, CB_W, CB_UU, CB_D, CB_PU, CB_OUT, CB_SENT, CB_DONE, CB_END, CHAIN_BARS };
 struct ChainShared {
+    uint8_t out[C * D * 2];  // a chunk's outputs on their way
     uint64_t bars[CHAIN_BARS];
     float factor[2][FACTORS];
-    float top[3][2][D];  // largest magnitudes of S, U and the next chunk's V: [half][row]
+    float top[3][2][D];  // largest magnitudes of S, U and V: [half][row]
     uint32_t tmem;
     int abort;
 };
@@ -627,7 +628,8 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             mbar_init(&sh.bars[CB_FULL + i], LOADERS / 32);
             mbar_init(&sh.bars[CB_EMPTY + i], 1 + 8);
         }
-        for (int i : {CB_S, CB_R, CB_W, CB_UU}) mbar_init(&sh.bars[i], 8);
+        for (int i : {CB_S, CB_R, CB_W, CB_UU, CB_OUT}) mbar_init(&sh.bars[i], 8);
+        mbar_init(&sh.bars[CB_SENT], LOADERS / 32);
         for (int i : {CB_X, CB_U, CB_D, CB_PU, CB_DONE}) mbar_init(&sh.bars[i], 1);
         mbar_init(&sh.bars[CB_END], CHAIN_THREADS / 32);
         sh.abort = 0;
@@ -652,6 +654,18 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
         // ---------------------------------------------------------------- loads
         const int lt = tid - 9 * 32;
         bool ok = true;
+        // chunk c's outputs from shared memory, 16 bytes at a time
+        auto send = [&](int c) {
+            ok = ok && chain::warp_wait(&sh.bars[CB_OUT], c & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
+            if (!ok) return;
+            const int row0 = start + c * C, n = min(C, end - row0);
+            T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.ldo + (int64_t)hv * D;
+            for (int r = lt >> 4; r < n; r += LOADERS / 16)
+                *reinterpret_cast<uint4*>(out + (int64_t)r * a.ldo + 8 * (lt & 15)) =
+                    *reinterpret_cast<const uint4*>(sh.out + r * (D * 2) + 16 * (lt & 15));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[CB_SENT]);
+        };
         for (int c = 0; c <= chunks && ok; ++c) {
             if (c > 0) {
                 // the chunk before has landed: to the tensor core's view, then on
@@ -697,72 +711,51 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                 for (int e = lt; e < FACTORS / 4; e += LOADERS) cp_async16_if(smem_u32(&sh.factor[s][4 * e]), f + 4 * e, true);
                 cp_async_commit();
             }
+            if (c > 1) send(c - 2);  // (formed at the start of chunk c - 1)
         }
+        if (chunks > 0) send(chunks - 1);
         cp_async_wait<0>();
     } else if (warp == 8) {
         // ---------------------------------------------------------------- MMA issue
+        // (One loop body for the four products keeps the code small: 550 cycles each, hand-offs included.)
+        const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);  // (uniform, for the compiler)
         bool ok = true;
         auto wait = [&](int bar, uint32_t parity) {
             ok = ok && chain::warp_wait(&sh.bars[bar], parity, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
             tc_fence_after();
-            return ok;
         };
-        constexpr uint32_t ID_X = idesc_f16_f32(128, 128), ID_D = idesc_f16_f32(128, 128) | (1u << 16);  // (B MN-major)
         for (int c = 0; c < chunks && ok; ++c) {
             const int s = c & 1;
             const uint32_t ph = c & 1;
-            const uint64_t dKQ = sw128_desc(smem_u32(stages[s].kq)), dK = mn_desc(smem_u32(stages[s].kq)),
-                           dT = sw128_desc(smem_u32(stages[s].tri));
-            // D (128 x 64) = (parts at a_tm) x (a triangle)^T: keys 16 s.. of the sum meet rows 16 s.. only
-            auto triangle = [&](uint32_t d_tm, uint32_t a_tm, int which) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t at = a_tm + 32u * (k >> 1) + 8u * (k & 1), id = idesc_f16_f32(128, 64 - 16 * k);
-                    const uint64_t hi = dT + (uint64_t)((which * TRI_BYTES + k * 2048 + k * 32) >> 4), lo = hi + (TRI_BYTES >> 4);
-                    chain::umma_f16_ts(d_tm + 16u * k, at + 16u, hi, id, k > 0);
-                    chain::umma_f16_ts(d_tm + 16u * k, at, lo, id, 1);
-                    chain::umma_f16_ts(d_tm + 16u * k, at, hi, id, 1);
-                }
-            };
+            const uint32_t kq = smem_u32(stages[s].kq);
+            const uint64_t dT = sw128_desc(smem_u32(stages[s].tri));
             if (c > 0) wait(CB_PU, ph ^ 1u);  // (X goes where its U parts were)
             wait(CB_FULL + s, (c >> 1) & 1);
-            if (!wait(CB_S, ph)) break;
-            if (chain::elect()) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const uint32_t at = tmem + 32u * (k >> 1) + 8u * (k & 1);
-                    const uint64_t d = dKQ + (uint64_t)(((k >> 2) * KQ_HALF + (k & 3) * 32) >> 4);
-                    chain::umma_f16_ts(tmem + 384u, at + 16u, d, ID_X, k > 0);
-                    chain::umma_f16_ts(tmem + 384u, at, d, ID_X, 1);
+#pragma unroll 1
+            for (int job = 0; job < 4 && ok; ++job) {
+                // X, U, U' K, P U; a triangle's K step k meets rows 16 k .. of it only
+                const bool tri = job & 1;
+                wait(job == 0 ? CB_S : job == 1 ? CB_R : job == 2 ? CB_W : CB_UU, ph);
+                const uint32_t d = tmem + (job == 0 ? 384u : job == 1 ? 256u : job == 2 ? 128u : 320u);
+                const uint32_t a_tm = tmem + (job == 0 ? 0u : job == 2 ? 256u : 384u);
+                const uint64_t b0 = job == 0 ? sw128_desc(kq) : job == 2 ? mn_desc(kq) : dT + (uint64_t)((job == 1 ? 0 : 2 * TRI_BYTES) >> 4);
+                const uint32_t id0 = job == 0 ? idesc_f16_f32(128, 128) : job == 2 ? idesc_f16_f32(128, 128) | (1u << 16) : idesc_f16_f32(128, 64);
+                const uint32_t b_step = job == 0 ? 2u : job == 2 ? 128u : 130u, steps = job == 0 ? 8u : 4u;
+                if (chain::elect()) {
+#pragma unroll 1
+                    for (uint32_t k = 0; k < steps; ++k) {
+                        const uint32_t at = a_tm + 32u * (k >> 1) + 8u * (k & 1), dk = tri ? d + 16u * k : d;
+                        const uint32_t id = tri ? id0 - k * (2u << 17) : id0;
+                        const uint64_t b = b0 + (uint64_t)((k & 3) * b_step + (k >> 2) * (KQ_HALF >> 4));
+                        chain::umma_f16_ts(dk, at + 16u, b, id, k > 0);
+                        if (tri) chain::umma_f16_ts(dk, at, b + (TRI_BYTES >> 4), id, 1);
+                        chain::umma_f16_ts(dk, at, b, id, 1);
+                    }
+                    umma_commit(&sh.bars[job == 0 ? CB_X : job == 1 ? CB_U : job == 2 ? CB_D : CB_PU]);
+                    if (job == 3) umma_commit(&sh.bars[CB_EMPTY + s]);
                 }
-                umma_commit(&sh.bars[CB_X]);
+                __syncwarp();
             }
-            __syncwarp();
-            if (!wait(CB_R, ph)) break;
-            if (chain::elect()) {
-                triangle(tmem + 256u, tmem + 384u, 0);
-                umma_commit(&sh.bars[CB_U]);
-            }
-            __syncwarp();
-            if (!wait(CB_W, ph)) break;
-            if (chain::elect()) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t at = tmem + 256u + 32u * (k >> 1) + 8u * (k & 1);
-                    const uint64_t d = dK + (uint64_t)((k * 2048) >> 4);
-                    chain::umma_f16_ts(tmem + 128u, at + 16u, d, ID_D, k > 0);
-                    chain::umma_f16_ts(tmem + 128u, at, d, ID_D, 1);
-                }
-                umma_commit(&sh.bars[CB_D]);
-            }
-            __syncwarp();
-            if (!wait(CB_UU, ph)) break;
-            if (chain::elect()) {
-                triangle(tmem + 320u, tmem + 384u, 2);
-                umma_commit(&sh.bars[CB_PU]);
-                umma_commit(&sh.bars[CB_EMPTY + s]);
-            }
-            __syncwarp();
         }
         // every MMA issued has completed before tensor memory is released
         if (chain::elect()) {
@@ -786,17 +779,7 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[bar]);
         };
-        // the halves' largest magnitudes meet in shared memory
-        float s_top, u_top = 0.f, v_top;
-        auto meet = [&](float s, float u, float v) {
-            sh.top[0][half][row] = s;
-            sh.top[1][half][row] = u;
-            sh.top[2][half][row] = v;
-            named_barrier_sync(1, 256);
-            s_top = fmaxf(s, sh.top[0][half ^ 1][row]);
-            u_top = fmaxf(u, sh.top[1][half ^ 1][row]);
-            v_top = fmaxf(v, sh.top[2][half ^ 1][row]);
-        };
+        float s_top = 0.f;  // the row's largest S part (of this half until the halves meet)
         auto values_top = [&](int s) {
             const unsigned short* v = reinterpret_cast<const unsigned short*>(stages[s].v) + 32 * half * D + row;
             uint32_t top = 0;
@@ -823,10 +806,12 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                     const float4 x = *reinterpret_cast<const float4*>(in + 4 * i);
                     top = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), top);
                 }
-            ok = chain::warp_wait(&sh.bars[CB_FULL], 0, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
-            meet(top, 0.f, ok ? values_top(0) : 0.f);
-            up_e = retarget(s_top);
-            s_top *= power(up_e);
+            sh.top[0][half][row] = top;
+            named_barrier_sync(1, 256);
+            top = fmaxf(top, sh.top[0][half ^ 1][row]);
+            up_e = retarget(top);
+            s_top = top * power(up_e);
+            named_barrier_sync(1, 256);
             const uint64_t up = both(power(up_e));
 #pragma unroll 1
             for (int q = 0; q < 2; ++q) {
@@ -839,21 +824,18 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             }
         }
         float Oq[32], o_scale = 0.f;
-        // chunk c's outputs: e^G S q is there, P U joins it
+        // chunk c's outputs: e^G S q is there, P U joins it; they leave through shared memory
         auto output = [&](int c) {
+            if (c > 0) wait(CB_SENT, (c - 1) & 1);
             uint32_t r[32];
             tmem_ld_32x32b_x32(tm + 320u + 32u * half, r);
             tmem_wait_ld(r);
-            const int row0 = start + c * C + 32 * half, n = end - row0;
-            T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.ldo + (int64_t)hv * D + row;
-            if (n >= 32) {
+            T* out = reinterpret_cast<T*>(sh.out) + 32 * half * D + row;
 #pragma unroll
-                for (int i = 0; i < 32; ++i, out += a.ldo) from_f32(fmaf(__uint_as_float(r[i]), o_scale, Oq[i]), *out);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (i < n) from_f32(fmaf(__uint_as_float(r[i]), o_scale, Oq[i]), out[i * a.ldo]);
-            }
+            for (int i = 0; i < 32; ++i) from_f32(fmaf(__uint_as_float(r[i]), o_scale, Oq[i]), out[i * D]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.bars[CB_OUT]);
         };
         if (chunks > 0) ready(CB_S);
         // (after an abort the waits return at once and the rest runs on: every warp meets the barriers as often as the others)
@@ -866,6 +848,13 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                 wait(CB_PU, ph ^ 1u);
                 output(c - 1);
             }
+            wait(CB_FULL + s, (c >> 1) & 1);
+            float v_top = values_top(s);
+            sh.top[0][half][row] = s_top;
+            sh.top[2][half][row] = v_top;
+            named_barrier_sync(1, 256);
+            s_top = fmaxf(s_top, sh.top[0][half ^ 1][row]);
+            v_top = fmaxf(v_top, sh.top[2][half ^ 1][row]);
             // R = V - e^G S k
             const float s_back = power(-up_e);
             float r_back;
@@ -926,14 +915,9 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             for (int i = 0; i < 16; ++i) top = pair_top(x[i], top);
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[CB_EMPTY + s]);  // this warp is done with the chunk's values and factors
-            float v_next = 0.f;
-            if (c + 1 < chunks) {
-                wait(CB_FULL + (s ^ 1), ((c + 1) >> 1) & 1);
-                v_next = values_top(s ^ 1);
-            }
-            const float before = s_top;
-            meet(0.f, top, v_next);
-            const int step = retarget(decay * before + u_top * grow * fabsf(s_scale));
+            sh.top[1][half][row] = top;
+            named_barrier_sync(1, 256);
+            const int step = retarget(decay * s_top + fmaxf(top, sh.top[1][half ^ 1][row]) * grow * fabsf(s_scale));
             up_e += step;
             const uint64_t keep = both(decay * power(step)), add = both(s_scale * power(step));
             // S <- e^G_C S + U' K
@@ -956,16 +940,16 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                 parts32(x, r);
                 chain::tmem_st32(tm + 64u * half + 32u * q, r);
             }
-            sh.top[0][half][row] = top;
-            if (c + 1 < chunks) {
+            s_top = top;
+            if (c + 1 < chunks)
                 ready(CB_S);
-            } else {
+            else
                 tmem_wait_st();
-            }
-            named_barrier_sync(1, 256);
-            s_top = fmaxf(top, sh.top[0][half ^ 1][row]);
         }
-        if (ok && chunks > 0 && wait(CB_PU, (chunks - 1) & 1)) output(chunks - 1);
+        if (chunks > 0) {
+            wait(CB_PU, (chunks - 1) & 1);
+            output(chunks - 1);
+        }
         if (a.state_out && ok) {
             float* o = a.state_out + (int64_t)b * a.v_heads * D * D + at;
             const float back = power(-up_e);
