@@ -262,6 +262,30 @@ struct PrepShared {
     float top[2][PREP_THREADS / 32];
 };
 
+__device__ __forceinline__ float2 pair_of(const float* x, int at) { return *reinterpret_cast<const float2*>(x + at); }
+
+// o[i] = sum over k < depth of a[i][k] b[k], rows of a AP apart, b's entries ldb: two products to an instruction.
+template <int R, int STEP>
+__device__ __forceinline__ void block_product(float (&o)[R], const float* a, const float* b, int ldb, int depth) {
+    uint64_t sum[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) sum[i] = 0;
+#pragma unroll 1
+    for (int k0 = 0; k0 < depth; k0 += STEP)
+#pragma unroll
+        for (int k = k0; k < k0 + STEP; k += 4) {
+            const uint64_t y0 = f2_pack(__float_as_uint(b[k * ldb]), __float_as_uint(b[(k + 1) * ldb]));
+            const uint64_t y1 = f2_pack(__float_as_uint(b[(k + 2) * ldb]), __float_as_uint(b[(k + 3) * ldb]));
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(a + i * AP + k);
+                sum[i] = f2_fma(x.y, y1, f2_fma(x.x, y0, sum[i]));
+            }
+        }
+#pragma unroll
+    for (int i = 0; i < R; ++i) o[i] = f2_lo(sum[i]) + f2_hi(sum[i]);
+}
+
 // T, P and the factors of one chunk, for one key head and `heads` of the value heads that share it.
 template <typename T>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArgs a, ChunkSpace w, int heads) {
@@ -419,17 +443,28 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
         }
         __syncthreads();
         // A into shared memory, P to its place
-        float p[8][4], largest = 0.f;
+        float p[8][4], largest = 0.f, row_Gh[2], row_Gl[2], row_k[2], row_q[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = warp * 16 + g + 8 * i;
+            row_Gh[i] = sh.Gh[r], row_Gl[i] = sh.Gl[r], row_k[i] = sh.rk[r] * sh.beta[r], row_q[i] = sh.rq[r];
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < 2 * warp + 2) {
+                const int c0 = 8 * j + 2 * t;
+                const float2 Gh = pair_of(sh.Gh, c0), Gl = pair_of(sh.Gl, c0), rk = pair_of(sh.rk, c0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = warp * 16 + g + 8 * (i >> 1), c = 8 * j + 2 * t + (i & 1);
-                    const float d = c <= r ? ex2((sh.Gh[r] - sh.Gh[c]) + (sh.Gl[r] - sh.Gl[c])) * sh.rk[c] : 0.f;
-                    sh.A[r * AP + c] = c < r ? kk[j][i] * d * sh.rk[r] * sh.beta[r] : 0.f;
-                    p[j][i] = c <= r ? qk[j][i] * d * sh.rq[r] : 0.f;
-                    largest = fmaxf(largest, fabsf(p[j][i]));
+                for (int i = 0; i < 2; ++i) {
+                    const int r = warp * 16 + g + 8 * i;
+                    const float d0 = c0 <= r ? ex2((row_Gh[i] - Gh.x) + (row_Gl[i] - Gl.x)) * rk.x : 0.f;
+                    const float d1 = c0 + 1 <= r ? ex2((row_Gh[i] - Gh.y) + (row_Gl[i] - Gl.y)) * rk.y : 0.f;
+                    float* x = &p[j][2 * i];
+                    *reinterpret_cast<float2*>(&sh.A[r * AP + c0]) = make_float2(c0 < r ? kk[j][2 * i] * d0 * row_k[i] : 0.f,
+                                                                                 c0 + 1 < r ? kk[j][2 * i + 1] * d1 * row_k[i] : 0.f);
+                    x[0] = c0 <= r ? qk[j][2 * i] * d0 * row_q[i] : 0.f;
+                    x[1] = c0 + 1 <= r ? qk[j][2 * i + 1] * d1 * row_q[i] : 0.f;
+                    largest = fmaxf(largest, fmaxf(fabsf(x[0]), fabsf(x[1])));
                 }
             }
         largest = warp_max(largest);
@@ -463,7 +498,13 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
             for (int i = 1; i < 16; ++i) {
                 float s = 0.f;
 #pragma unroll
-                for (int j = 0; j < i; ++j) s = fmaf(Ab[i * AP + j], x[j], s);
+                for (int j = 0; j < i; j += 4) {  // (A's entries from the diagonal on are zero)
+                    const float4 y = *reinterpret_cast<const float4*>(Ab + i * AP + j);
+                    s = fmaf(y.x, x[j], s);
+                    if (j + 1 < i) s = fmaf(y.y, x[j + 1], s);
+                    if (j + 2 < i) s = fmaf(y.z, x[j + 2], s);
+                    if (j + 3 < i) s = fmaf(y.w, x[j + 3], s);
+                }
                 if (i != lane) x[i] = i > lane ? -s : 0.f;
             }
 #pragma unroll
@@ -473,23 +514,13 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
         // the block below two neighbours: -T11 A10 T00, first for 16 x 16 blocks, then for 32 x 32
         {
             const int pr = tid >> 6, c = tid & 15, r0 = ((tid >> 4) & 3) * 4, b0 = 32 * pr;
-            float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float y = sh.T[(b0 + k) * AP + b0 + c];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = fmaf(sh.A[(b0 + 16 + r0 + i) * AP + b0 + k], y, o[i]);
-            }
+            float o[4];
+            block_product<4, 16>(o, sh.A + (b0 + 16 + r0) * AP + b0, sh.T + b0 * AP + b0 + c, AP, 16);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sh.tmp[(16 * pr + r0 + i) * 36 + c] = o[i];
             __syncthreads();
-            float z[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const float y = sh.tmp[(16 * pr + k) * 36 + c];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) z[i] = fmaf(sh.T[(b0 + 16 + r0 + i) * AP + b0 + 16 + k], y, z[i]);
-            }
+            float z[4];
+            block_product<4, 16>(z, sh.T + (b0 + 16 + r0) * AP + b0 + 16, sh.tmp + 16 * pr * 36 + c, 36, 16);
 #pragma unroll
             for (int i = 0; i < 4; ++i) sh.T[(b0 + 16 + r0 + i) * AP + b0 + c] = -z[i];
             // the 16 x 16 blocks above the diagonal are zero
@@ -499,33 +530,13 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
         __syncthreads();
         {
             const int c = lane, r0 = warp * 8;
-            float o[8] = {};
-#pragma unroll 4
-            for (int k = 0; k < 32; k += 4) {
-                float y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = sh.T[(k + j) * AP + c];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(&sh.A[(32 + r0 + i) * AP + k]);
-                    o[i] = fmaf(x.w, y[3], fmaf(x.z, y[2], fmaf(x.y, y[1], fmaf(x.x, y[0], o[i]))));
-                }
-            }
+            float o[8];
+            block_product<8, 16>(o, sh.A + (32 + r0) * AP, sh.T + c, AP, 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sh.tmp[(r0 + i) * 36 + c] = o[i];
             __syncthreads();
-            float z[8] = {};
-#pragma unroll 4
-            for (int k = 0; k < 32; k += 4) {
-                float y[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = sh.tmp[(k + j) * 36 + c];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(&sh.T[(32 + r0 + i) * AP + 32 + k]);
-                    z[i] = fmaf(x.w, y[3], fmaf(x.z, y[2], fmaf(x.y, y[1], fmaf(x.x, y[0], z[i]))));
-                }
-            }
+            float z[8];  // (T11's rows end at the diagonal)
+            block_product<8, 8>(z, sh.T + (32 + r0) * AP + 32, sh.tmp + c, 36, r0 + 8);
 #pragma unroll
             for (int i = 0; i < 8; ++i) sh.T[(32 + r0 + i) * AP + c] = -z[i];
         }
@@ -534,11 +545,16 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < 2 * warp + 2) {
+                const int c0 = 8 * j + 2 * t;
+                const float2 beta = pair_of(sh.beta, c0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = warp * 16 + g + 8 * (i >> 1), c = 8 * j + 2 * t + (i & 1);
-                    p[j][i] = c <= r ? sh.T[r * AP + c] * sh.beta[c] : 0.f;
-                    largest = fmaxf(largest, fabsf(p[j][i]));
+                for (int i = 0; i < 2; ++i) {
+                    const int r = warp * 16 + g + 8 * i;
+                    const float2 y = pair_of(sh.T, r * AP + c0);
+                    float* x = &p[j][2 * i];
+                    x[0] = c0 <= r ? y.x * beta.x : 0.f;
+                    x[1] = c0 + 1 <= r ? y.y * beta.y : 0.f;
+                    largest = fmaxf(largest, fmaxf(fabsf(x[0]), fabsf(x[1])));
                 }
             }
         largest = warp_max(largest);
