@@ -579,7 +579,7 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, boo
 // bound (2^6) costs nothing, because f16 parts of a row scaled to 2^15 reach down to 2^-40 of it.
 // The code is kept small: what the warps of an SM run between two products has to stay in its instruction cache.
 //
-// Warps 0-7: the rows' arithmetic (thread: row 32 (w & 3) + lane; half w >> 2 of the keys, or of the tokens);
+// Warps 0-7: the rows' arithmetic (thread: row 32 (w & 3) + lane; tokens 32 (w >> 2) .. + 31, or these and the keys 64 further on);
 // 8: MMA issue and tensor memory; 9-11: loads of the next chunk, outputs of the last.
 // Tensor memory columns: S parts 0-127, U' K 128-255, U 256-319 (then U' parts in its place), P U 320-383, X_k 384-447
 // (then R parts, then U parts), X_q 448-511.  Parts of 32 values lie in 32 columns: 16 of first parts (two values to a
@@ -593,11 +593,11 @@ struct ChainStage {
     uint8_t tri[4][TRI_BYTES];  // T hi, T lo, P hi, P lo: 64 rows of 128 bytes, 128-byte swizzle
     uint8_t v[C * D * 2];
 };
-enum ChainBar { CB_FULL = 0, CB_EMPTY = 2, CB_S = 4, CB_X, CB_R, CB_U, CB_W, CB_UU, CB_D, CB_PU, CB_OUT, CB_SENT, CB_DONE, CB_END, CHAIN_BARS };
+enum ChainBar { CB_FULL = 0, CB_EMPTY = 2, CB_S = 4, CB_D = 6, CB_X = 8, CB_R, CB_U, CB_W, CB_UU, CB_PU, CB_OUT, CB_SENT, CB_DONE, CB_END, CHAIN_BARS };
 struct ChainShared {
     uint8_t out[C * D * 2];  // a chunk's outputs on their way
     uint64_t bars[CHAIN_BARS];
-    float factor[2][FACTORS];
+    alignas(16) float factor[2][FACTORS];
     float top[3][2][D];  // largest magnitudes of S, U and V: [half][row]
     uint32_t tmem;
     int abort;
@@ -625,10 +625,8 @@ __device__ __forceinline__ void parts32(const uint64_t (&x)[16], uint32_t (&r)[3
     }
 }
 __device__ __forceinline__ uint64_t both(float x) { return f2_pack(__float_as_uint(x), __float_as_uint(x)); }
-// Two factors of neighbouring tokens from shared memory.
-__device__ __forceinline__ uint64_t pair_at(const float* f) { return *reinterpret_cast<const uint64_t*>(f); }
-// The larger magnitude of a pair.
-__device__ __forceinline__ float pair_top(uint64_t x, float top) { return fmaxf(top, fmaxf(fabsf(f2_lo(x)), fabsf(f2_hi(x)))); }
+// Four factors of neighbouring tokens from shared memory.
+__device__ __forceinline__ ulonglong2 pairs_at(const float* f) { return *reinterpret_cast<const ulonglong2*>(f); }
 
 template <typename T>
 __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs a, ChunkSpace w, int* err) {
@@ -643,10 +641,12 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.bars[CB_FULL + i], LOADERS / 32);
             mbar_init(&sh.bars[CB_EMPTY + i], 1 + 8);
+            mbar_init(&sh.bars[CB_S + i], 8);
+            mbar_init(&sh.bars[CB_D + i], 1);
         }
-        for (int i : {CB_S, CB_R, CB_W, CB_UU, CB_OUT}) mbar_init(&sh.bars[i], 8);
+        for (int i : {CB_R, CB_W, CB_UU, CB_OUT}) mbar_init(&sh.bars[i], 8);
         mbar_init(&sh.bars[CB_SENT], LOADERS / 32);
-        for (int i : {CB_X, CB_U, CB_D, CB_PU, CB_DONE}) mbar_init(&sh.bars[i], 1);
+        for (int i : {CB_X, CB_U, CB_PU, CB_DONE}) mbar_init(&sh.bars[i], 1);
         mbar_init(&sh.bars[CB_END], CHAIN_THREADS / 32);
         sh.abort = 0;
         fence_barrier_init();
@@ -733,7 +733,8 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
         cp_async_wait<0>();
     } else if (warp == 8) {
         // ---------------------------------------------------------------- MMA issue
-        // (One loop body for the four products keeps the code small: 550 cycles each, hand-offs included.)
+        // Six jobs a chunk, one loop body: X from the first and the last 64 keys, U, U' K for the first and the last 64
+        // keys, P U.  (Halves, because the state's arithmetic before X and after U' K goes by halves too.)
         const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);  // (uniform, for the compiler)
         bool ok = true;
         auto wait = [&](int bar, uint32_t parity) {
@@ -748,27 +749,28 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             if (c > 0) wait(CB_PU, ph ^ 1u);  // (X goes where its U parts were)
             wait(CB_FULL + s, (c >> 1) & 1);
 #pragma unroll 1
-            for (int job = 0; job < 4 && ok; ++job) {
-                // X, U, U' K, P U; a triangle's K step k meets rows 16 k .. of it only
-                const bool tri = job & 1;
-                wait(job == 0 ? CB_S : job == 1 ? CB_R : job == 2 ? CB_W : CB_UU, ph);
-                const uint32_t d = tmem + (job == 0 ? 384u : job == 1 ? 256u : job == 2 ? 128u : 320u);
-                const uint32_t a_tm = tmem + (job == 0 ? 0u : job == 2 ? 256u : 384u);
-                const uint64_t b0 = job == 0 ? sw128_desc(kq) : job == 2 ? mn_desc(kq) : dT + (uint64_t)((job == 1 ? 0 : 2 * TRI_BYTES) >> 4);
-                const uint32_t id0 = job == 0 ? idesc_f16_f32(128, 128) : job == 2 ? idesc_f16_f32(128, 128) | (1u << 16) : idesc_f16_f32(128, 64);
-                const uint32_t b_step = job == 0 ? 2u : job == 2 ? 128u : 130u, steps = job == 0 ? 8u : 4u;
+            for (int job = 0; job < 6 && ok; ++job) {
+                // a triangle's K step k meets rows 16 k .. of it only
+                const bool tri = job == 2 || job == 5, state = job < 2;
+                const uint32_t half = job & 1;  // (of X, job 0 and 1, and of U' K, jobs 3 and 4: 1 for the first half)
+                wait(state ? CB_S + job : job == 2 ? CB_R : job == 5 ? CB_UU : CB_W, ph);
+                const uint32_t d = tmem + (state ? 384u : job == 2 ? 256u : job == 5 ? 320u : 192u - 64u * half);
+                const uint32_t a_tm = tmem + (state ? 64u * job : tri ? 384u : 256u);
+                const uint64_t b0 = state ? sw128_desc(kq + KQ_HALF * job) : job == 2 ? dT : job == 5 ? dT + (2 * TRI_BYTES >> 4) : mn_desc(kq + KQ_HALF * (1u - half));
+                const uint32_t id0 = state ? idesc_f16_f32(128, 128) : tri ? idesc_f16_f32(128, 64) : idesc_f16_f32(128, 64) | (1u << 16);
+                const uint32_t b_step = state ? 2u : tri ? 130u : 128u;
                 if (chain::elect()) {
 #pragma unroll 1
-                    for (uint32_t k = 0; k < steps; ++k) {
+                    for (uint32_t k = 0; k < 4; ++k) {
                         const uint32_t at = a_tm + 32u * (k >> 1) + 8u * (k & 1), dk = tri ? d + 16u * k : d;
                         const uint32_t id = tri ? id0 - k * (2u << 17) : id0;
-                        const uint64_t b = b0 + (uint64_t)((k & 3) * b_step + (k >> 2) * (KQ_HALF >> 4));
-                        chain::umma_f16_ts(dk, at + 16u, b, id, k > 0);
+                        const uint64_t b = b0 + (uint64_t)(k * b_step);
+                        chain::umma_f16_ts(dk, at + 16u, b, id, k > 0 || job == 1);
                         if (tri) chain::umma_f16_ts(dk, at, b + (TRI_BYTES >> 4), id, 1);
                         chain::umma_f16_ts(dk, at, b, id, 1);
                     }
-                    umma_commit(&sh.bars[job == 0 ? CB_X : job == 1 ? CB_U : job == 2 ? CB_D : CB_PU]);
-                    if (job == 3) umma_commit(&sh.bars[CB_EMPTY + s]);
+                    if (job > 0) umma_commit(&sh.bars[job == 1 ? CB_X : job == 2 ? CB_U : job == 5 ? CB_PU : CB_D + job - 3]);
+                    if (job == 5) umma_commit(&sh.bars[CB_EMPTY + s]);
                 }
                 __syncwarp();
             }
@@ -795,14 +797,14 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[bar]);
         };
-        float s_top = 0.f;  // the row's largest S part (of this half until the halves meet)
-        auto values_top = [&](int s) {
-            const unsigned short* v = reinterpret_cast<const unsigned short*>(stages[s].v) + 32 * half * D + row;
-            uint32_t top = 0;
-#pragma unroll 8
-            for (int i = 0; i < 32; ++i) top = max(top, (uint32_t)v[i * D] & 0x7fffu);
-            return lane16<T>(top);
+        float s_top = 0.f;  // the row's largest S part (of these keys until the halves meet)
+        // largest magnitude among first parts (rounding moves it by 2^-11, which the bounds below allow for)
+        auto parts_top = [](const uint32_t (&r)[32], __half2 top) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = __hmax2(top, __habs2(*reinterpret_cast<const __half2*>(&r[i])));
+            return top;
         };
+        auto top_of = [](__half2 x) { return __half2float(__hmax(__low2half(x), __high2half(x))); };
         // a power of two 2^e (e of a float's exponent field) and the next one for a largest magnitude of `bound`
         int up_e = 0;  // S parts hold S 2^up_e
         auto power = [](int e) { return __uint_as_float((uint32_t)(127 + e) << 23); };
@@ -811,7 +813,7 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             const int step = bound > 0.f && e < 128 ? 14 - e : 0;
             return min(max(max(step, -100), -100 - up_e), min(100, 100 - up_e));
         };
-        const int64_t at = ((int64_t)hv * D + row) * D + 64 * half;
+        const int64_t at = ((int64_t)hv * D + row) * D + 32 * half;  // this thread's keys: 32 half .. + 31, and 64 further on
         if (chunks > 0) {
             // the state that is given, looked at once for its largest value, then split
             float top = 0.f;
@@ -819,7 +821,7 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             if (in)
 #pragma unroll 4
                 for (int i = 0; i < 16; ++i) {
-                    const float4 x = *reinterpret_cast<const float4*>(in + 4 * i);
+                    const float4 x = *reinterpret_cast<const float4*>(in + 4 * i + 32 * (i >> 3));
                     top = fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), top);
                 }
             sh.top[0][half][row] = top;
@@ -833,13 +835,15 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             for (int q = 0; q < 2; ++q) {
                 uint64_t x[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = in ? f2_mul(*reinterpret_cast<const uint64_t*>(in + 32 * q + 2 * i), up) : 0ull;
+                for (int i = 0; i < 16; ++i) x[i] = in ? f2_mul(*reinterpret_cast<const uint64_t*>(in + 64 * q + 2 * i), up) : 0ull;
                 uint32_t r[32];
                 parts32(x, r);
-                chain::tmem_st32(tm + 64u * half + 32u * q, r);
+                chain::tmem_st32(tm + 64u * q + 32u * half, r);
+                ready(CB_S + q);
             }
         }
-        float Oq[32], o_scale = 0.f;
+        uint64_t Oq[16];
+        float o_scale = 0.f;
         // chunk c's outputs: e^G S q is there, P U joins it; they leave through shared memory
         auto output = [&](int c) {
             if (c > 0) wait(CB_SENT, (c - 1) & 1);
@@ -848,45 +852,59 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             tmem_wait_ld(r);
             T* out = reinterpret_cast<T*>(sh.out) + 32 * half * D + row;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) from_f32(fmaf(__uint_as_float(r[i]), o_scale, Oq[i]), out[i * D]);
+            for (int i = 0; i < 16; ++i) {
+                const uint64_t o = f2_fma(f2_pack(r[2 * i], r[2 * i + 1]), both(o_scale), Oq[i]);
+                from_f32(f2_lo(o), out[2 * i * D]);
+                from_f32(f2_hi(o), out[(2 * i + 1) * D]);
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[CB_OUT]);
         };
-        if (chunks > 0) ready(CB_S);
         // (after an abort the waits return at once and the rest runs on: every warp meets the barriers as often as the others)
         for (int c = 0; c < chunks; ++c) {
             const int s = c & 1;
             const uint32_t ph = c & 1;
             const float* f = sh.factor[s];
-            // while X is formed: the chunk before goes out
+            uint32_t r[32];
+            uint64_t x[16];
+            // while X is formed: V, and the chunk before goes out
+            wait(CB_FULL + s, (c >> 1) & 1);
+            uint32_t V[16], v_bits = 0;
+            {
+                const unsigned short* v = reinterpret_cast<const unsigned short*>(stages[s].v) + 32 * half * D + row;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    V[i] = (uint32_t)v[2 * i * D] | (uint32_t)v[(2 * i + 1) * D] << 16;
+                    v_bits = __vmaxu2(v_bits, V[i] & 0x7fff7fffu);
+                }
+            }
+            sh.top[0][half][row] = s_top;
+            sh.top[2][half][row] = lane16<T>(max(v_bits & 0xffffu, v_bits >> 16));
             if (c > 0) {
                 wait(CB_PU, ph ^ 1u);
                 output(c - 1);
             }
-            wait(CB_FULL + s, (c >> 1) & 1);
-            float v_top = values_top(s);
-            sh.top[0][half][row] = s_top;
-            sh.top[2][half][row] = v_top;
             named_barrier_sync(1, 256);
             s_top = fmaxf(s_top, sh.top[0][half ^ 1][row]);
-            v_top = fmaxf(v_top, sh.top[2][half ^ 1][row]);
+            const float v_top = fmaxf(sh.top[2][0][row], sh.top[2][1][row]);
             // R = V - e^G S k
             const float s_back = power(-up_e);
             float r_back;
             const float r_up = row_power(v_top + f[F_REACH] * (s_top * s_back), r_back);
             wait(CB_X, ph);
-            uint32_t r[32];
-            uint64_t x[16];
             tmem_ld_32x32b_x32(tm + 384u + 32u * half, r);
             tmem_wait_ld(r);
             {
                 const uint64_t k = both(-s_back * r_up), up = both(r_up);
-                const unsigned short* v = reinterpret_cast<const unsigned short*>(stages[s].v) + 32 * half * D + row;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint64_t vv = f2_pack(__float_as_uint(lane16<T>(v[2 * i * D])), __float_as_uint(lane16<T>(v[(2 * i + 1) * D])));
-                    x[i] = f2_fma(f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k), pair_at(f + F_R + 32 * half + 2 * i), f2_mul(vv, up));
+                for (int i = 0; i < 16; i += 2) {
+                    const ulonglong2 w = pairs_at(f + F_R + 32 * half + 2 * i);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint64_t vv = f2_pack(__float_as_uint(lane16<T>(V[i + j] & 0xffffu)), __float_as_uint(lane16<T>(V[i + j] >> 16)));
+                        x[i + j] = f2_fma(f2_mul(f2_pack(r[2 * i + 2 * j], r[2 * i + 2 * j + 1]), k), j ? w.y : w.x, f2_mul(vv, up));
+                    }
                 }
                 parts32(x, r);
             }
@@ -898,9 +916,10 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             {
                 const uint64_t k = both(s_back);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint64_t o = f2_mul(f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k), pair_at(f + F_O + 32 * half + 2 * i));
-                    Oq[2 * i] = f2_lo(o), Oq[2 * i + 1] = f2_hi(o);
+                for (int i = 0; i < 16; i += 2) {
+                    const ulonglong2 w = pairs_at(f + F_O + 32 * half + 2 * i);
+                    Oq[i] = f2_mul(f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k), w.x);
+                    Oq[i + 1] = f2_mul(f2_mul(f2_pack(r[2 * i + 2], r[2 * i + 3]), k), w.y);
                 }
             }
             // U in units of 2^22 / (r_up x T's power): at most 2^14 whatever R and T are
@@ -910,14 +929,16 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             wait(CB_U, ph);
             tmem_ld_32x32b_x32(tm + 256u + 32u * half, r);
             tmem_wait_ld(r);
-            float top = 0.f;
             {
                 const uint64_t k = both(2.3841858e-7f);
                 uint64_t y[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
+                for (int i = 0; i < 16; i += 2) {
+                    const ulonglong2 w = pairs_at(f + F_U + 32 * half + 2 * i);
                     x[i] = f2_mul(f2_pack(r[2 * i], r[2 * i + 1]), k);
-                    y[i] = f2_mul(x[i], pair_at(f + F_U + 32 * half + 2 * i));
+                    x[i + 1] = f2_mul(f2_pack(r[2 * i + 2], r[2 * i + 3]), k);
+                    y[i] = f2_mul(x[i], w.x);
+                    y[i + 1] = f2_mul(x[i + 1], w.y);
                 }
                 parts32(y, r);
             }
@@ -927,23 +948,22 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             chain::tmem_st32(tm + 384u + 32u * half, r);
             ready(CB_UU);
             // while U' K is formed: what the next chunk's powers of two need
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = pair_top(x[i], top);
+            const float u_top = top_of(parts_top(r, __half2{}));
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[CB_EMPTY + s]);  // this warp is done with the chunk's values and factors
-            sh.top[1][half][row] = top;
+            sh.top[1][half][row] = u_top;
             named_barrier_sync(1, 256);
-            const int step = retarget(decay * s_top + fmaxf(top, sh.top[1][half ^ 1][row]) * grow * fabsf(s_scale));
+            const int step = retarget(decay * s_top + fmaxf(u_top, sh.top[1][half ^ 1][row]) * grow * fabsf(s_scale));
             up_e += step;
             const uint64_t keep = both(decay * power(step)), add = both(s_scale * power(step));
             // S <- e^G_C S + U' K
-            wait(CB_D, ph);
-            top = 0.f;
+            __half2 top{};
 #pragma unroll 1
             for (int q = 0; q < 2; ++q) {
                 uint32_t d[32];
-                tmem_ld_32x32b_x32(tm + 64u * half + 32u * q, r);
-                tmem_ld_32x32b_x32(tm + 128u + 64u * half + 32u * q, d);
+                wait(CB_D + q, ph);
+                tmem_ld_32x32b_x32(tm + 64u * q + 32u * half, r);
+                tmem_ld_32x32b_x32(tm + 128u + 64u * q + 32u * half, d);
                 tmem_wait_ld(r);
                 chain::tie32(d);
 #pragma unroll
@@ -951,16 +971,13 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&r[i])), l = __half22float2(*reinterpret_cast<const __half2*>(&r[16 + i]));
                     const uint64_t old = f2_add(f2_pack(__float_as_uint(h.x), __float_as_uint(h.y)), f2_pack(__float_as_uint(l.x), __float_as_uint(l.y)));
                     x[i] = f2_fma(f2_pack(d[2 * i], d[2 * i + 1]), add, f2_mul(old, keep));
-                    top = pair_top(x[i], top);
                 }
                 parts32(x, r);
-                chain::tmem_st32(tm + 64u * half + 32u * q, r);
+                chain::tmem_st32(tm + 64u * q + 32u * half, r);
+                ready(CB_S + q);  // (half of the next X is formed while the other half is updated)
+                top = parts_top(r, top);
             }
-            s_top = top;
-            if (c + 1 < chunks)
-                ready(CB_S);
-            else
-                tmem_wait_st();
+            s_top = top_of(top);
         }
         if (chunks > 0) {
             wait(CB_PU, (chunks - 1) & 1);
@@ -973,7 +990,7 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
             for (int q = 0; q < 2; ++q) {
                 uint32_t r[32];
                 if (chunks > 0) {
-                    tmem_ld_32x32b_x32(tm + 64u * half + 32u * q, r);
+                    tmem_ld_32x32b_x32(tm + 64u * q + 32u * half, r);
                     tmem_wait_ld(r);
                 }
 #pragma unroll
@@ -984,9 +1001,9 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                         const float2 h1 = __half22float2(*reinterpret_cast<const __half2*>(&r[2 * i + 1])), l1 = __half22float2(*reinterpret_cast<const __half2*>(&r[17 + 2 * i]));
                         y = make_float4((h0.x + l0.x) * back, (h0.y + l0.y) * back, (h1.x + l1.x) * back, (h1.y + l1.y) * back);
                     } else if (a.state_in) {
-                        y = *reinterpret_cast<const float4*>(a.state_in + (int64_t)b * a.state_stride + at + 32 * q + 4 * i);
+                        y = *reinterpret_cast<const float4*>(a.state_in + (int64_t)b * a.state_stride + at + 64 * q + 4 * i);
                     }
-                    *reinterpret_cast<float4*>(o + 32 * q + 4 * i) = y;
+                    *reinterpret_cast<float4*>(o + 64 * q + 4 * i) = y;
                 }
             }
         }
