@@ -77,6 +77,7 @@ __device__ __forceinline__ float warp_sum(float x) {
 // 4l..4l+3, so each row is one 512-byte access) and never meets another warp.  Both products of a
 // token are taken from the old state, S_new q = e^g S q + u (k.q), so the rows' 16 sums fold
 // together: 16 values over 32 lanes in 16 shuffles, after which lane l holds sum l / 2.
+// B200, 128 items of one token, 32 heads: 80 us, 6.7 TB/s, the copy's rate; one item: 15 us, launch latency.
 constexpr int STEP_ROWS = 8, STEP_WARPS = 4;
 
 template <typename T>
@@ -158,8 +159,11 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) delta_step_kernel(DeltaArgs a
 // the chunk,
 //   A_ij = beta_i e^(G_i - G_j) k_i.k_j (j < i),  T = (I + A)^-1 diag(beta),  P_ij = e^(G_i - G_j) q_i.k_j (j <= i)
 //   U = T (V - diag(e^G) K S0^T),  O = diag(e^G) Q S0^T + P U,  S1 = e^G_C S0 + sum_i e^(G_C - G_i) u_i k_i^T
-// T and P need no state: delta_prepare_kernel forms them for all chunks at once; delta_chunk_kernel then
-// walks a sequence's chunks.
+// T and P need no state: delta_prepare_kernel forms them for all chunks at once; delta_chain_kernel then
+// walks a sequence's chunks.  Chunks of 64: the walk's steps are a chain whose length is the number of chunks, and
+// 64 is the largest chunk whose triangles' parts fit in shared memory twice.  B200, 16 key and 32 value heads:
+// 512 tokens 56 us, 8229 tokens 635 us (47 TFLOP/s counted as the recurrence), 64 items of 16 to 1024 tokens 1.0 ms
+// (124 TFLOP/s).
 //
 // Numerics.  The state has to keep f32's accuracy through f16 tensor products: k and q enter them exactly
 // (bf16 rows as f16 after a power of two per row, which loses nothing within 2^-24 of the row's largest
@@ -286,7 +290,11 @@ __device__ __forceinline__ void block_product(float (&o)[R], const float* a, con
     for (int i = 0; i < R; ++i) o[i] = f2_lo(sum[i]) + f2_hi(sum[i]);
 }
 
-// T, P and the factors of one chunk, for one key head and `heads` of the value heads that share it.
+// T, P and the factors of one chunk, for one key head and `heads` of the value heads that share it.  K K^T and Q K^T on
+// mma.sync, once for the value heads of a key head; the inverse by blocks, -T11 A10 T00 from 16 x 16 to 64 x 64, in f32, because
+// an f16 product would lose what the state is to keep.  Bound by instruction issue and by the
+// barriers between its short steps, which 4 CTAs an SM cover in part.  B200: 0.40 ms of the 1.0 ms of 64 items, 0.11 ms of
+// the 0.64 of 8229 tokens.
 template <typename T>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArgs a, ChunkSpace w, int heads) {
     extern __shared__ __align__(16) uint8_t prep_smem[];
@@ -578,6 +586,9 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, boo
 // max |S k| <= sqrt(128) |k| max |S| for R, e^G_C max |S| + max |U| sum e^(G_C-G_i) |k_i| for the next S; the slack of a
 // bound (2^6) costs nothing, because f16 parts of a row scaled to 2^15 reach down to 2^-40 of it.
 // The code is kept small: what the warps of an SM run between two products has to stay in its instruction cache.
+// B200: 8000 cycles per chunk, most of them the rows' arithmetic and hand-offs (the products: 16 MMAs of 128 x 128 x 16 or
+// the like per job, 500 to 700 cycles each; 16 warps for the rows instead of 8 were no faster).  One CTA per SM (shared memory, all of tensor memory), so one item of 32 heads
+// keeps 32 SMs busy.
 //
 // Warps 0-7: the rows' arithmetic (thread: row 32 (w & 3) + lane; tokens 32 (w >> 2) .. + 31, or these and the keys 64 further on);
 // 8: MMA issue and tensor memory; 9-11: loads of the next chunk, outputs of the last.
@@ -1020,7 +1031,8 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
     }
 }
 
-// Up to this many tokens per item the recurrence is faster than a chunk.
+// Up to this many tokens per item the recurrence is faster than a chunk (128 items of 32 heads, recurrence / chunks, us:
+// 8 tokens 209 / 565, 16 379 / 571, 24 551 / 577, 32 724 / 581; one item: 16 20 / 36, 32 23 / 31, 64 38 / 31).
 constexpr int STEP_TOKENS = DB_DELTA_STEP_TOKENS;
 
 template <typename T>
@@ -1033,7 +1045,8 @@ cudaError_t launch(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     chunk_space(a.items, a.rows, a.k_heads, a.v_heads, !std::is_same<T, __half>::value, static_cast<uint8_t*>(workspace), &w);
     cudaError_t e = db_set_max_smem(reinterpret_cast<const void*>(delta_prepare_kernel<T>), sizeof(PrepShared));
     if (e != cudaSuccess) return e;
-    // a CTA per value head while that still finds idle SMs, else one for all that share a key head
+    // a CTA per value head while that still finds idle SMs, else one for all that share a key head (per value head / per
+    // key head, us of the whole call: 512 tokens 57 / 61, 8229 tokens 663 / 636, 64 items of 16 to 1024 tokens 1122 / 1002)
     const int64_t ids = chunk_ids(a.rows, a.items);
     const int group = a.v_heads / a.k_heads, heads = ids * a.k_heads < 4 * db_num_sms() ? 1 : group;
     e = db_launch_pdl(delta_prepare_kernel<T>, dim3((unsigned)ids, a.k_heads, (group + heads - 1) / heads), dim3(PREP_THREADS),
@@ -1067,7 +1080,7 @@ int db_gated_delta(const void* q, const void* k, const void* v, int dtype, int64
         return db_fail(DB_ERR_UNSUPPORTED, "UNSUPPORTED", "gated delta rule: q, k and v are f16 or bf16");
     const int64_t most = (int64_t)1 << 31;
     if (items < 0 || rows < 0 || max_len < 0 || rows >= most || items > 65535 || k_heads <= 0 || v_heads <= 0 ||
-        v_heads > 65535 || v_heads % k_heads || (!cu_seqlens && rows != items * max_len) || max_len > rows)
+        v_heads > 65535 || v_heads % k_heads || max_len > rows || (!cu_seqlens && rows != items * max_len))
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "gated delta rule: bad shape");
     if (items == 0) return DB_OK;
     if (rows > 0 && (!q || !k || !v || !g || !beta || !out || ldq < k_heads * 128 || ldk < k_heads * 128 ||
