@@ -586,9 +586,8 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, boo
 // max |S k| <= sqrt(128) |k| max |S| for R, e^G_C max |S| + max |U| sum e^(G_C-G_i) |k_i| for the next S; the slack of a
 // bound (2^6) costs nothing, because f16 parts of a row scaled to 2^15 reach down to 2^-40 of it.
 // The code is kept small: what the warps of an SM run between two products has to stay in its instruction cache.
-// B200: 8000 cycles per chunk, most of them the rows' arithmetic and hand-offs (the products: 16 MMAs of 128 x 128 x 16 or
-// the like per job, 500 to 700 cycles each; 16 warps for the rows instead of 8 were no faster).  One CTA per SM (shared memory, all of tensor memory), so one item of 32 heads
-// keeps 32 SMs busy.
+// B200: 8000 cycles per chunk, most of them the rows' arithmetic and hand-offs (16 warps for the rows instead of 8 were
+// no faster).  One CTA per SM (shared memory, all of tensor memory), so one item of 32 heads keeps 32 SMs busy.
 //
 // Warps 0-7: the rows' arithmetic (thread: row 32 (w & 3) + lane; tokens 32 (w >> 2) .. + 31, or these and the keys 64 further on);
 // 8: MMA issue and tensor memory; 9-11: loads of the next chunk, outputs of the last.

@@ -275,7 +275,9 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
  * k' = k, q' = scale * q.  g = -inf forgets everything before the token.  state_in f32 [v_heads, 128, 128]
  * per item, state_stride floats apart (0: one kept prefix state for all items; NULL: zeros); state_out
  * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own).
- * An item without rows passes its state on.  out [rows, v_heads, 128] in v's type.  workspace: device
+ * An item without rows passes its state on.  States keep f32's accuracy within 2^-22 of the largest terms of their
+ * value row (items longer than DB_DELTA_STEP_TOKENS multiply two f16 parts of every operand; f16 keys enter as they are, so with
+ * norm_eps >= 0 a key row far shorter than 2^-14 of the chunk's others counts with fewer bits).  out [rows, v_heads, 128] in v's type.  workspace: device
  * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0; it is 0 up to max_len =
  * DB_DELTA_STEP_TOKENS). */
 #define DB_DELTA_STEP_TOKENS 16
@@ -316,7 +318,8 @@ int db_kv8_append(const db_kv8_cache *cache, const void *k, int64_t ldk, const v
  * [rows, q_heads, 128]; query head h uses kv head h / (q_heads / kv_heads).  max_keys > 0: the caller's
  * estimate of the longest item's keys (table_width * 64 when nothing better is known); it sizes the launch
  * and the workspace and changes no result's meaning.  A row that can read no key (its pages are missing) is
- * 0.  workspace: device bytes from db_kv8_attention_workspace_bytes (may be NULL where that is 0). */
+ * 0.  More than 16 rows per kv head and item: blocks whose value scale is below 2^-24 of the largest that the row's
+ * neighbours read count as 2^-24 of it.  workspace: device bytes from db_kv8_attention_workspace_bytes (may be NULL where that is 0). */
 size_t db_kv8_attention_workspace_bytes(int64_t items, int64_t max_rows, int64_t max_keys, int64_t kv_heads,
                                         int64_t q_heads);
 int db_kv8_attention(const db_kv8_cache *cache, const void *q, int64_t ldq, const int32_t *lengths,
