@@ -261,8 +261,8 @@ struct PrepShared {
         };
     };
     float tmp[32 * 36];
-    float Gh[C], Gl[C];  // decay sums (log2) in two parts: their differences keep what one would round away
-    float beta[C], rk[C], rq[C], nk[C];
+    float Gh[PREP_THREADS / 32][C], Gl[PREP_THREADS / 32][C];  // per head of a batch: decay sums (log2) in two parts: their differences keep what one would round away
+    float beta[PREP_THREADS / 32][C], rk[C], rq[C], nk[C];
     float top[2][PREP_THREADS / 32];
 };
 
@@ -315,6 +315,67 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
     const int row0 = start + (id - (start / C + lo)) * C;
     if (row0 < start || row0 >= end) return;
     const int n = min(C, end - row0);
+
+    // warp i of a batch of heads forms the factors of its i-th head; its gates are loaded ahead of the tiles
+    constexpr int WARPS = PREP_THREADS / 32;
+    const int group = a.v_heads / a.k_heads, first = hk * group + blockIdx.z * heads, last = min(first + heads, (hk + 1) * group);
+    float gate[2] = {}, beta[2] = {};
+    auto load_gates = [&](int batch) {
+        if (batch + warp >= last) return;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * lane + j;
+            gate[j] = i < n ? a.g[(int64_t)(row0 + i) * a.ldg + batch + warp] : 0.f;
+            beta[j] = i < n ? a.beta[(int64_t)(row0 + i) * a.ldb + batch + warp] : 0.f;
+        }
+    };
+    auto factors = [&](int batch) {
+        if (batch + warp >= last) return;
+        float* factor = w.factor + ((int64_t)id * a.v_heads + batch + warp) * FACTORS;
+        double x[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            x[j] = gate[j] < -1e4f ? -1e4 : (double)gate[j];  // e^-10000 = 0; -inf would make differences NaN
+            sh.beta[warp][2 * lane + j] = beta[j];
+        }
+        double sum = x[0] + x[1];
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const double all = __shfl_sync(0xffffffffu, sum, 31);
+        float fu[2], reach = 0.f, largest = 0.f, grow = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int i = 2 * lane + j;
+            const double G = j ? sum : sum - x[1], two = G * 1.4426950408889634;
+            sh.Gh[warp][i] = (float)two;
+            sh.Gl[warp][i] = (float)(two - (double)sh.Gh[warp][i]);
+            const float e = expf((float)G);
+            factor[F_R + i] = e * sh.rk[i];
+            factor[F_O + i] = e * sh.rq[i];
+            const float left = expf((float)(all - G));
+            fu[j] = left * sh.rk[i];
+            grow += left * sh.nk[i];
+            reach = fmaxf(reach, e * sh.nk[i]);
+            largest = fmaxf(largest, fabsf(fu[j]));
+        }
+        reach = warp_max(reach);
+        largest = warp_max(largest);
+        grow = warp_sum(grow);
+        float back;
+        const float omega = row_power(largest, back) * (1.f / 65536.f);  // factors of U' to at most 1/2
+        factor[F_U + 2 * lane] = fu[0] * omega;
+        factor[F_U + 2 * lane + 1] = fu[1] * omega;
+        if (lane == 0) {
+            factor[F_DECAY] = expf((float)all);
+            factor[F_OMEGA] = back * 65536.f;
+            factor[F_REACH] = 11.4f * reach;  // |S k| <= sqrt(128) |k| max |S|
+            factor[F_GROW] = omega * grow;    // |sum U'_i k_i| <= max |U| sum of the weights
+        }
+    };
+    load_gates(first);
 
     // rows into shared memory as f16, with their factors
     constexpr bool COPY = sizeof(T) == 2 && !std::is_same<T, __half>::value;
@@ -373,6 +434,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
     }
     __syncthreads();
 
+    factors(first);
     // K K^T and Q K^T, rows 16 warp .. + 15, columns up to the diagonal
     float kk[8][4], qk[8][4];
 #pragma unroll
@@ -398,70 +460,31 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
             }
     }
 
-    const int group = a.v_heads / a.k_heads, first = hk * group + blockIdx.z * heads;
-    for (int hv = first; hv < min(first + heads, (hk + 1) * group); ++hv) {
+    for (int hv = first; hv < last; ++hv) {
+        const int h = (hv - first) % WARPS;
+        if (h == 0) {
+            if (hv > first) {
+                __syncthreads();
+                load_gates(hv);
+                factors(hv);
+            }
+            __syncthreads();  // the tiles, or the last head's triangles, have been read; the factors are there
+        }
         __half* tri = w.tri + ((int64_t)id * a.v_heads + hv) * 4 * TRI;
         float* factor = w.factor + ((int64_t)id * a.v_heads + hv) * FACTORS;
-        __syncthreads();  // the tiles, or the previous head's triangles, have been read
-        if (warp == 0) {
-            double x[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = 2 * lane + j;
-                const float gi = i < n ? a.g[(int64_t)(row0 + i) * a.ldg + hv] : 0.f;
-                x[j] = gi < -1e4f ? -1e4 : (double)gi;  // e^-10000 = 0; -inf would make differences NaN
-                sh.beta[i] = i < n ? a.beta[(int64_t)(row0 + i) * a.ldb + hv] : 0.f;
-            }
-            double sum = x[0] + x[1];
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double y = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += y;
-            }
-            const double all = __shfl_sync(0xffffffffu, sum, 31);
-            float fu[2], reach = 0.f, largest = 0.f, grow = 0.f;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int i = 2 * lane + j;
-                const double G = j ? sum : sum - x[1], two = G * 1.4426950408889634;
-                sh.Gh[i] = (float)two;
-                sh.Gl[i] = (float)(two - (double)sh.Gh[i]);
-                const float e = expf((float)G);
-                factor[F_R + i] = e * sh.rk[i];
-                factor[F_O + i] = e * sh.rq[i];
-                const float left = expf((float)(all - G));
-                fu[j] = left * sh.rk[i];
-                grow += left * sh.nk[i];
-                reach = fmaxf(reach, e * sh.nk[i]);
-                largest = fmaxf(largest, fabsf(fu[j]));
-            }
-            reach = warp_max(reach);
-            largest = warp_max(largest);
-            grow = warp_sum(grow);
-            float back;
-            const float omega = row_power(largest, back) * (1.f / 65536.f);  // factors of U' to at most 1/2
-            factor[F_U + 2 * lane] = fu[0] * omega;
-            factor[F_U + 2 * lane + 1] = fu[1] * omega;
-            if (lane == 0) {
-                factor[F_DECAY] = expf((float)all);
-                factor[F_OMEGA] = back * 65536.f;
-                factor[F_REACH] = 11.4f * reach;  // |S k| <= sqrt(128) |k| max |S|
-                factor[F_GROW] = omega * grow;    // |sum U'_i k_i| <= max |U| sum of the weights
-            }
-        }
-        __syncthreads();
+        const float *Ghs = sh.Gh[h], *Gls = sh.Gl[h], *betas = sh.beta[h];
         // A into shared memory, P to its place
         float p[8][4], largest = 0.f, row_Gh[2], row_Gl[2], row_k[2], row_q[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = warp * 16 + g + 8 * i;
-            row_Gh[i] = sh.Gh[r], row_Gl[i] = sh.Gl[r], row_k[i] = sh.rk[r] * sh.beta[r], row_q[i] = sh.rq[r];
+            row_Gh[i] = Ghs[r], row_Gl[i] = Gls[r], row_k[i] = sh.rk[r] * betas[r], row_q[i] = sh.rq[r];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if (j < 2 * warp + 2) {
                 const int c0 = 8 * j + 2 * t;
-                const float2 Gh = pair_of(sh.Gh, c0), Gl = pair_of(sh.Gl, c0), rk = pair_of(sh.rk, c0);
+                const float2 Gh = pair_of(Ghs, c0), Gl = pair_of(Gls, c0), rk = pair_of(sh.rk, c0);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int r = warp * 16 + g + 8 * i;
@@ -499,22 +522,19 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
         // (I + A)^-1, 16 x 16 blocks on the diagonal: lane c < 16 of warp b solves for column c of block b
         if (lane < 16) {
             const float* Ab = sh.A + (16 * warp) * AP + 16 * warp;
-            float x[16];
+            float x[16];  // each entry, once it is known, leaves all later ones: the sums do not wait for one another
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = i == lane ? 1.f : 0.f;
 #pragma unroll
-            for (int i = 1; i < 16; ++i) {
-                float s = 0.f;
+            for (int j = 0; j < 15; j += 4)
 #pragma unroll
-                for (int j = 0; j < i; j += 4) {  // (A's entries from the diagonal on are zero)
+                for (int i = j + 1; i < 16; ++i) {  // (A's entries from the diagonal on are zero)
                     const float4 y = *reinterpret_cast<const float4*>(Ab + i * AP + j);
-                    s = fmaf(y.x, x[j], s);
-                    if (j + 1 < i) s = fmaf(y.y, x[j + 1], s);
-                    if (j + 2 < i) s = fmaf(y.z, x[j + 2], s);
-                    if (j + 3 < i) s = fmaf(y.w, x[j + 3], s);
+                    x[i] = fmaf(-y.x, x[j], x[i]);
+                    if (j + 1 < i) x[i] = fmaf(-y.y, x[j + 1], x[i]);
+                    if (j + 2 < i) x[i] = fmaf(-y.z, x[j + 2], x[i]);
+                    if (j + 3 < i) x[i] = fmaf(-y.w, x[j + 3], x[i]);
                 }
-                if (i != lane) x[i] = i > lane ? -s : 0.f;
-            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) sh.T[(16 * warp + i) * AP + 16 * warp + lane] = x[i];
         }
@@ -554,7 +574,7 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
         for (int j = 0; j < 8; ++j)
             if (j < 2 * warp + 2) {
                 const int c0 = 8 * j + 2 * t;
-                const float2 beta = pair_of(sh.beta, c0);
+                const float2 beta = pair_of(betas, c0);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int r = warp * 16 + g + 8 * i;
