@@ -180,18 +180,23 @@ __global__ void __launch_bounds__(RULE_THREADS, 3) logit_rules_kernel(RuleArgs a
         const uint32_t allowed = (mask ? mask[v0 >> 5] & ~named : ~named) >> shift;
         const uint32_t left = (named >> shift) & 0xffu;
         float top = -INFINITY;
-        if (!left && whole) {
+        // a named token's logit is written as it came (the logits may be changed in place) and again when its rules have run:
+        // lanes that hold one then store like the others (93 -> 89 us for 256 rows with 1000 tokens of history)
+        const uint32_t shown = allowed | left;
 #pragma unroll
-            for (int i = 0; i < RULE_STEP; ++i) x[i] = (allowed >> i & 1) ? x[i] : -INFINITY;
+        for (int i = 0; i < RULE_STEP; ++i) x[i] = (shown >> i & 1) ? x[i] : -INFINITY;
+        if (whole) {
 #pragma unroll
             for (int i = 0; i < RULE_STEP; i += 4)
                 __stcs(reinterpret_cast<float4*>(out + v0 + i), make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]));
         } else {
 #pragma unroll
-            for (int i = 0; i < RULE_STEP; ++i) {
-                x[i] = (allowed >> i & 1) ? x[i] : -INFINITY;
-                if (!(left >> i & 1) && v0 + i < a.vocab) out[v0 + i] = x[i];
-            }
+            for (int i = 0; i < RULE_STEP; ++i)
+                if (v0 + i < a.vocab) out[v0 + i] = x[i];
+        }
+        if (left) {
+#pragma unroll
+            for (int i = 0; i < RULE_STEP; ++i) x[i] = (left >> i & 1) ? -INFINITY : x[i];
         }
 #pragma unroll
         for (int i = 0; i < RULE_STEP; ++i) top = fmaxf(top, x[i]);
