@@ -58,6 +58,24 @@ def test_a_prompt_at_once_is_its_tokens_one_by_one(hybrid):
             assert ((x - y).square().mean().sqrt() / y.square().mean().sqrt()).item() < 0.05
 
 
+@pytest.mark.parametrize("v_heads", [1, 5, 9])
+def test_heads_that_share_a_key_head(v_heads):
+    """Many chunks, so that one CTA prepares all value heads of a key head, in batches: the same products in the same order as
+    with a key head for each, so the same bits."""
+    import decisive_b200 as db
+    rng, rows = torch.Generator("cuda").manual_seed(v_heads), 64 * 600 + 7
+    q, k = (torch.randn(rows, 1, 128, generator=rng, device="cuda").bfloat16() for _ in range(2))
+    v = torch.randn(rows, v_heads, 128, generator=rng, device="cuda").bfloat16()
+    g = -torch.rand(rows, v_heads, generator=rng, device="cuda")
+    beta = torch.rand(rows, v_heads, generator=rng, device="cuda")
+    cu = torch.tensor([0, 64 * 300 + 5, rows], dtype=torch.int32, device="cuda")
+    shared = db.gated_delta(q, k, v, g, beta, items=2, cu_seqlens=cu)
+    own = db.gated_delta(q.expand(-1, v_heads, -1).contiguous(), k.expand(-1, v_heads, -1).contiguous(), v, g, beta, items=2,
+                         cu_seqlens=cu)
+    for x, y in zip(shared, own):
+        assert bool(torch.isfinite(x).all()) and torch.equal(x, y)
+
+
 @pytest.mark.parametrize("rows", [1, 40])  # per kv head: the two forms of the attention
 def test_pages_past_32_bits(rows):
     """A page whose first code lies 2.4 billion bytes into the pool reads as page 0 does."""
