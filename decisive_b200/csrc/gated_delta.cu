@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) delta_step_kernel(DeltaArgs a
 // T and P need no state: delta_prepare_kernel forms them for all chunks at once; delta_chain_kernel then
 // walks a sequence's chunks.  Chunks of 64: the walk's steps are a chain whose length is the number of chunks, and
 // 64 is the largest chunk whose triangles' parts fit in shared memory twice.  B200, 16 key and 32 value heads:
-// 512 tokens 56 us, 8229 tokens 635 us (47 TFLOP/s counted as the recurrence), 64 items of 16 to 1024 tokens 1.0 ms
-// (124 TFLOP/s).
+// 512 tokens 55 us, 8229 tokens 625 us (48 TFLOP/s counted as the recurrence), 64 items of 16 to 1024 tokens 0.97 ms
+// (128 TFLOP/s).
 //
 // Numerics.  The state has to keep f32's accuracy through f16 tensor products: k and q enter them exactly
 // (bf16 rows as f16 after a power of two per row, which loses nothing within 2^-24 of the row's largest
@@ -292,9 +292,9 @@ __device__ __forceinline__ void block_product(float (&o)[R], const float* a, con
 
 // T, P and the factors of one chunk, for one key head and `heads` of the value heads that share it.  K K^T and Q K^T on
 // mma.sync, once for the value heads of a key head; the inverse by blocks, -T11 A10 T00 from 16 x 16 to 64 x 64, in f32, because
-// an f16 product would lose what the state is to keep.  Bound by instruction issue and by the
-// barriers between its short steps, which 4 CTAs an SM cover in part.  B200: 0.40 ms of the 1.0 ms of 64 items, 0.11 ms of
-// the 0.64 of 8229 tokens.
+// an f16 product would lose what the state is to keep.  Bound by shared memory's latency
+// and wavefronts (58% of their rate; issue 47%) and the barriers between its short steps, which 4 CTAs an SM cover in part.
+// B200: 0.37 ms of the 0.97 ms of 64 items, 0.10 ms of the 0.63 of 8229 tokens.
 template <typename T>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArgs a, ChunkSpace w, int heads) {
     extern __shared__ __align__(16) uint8_t prep_smem[];
