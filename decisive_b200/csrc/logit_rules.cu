@@ -290,8 +290,8 @@ template <typename T>
 cudaError_t launch(RuleArgs a, int rows, cudaStream_t stream) {
     const bool vec = !(((uintptr_t)a.logits | (uintptr_t)a.out) & 15) && !((a.ld * sizeof(T)) & 15) && !((a.ldo * 4) & 15);
     // CTAs per row: for few rows one per stripe, up to 16; for many only as many as fill the SMs with three
-    // each, so that a CTA's fixed work is spread over more tokens (three / six / one per SM, us, 151936 tokens: 16 rows
-    // 22 / 18 / 22, 64 rows 31 / 37 / 31, 256 rows 93 / 93 / 93, before named tokens were stored with the stream)
+    // each, so that a CTA's fixed work is spread over more tokens (64 rows of 151936 tokens, 8 CTAs each: 31 us; with six
+    // to an SM, 16 CTAs each: 37 us)
     const int stripes = (a.vocab + STRIPE - 1) / STRIPE, fill = 3 * db_num_sms();
     int ctas = 1;
     while (ctas < RULE_MAX_CTAS && ctas < stripes && (stripes > ctas * (RULE_MAX_SLICE / 2 / STRIPE) || rows * ctas < fill)) ctas *= 2;
