@@ -283,15 +283,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // bytes 4s..4s+3 of each lane's 16; and key 16 (r >> 1) + 4 s + 2 half + (r & 1) sits in row r of
 // half `half` of score tile s, which makes P^T's fragment the four bytes 4s..4s+3 of each 16 of V^T.
 // Codes become f16 exactly; q is scaled by a power of two per row into f16 (bf16 has fewer bits
-// and more range), so the scores' product rounds neither operand.  P is rounded after its f32 sum is
-// taken, to one f16 for bf16 outputs and to two for f16 ones (one rounding of P to f16 is as large as the
-// output's own).  A block's own context is scaled by its value scale when it joins the running one, in f32.
+// and more range), so the scores' product rounds neither operand.  P enters its product as two f16 parts, 22 bits (one
+// f16 would change one bf16 output in 15 and is as large a rounding as an f16 output's own); its sum is taken from the f32
+// values.  A block's own context is scaled by its value scale when it joins the running one, in f32.
 //
 // The tile of 8 NT query rows that a warp works on, with its running maxima and sums (log2 domain; column
 // 2 t + j of n tile n in [n][j], equal in the 8 lanes g) and its context (feature 16 d + 8 (j >> 1) + g).
 template <typename T, int NT>
 struct Tile {
-    static constexpr bool TWO = std::is_same<T, __half>::value;
     // query fragments, k step 4 c + s: in registers, or for more rows in shared memory ([NT][8][32], the warp's own)
     uint2 qf[NT == 1 ? 8 : 1];
     uint2* qs;
@@ -471,7 +470,7 @@ struct Tile {
                 vf[n][j] = limit[n][j] >= base ? vs : 0.f;  // a block that a row does not see must not reach it (0 x NaN)
             }
         soften(s, scaled, base, alpha);
-        uint32_t p[NT][4][2], rest[TWO ? NT : 1][4][2];
+        uint32_t p[NT][4][2], rest[NT][4][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -481,9 +480,8 @@ struct Tile {
                     const float x = s[i][n][2 * half], y = s[i][n][2 * half + 1];
                     const uint32_t hi = pack2<__half>(x, y);
                     p[n][i][half] = transpose8(hi);
-                    if constexpr (TWO)
-                        rest[n][i][half] = transpose8(
-                            pack2<__half>(x - from_bits<__half>(hi & 0xffffu), y - from_bits<__half>(hi >> 16)));
+                    rest[n][i][half] =
+                        transpose8(pack2<__half>(x - from_bits<__half>(hi & 0xffffu), y - from_bits<__half>(hi >> 16)));
                 }
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -504,7 +502,7 @@ struct Tile {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     mma16(o[n], f, p[n][st][0], p[n][st][1], __half());
-                    if constexpr (TWO) mma16(o[n], f, rest[n][st][0], rest[n][st][1], __half());
+                    mma16(o[n], f, rest[n][st][0], rest[n][st][1], __half());
                 }
             }
 #pragma unroll
@@ -551,18 +549,23 @@ struct Tile {
 #pragma unroll
         for (int n = 0; n < NT; ++n) unscaled[n][0] = unscaled[n][1] = plain;
         soften(s, unscaled, base, alpha);
-        // P in two parts of the tail's type, so that bf16 loses no more than f16
-        uint32_t p[NT][4][2], rest[NT][4][2];
+        // P in parts of the tail's type: two of f16 hold 22 bits, three of bf16 24
+        constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+        uint32_t p[PARTS][NT][4][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const float x = s[i][n][2 * half], y = s[i][n][2 * half + 1];
-                    const uint32_t hi = pack2<T>(x, y);
-                    p[n][i][half] = transpose8(hi);
-                    rest[n][i][half] = transpose8(pack2<T>(x - from_bits<T>(hi & 0xffffu), y - from_bits<T>(hi >> 16)));
+                    float x = s[i][n][2 * half], y = s[i][n][2 * half + 1];
+#pragma unroll
+                    for (int k = 0; k < PARTS; ++k) {
+                        const uint32_t part = pack2<T>(x, y);
+                        p[k][n][i][half] = transpose8(part);
+                        x -= from_bits<T>(part & 0xffffu);
+                        y -= from_bits<T>(part >> 16);
+                    }
                 }
         constexpr int BATCH = NT == 1 ? 2 : 1;  // feature tiles whose values are loaded together
 #pragma unroll 1
@@ -601,10 +604,9 @@ struct Tile {
                 for (int st = 0; st < 4; ++st) {
                     const uint32_t fa[4] = {f[d][0][2 * st], f[d][1][2 * st], f[d][0][2 * st + 1], f[d][1][2 * st + 1]};
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        mma16(o[d][n], fa, p[n][st][0], p[n][st][1], T());
-                        mma16(o[d][n], fa, rest[n][st][0], rest[n][st][1], T());
-                    }
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < PARTS; ++k) mma16(o[d][n], fa, p[k][n][st][0], p[k][n][st][1], T());
                 }
             }
             if (__any_sync(0xffffffffu, odd)) {

@@ -7,7 +7,7 @@
 //   S = Q K^T (codes as exact f16),  P = 2^(S c - m),  O += P V (codes as exact f16)
 // Six warps turn codes into f16 tiles in shared memory, in the order in which the MMAs take them; a value page is
 // stored [128][64 tokens], which is already the K-major operand.  P stays in tensor memory: it overwrites S
-// and is the A operand of the second product, as one f16 for bf16 outputs, as two for f16 ones.  Where scales go: a
+// and is the A operand of the second product, as two f16 parts, 22 bits (one f16 would change one bf16 output in 15).  Where scales go: a
 // key block's into the exponent's factor, a value block's into P, relative to the largest value scale of the
 // keys that the CTA reads (blocks below 2^-24 of that count as 2^-24), the row sum taken back by its inverse.  The
 // maximum moves only when a tile raises it by more than 8 (log2), so accumulators are rarely rescaled.
@@ -74,7 +74,7 @@ __device__ __forceinline__ void sts128u(uint8_t* base, uint32_t at, uint32_t a, 
 // One row's softmax step on a tile's 64 scores: moves the maximum m (and l) if the tile raises it by more than 8, writes
 // P = 2^(S scale + shift - m) over S as the f16 operand (32 keys to 32 columns: 16 of first parts, 16 of second), returns
 // its sum.  MASKED: only keys 0 .. seen count; a scale of 0 or NaN must not reach the others.
-template <bool TWO, bool MASKED>
+template <bool MASKED>
 __device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float scale, float shift, float& m, float& l, float& move,
                                         uint32_t s_tm) {
     if (MASKED) {
@@ -114,16 +114,11 @@ __device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float sc
             const uint64_t xy = f2_pack(__float_as_uint(x), __float_as_uint(y));
             sum[i & 1] = f2_add(sum[i & 1], xy);
             pk[i] = pack2<__half>(x, y);
-            if (TWO) {
-                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pk[i]));
-                const uint64_t left = f2_fma(f2_pack(__float_as_uint(h.x), __float_as_uint(h.y)), minus, xy);
-                pk[16 + i] = pack2<__half>(f2_lo(left), f2_hi(left));
-            }
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pk[i]));
+            const uint64_t left = f2_fma(f2_pack(__float_as_uint(h.x), __float_as_uint(h.y)), minus, xy);
+            pk[16 + i] = pack2<__half>(f2_lo(left), f2_hi(left));
         }
-        if (TWO)
-            chain::tmem_st32(s_tm + 32u * c, pk);
-        else
-            chain::tmem_st16(s_tm + 32u * c, pk);
+        chain::tmem_st32(s_tm + 32u * c, pk);
     }
     const uint64_t both = f2_add(sum[0], sum[1]);
     return f2_lo(both) + f2_hi(both);
@@ -140,8 +135,7 @@ __device__ __forceinline__ bool warp_wait_idle(uint64_t* bar, uint32_t parity, v
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
-    constexpr bool TWO = std::is_same<T, __half>::value;
-    constexpr uint32_t INF = TWO ? 0x7c00u : 0x7f80u;
+    constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
     extern __shared__ uint8_t rows_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rows_smem) + 1023) & ~uintptr_t(1023));
     uint8_t* ring = smem + Q_BYTES;
@@ -419,8 +413,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                 for (int kk = 0; kk < BLK / 16; ++kk) {
                     // 32 keys lie in 32 columns: 16 of the first parts, 16 of the second
                     const uint32_t at = s_tm + 64u * slot + 32u * (kk >> 1) + 8u * (kk & 1);
-                    if (TWO) chain::umma_f16_ts(o_tm, at + 16u, dV + (uint64_t)(kk * 2), IDESC_O, p > 0 || kk > 0);
-                    chain::umma_f16_ts(o_tm, at, dV + (uint64_t)(kk * 2), IDESC_O, TWO || p > 0 || kk > 0);
+                    chain::umma_f16_ts(o_tm, at + 16u, dV + (uint64_t)(kk * 2), IDESC_O, p > 0 || kk > 0);
+                    chain::umma_f16_ts(o_tm, at, dV + (uint64_t)(kk * 2), IDESC_O, 1);
                 }
                 umma_commit(&sh.bars[EMPTY + st]);
                 umma_commit(&sh.bars[PV_DONE + 2 * t + slot]);
@@ -463,9 +457,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             const float scale = factor * n.ks;
             float move = 1.f, all;
             if (__any_sync(0xffffffffu, seen < BLK - 1))
-                all = soften<TWO, true>(r, seen, scale, n.shift, m, l, move, s_tm);
+                all = soften<true>(r, seen, scale, n.shift, m, l, move, s_tm);
             else
-                all = soften<TWO, false>(r, seen, scale, n.shift, m, l, move, s_tm);
+                all = soften<false>(r, seen, scale, n.shift, m, l, move, s_tm);
             if (all != 0.f) l = fmaf(all, n.undo, l);
             // O is stable once the previous P V of this parity is done
             const bool rescale = p > 0 && __any_sync(0xffffffffu, move != 1.f);
