@@ -8,9 +8,13 @@
 // Six warps turn codes into f16 tiles in shared memory, in the order in which the MMAs take them; a value page is
 // stored [128][64 tokens], which is already the K-major operand.  P stays in tensor memory: it overwrites S
 // and is the A operand of the second product, as two f16 parts, 22 bits (one f16 would change one bf16 output in 15).  Where scales go: a
-// key block's into the exponent's factor, a value block's into P, relative to the largest value scale of the
-// keys that the CTA reads (blocks below 2^-24 of that count as 2^-24), the row sum taken back by its inverse.  The
-// maximum moves only when a tile raises it by more than 8 (log2), so accumulators are rarely rescaled.
+// key block's into the exponent's factor, a value block's into P, relative to the accumulator's unit, a power of two
+// of its warpgroup's; the row sum is taken back by the inverse.  The unit starts at 2 to 4 times the first block's value scale
+// and moves, with the accumulator, to a block whose scale is above it or below 2^-6 of it, so P's parts always lie in
+// f16's normal range; a row depends only on what it sees, because the accumulator's factors are powers of two.  The
+// unit stays above 2^-80 of the largest so far (the accumulator must not overflow): under a block 2^80 times as large,
+// values end at 2^-100 of that block's.  The maximum moves only when a tile raises it by more than 8 (log2), so
+// accumulators are rarely rescaled.
 //
 // Warps: 0-3, 14 and 15 conversion, 4-7 softmax of even tiles, 8-11 of odd tiles, 12 and 13 MMA issue for even and odd
 // tiles (one issuer for both was the kernel's bound: 3600 of 6600 cycles per pair of tiles), 12 tensor memory.
@@ -19,6 +23,8 @@
 // keys, 16 / 8 heads: 144 us for f16 (426 TFLOP/s, 26% of the dense f16 rate; P's second part is a third of the products
 // and not counted), 133 us for bf16.
 // Tensor memory (512 columns): S / P of (parity, slot) at 128 parity + 64 slot, O even 256-383, O odd 384-511.
+#include <float.h>
+
 #include "kv8.cuh"
 #include "capi_internal.h"
 #include "kernels.h"
@@ -41,10 +47,13 @@ constexpr uint64_t DRAIN_NS = 100000000ull;
 enum Bar { FULL = 0, EMPTY = FULL + STAGES, S_FULL = EMPTY + STAGES, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
            JOIN = PV_DONE + 4, MMA_DONE, END = MMA_DONE + 2, BARS };
 
+constexpr int SHIFT = 7;         // P of the maximum is 2^SHIFT (value scale / unit), of a key up to 8 (log2) above it 2^15 at most
+constexpr int NO_SCALE = -1000;  // a value scale that moves no unit
+constexpr int LEAST = -40;       // P this far down is 0 in both parts
 struct Info {
-    float ks;     // key scale
-    float shift;  // 7 + log2 (value scale / reference)
-    float undo;   // 2^-shift
+    float ks;      // key scale
+    int e;         // the value scale is 2^e f, 1 <= f < 2; NO_SCALE: 0 (its block adds nothing) or not finite
+    float lf, inv; // log2 f and 1 / f (NaN where the scale is not finite)
     int there;
 };
 struct Shared {
@@ -52,9 +61,10 @@ struct Shared {
     Info info[INFO];
     float row_factor[ROWS];
     float join_m[2][ROWS], join_l[2][ROWS];
+    int join_unit[2][ROWS];
     uint32_t tmem;
     int abort;
-    uint32_t vref, tail_k, tail_v;  // largest value scale (bits); the open block's largest magnitudes (16-bit bits)
+    uint32_t tail_k, tail_v;        // the open block's largest magnitudes (16-bit bits)
     int odd;                        // the open block has values that are not finite
 };
 constexpr int SMEM = 1024 + Q_BYTES + STAGES * STAGE + sizeof(Shared);
@@ -67,6 +77,8 @@ __device__ __forceinline__ float code_power(float m, float& back) {
     back = __uint_as_float((uint32_t)(127 - k) << 23);
     return __uint_as_float((uint32_t)(127 + k) << 23);
 }
+// 2^n, 0 below f32's normal range (n <= 127)
+__device__ __forceinline__ float power2(int n) { return n < -126 ? 0.f : __uint_as_float((uint32_t)(127 + n) << 23); }
 __device__ __forceinline__ void sts128u(uint8_t* base, uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     *reinterpret_cast<uint4*>(base + at) = make_uint4(a, b, c, d);
 }
@@ -174,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         mbar_init(&sh.bars[MMA_DONE + 1], 1);
         mbar_init(&sh.bars[END], THREADS / 32);
         sh.abort = 0;
-        sh.vref = sh.tail_k = sh.tail_v = 0;
+        sh.tail_k = sh.tail_v = 0;
         sh.odd = 0;
         fence_barrier_init();
     }
@@ -203,18 +215,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         *reinterpret_cast<uint2*>(smem + at) = make_uint2(pack2<__half>(x[0] * up, x[1] * up), pack2<__half>(x[2] * up, x[3] * up));
     }
     __syncthreads();
-    // the largest value scale that is read, and the open block's magnitudes
+    // the open block's magnitudes
     {
-        float top = 0.f;
-        for (int i = tid; i < min(blocks, whole); i += THREADS) {
-            const int p = i < a.kv.c.table_width ? a.kv.c.page_table[(int64_t)b * a.kv.c.table_width + i] : -1;
-            if ((unsigned)p < (unsigned)a.kv.c.pages) {
-                const float s = a.kv.c.v_scales[(int64_t)p * Hk + h];
-                if (s < INFINITY) top = fmaxf(top, s);
-            }
-        }
-        top = warp_max(top);
-        if (lane == 0 && top > 0.f) atomicMax(&sh.vref, __float_as_uint(top));
         uint32_t km = 0, vm = 0;
         bool odd = false;
         for (int e = tid; inside && e < BLK * D / 8; e += THREADS) {
@@ -247,7 +249,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
     const uint32_t tmem = sh.tmem;
     float kt_back, vt_back;
     const float kt_up = code_power(from_bits<T>(sh.tail_k), kt_back), vt_up = code_power(from_bits<T>(sh.tail_v), vt_back);
-    const float vref0 = fmaxf(__uint_as_float(sh.vref), inside ? vt_back : 0.f), vref = vref0 > 0.f ? vref0 : 1.f;
 
     if (warp < 4 || warp > 13) {
         // ---------------------------------------------------------------- codes -> f16 tiles
@@ -359,10 +360,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                 }
             }
             if (!is_v && lane == 0) {
-                float ratio = v_scale / vref;
-                ratio = ratio < 5.9604645e-8f ? 5.9604645e-8f : ratio;  // (a NaN stays)
-                n.shift = 7.f + log2f(ratio);
-                n.undo = 0.0078125f / ratio;
+                const bool some = v_scale >= FLT_MIN && v_scale < INFINITY;
+                const float f = __uint_as_float((__float_as_uint(v_scale) & 0x7fffffu) | 0x3f800000u);
+                n.e = some ? (int)(__float_as_uint(v_scale) >> 23) - 127 : NO_SCALE;
+                n.lf = some ? log2f(f) : v_scale < FLT_MIN ? 0.f : NAN;
+                n.inv = some ? __fdividef(1.f, f) : v_scale < FLT_MIN ? 1.f : NAN;
                 n.there = paged || tail;
                 sh.info[j & (INFO - 1)] = n;
             }
@@ -441,6 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         const int limit = row0 + row < rows ? len + (row0 + row) / a.group : -1;
         const float factor = sh.row_factor[row];
         float m = -INFINITY, l = 0.f;
+        int unit = NO_SCALE, largest = NO_SCALE;  // O is in units of 2^(unit - SHIFT)
         bool ok = true;
         for (int p = 0; p < pairs; ++p) {
             const int slot = p & 1, base = (2 * p + t) * BLK;
@@ -456,11 +459,25 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             const int seen = n.there ? limit - base : -1;  // keys 0 .. seen of the tile
             const float scale = factor * n.ks;
             float move = 1.f, all;
+            int raise = 0;
+            if (n.there && n.e != NO_SCALE) {
+                if (unit == NO_SCALE) {
+                    unit = n.e + 2;  // (O is 0 so far)
+                } else if (n.e >= unit || n.e < unit - 6) {
+                    const int next = max(n.e + 2, largest - 80);
+                    raise = unit - next;
+                    unit = next;
+                }
+                largest = max(largest, unit);
+            }
+            const int down = n.e == NO_SCALE ? LEAST : max(SHIFT + n.e - unit, LEAST);
+            const float shift = (float)down + n.lf;
             if (__any_sync(0xffffffffu, seen < BLK - 1))
-                all = soften<true>(r, seen, scale, n.shift, m, l, move, s_tm);
+                all = soften<true>(r, seen, scale, shift, m, l, move, s_tm);
             else
-                all = soften<false>(r, seen, scale, n.shift, m, l, move, s_tm);
-            if (all != 0.f) l = fmaf(all, n.undo, l);
+                all = soften<false>(r, seen, scale, shift, m, l, move, s_tm);
+            if (all != 0.f) l = fmaf(all, n.inv * power2(-down), l);
+            move *= power2(raise);
             // O is stable once the previous P V of this parity is done
             const bool rescale = p > 0 && __any_sync(0xffffffffu, move != 1.f);
             if (rescale) {
@@ -487,6 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             tc_fence_after();
             sh.join_m[t][row] = m;
             sh.join_l[t][row] = l;
+            sh.join_unit[t][row] = unit;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.bars[JOIN]);
             ok = warp_wait(&sh.bars[JOIN], 0, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI);
@@ -494,8 +512,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         if (ok) {
             const float m0 = sh.join_m[0][row], m1 = sh.join_m[1][row], mm = fmaxf(m0, m1), at = mm == -INFINITY ? 0.f : mm;
             const float f0 = ex2(m0 - at), f1 = ex2(m1 - at), sum = sh.join_l[0][row] * f0 + sh.join_l[1][row] * f1;
-            const float norm = sum == 0.f ? 0.f : vref * 0.0078125f / sum;  // no key could be read: 0
-            const float g0 = f0, g1 = f1;
+            const int u0 = sh.join_unit[0][row], u1 = sh.join_unit[1][row], u = max(u0, u1);
+            const float norm = sum == 0.f ? 0.f : 1.f / sum, back = ldexpf(1.f, u - SHIFT);  // no key could be read: 0
+            const float g0 = f0 * power2(u0 - u) * norm, g1 = f1 * power2(u1 - u) * norm;
             const int n = row0 + row;
             T* out = static_cast<T*>(a.out) + (int64_t)(start + n / a.group) * a.ldo + ((int64_t)h * a.group + n % a.group) * D + 64 * t;
 #pragma unroll
@@ -508,7 +527,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                 tie32(o);
                 float v[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = (__uint_as_float(e[i]) * g0 + __uint_as_float(o[i]) * g1) * norm;
+                for (int i = 0; i < 32; ++i) v[i] = (__uint_as_float(e[i]) * g0 + __uint_as_float(o[i]) * g1) * back;
                 if (sh.odd) {
                     // values of the open block that are not finite reach the rows that see their tokens
                     for (int key = 0; key < min(inside, limit - whole * BLK + 1); ++key)

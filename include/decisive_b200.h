@@ -318,8 +318,8 @@ int db_kv8_append(const db_kv8_cache *cache, const void *k, int64_t ldk, const v
  * [rows, q_heads, 128]; query head h uses kv head h / (q_heads / kv_heads).  max_keys > 0: the caller's
  * estimate of the longest item's keys (table_width * 64 when nothing better is known); it sizes the launch
  * and the workspace and changes no result's meaning.  A row that can read no key (its pages are missing) is
- * 0.  More than 16 rows per kv head and item: blocks whose value scale is below 2^-24 of the largest that the row's
- * neighbours read count as 2^-24 of it.  workspace: device bytes from db_kv8_attention_workspace_bytes (may be NULL where that is 0). */
+ * 0.  More than 16 rows per kv head and item: after a block whose value scale is more than 2^80 times a later block's, the
+ * later one's values end at 2^-100 of the former's.  workspace: device bytes from db_kv8_attention_workspace_bytes (may be NULL where that is 0). */
 size_t db_kv8_attention_workspace_bytes(int64_t items, int64_t max_rows, int64_t max_keys, int64_t kv_heads,
                                         int64_t q_heads);
 int db_kv8_attention(const db_kv8_cache *cache, const void *q, int64_t ldq, const int32_t *lengths,

@@ -24,9 +24,9 @@ def cached_rows(db, dtype, k, v, q, scale=128 ** -0.5, before=0, cache=None):
 
 
 def check_rows(out, want, dtype):
-    """As check_attention, with each row's and head's own RMS as the floor."""
+    """As check_attention, with each row's and head's own RMS as the floor; f16 outputs below 2^-14 lie 2^-24 apart."""
     err = (out.double().cpu() - want).abs()
-    bound = 2 * EPS16[dtype] * (want.abs() + want.square().mean(-1, keepdim=True).sqrt())
+    bound = 2 * EPS16[dtype] * (want.abs() + want.square().mean(-1, keepdim=True).sqrt()) + (2.0 ** -24 if dtype == "f16" else 0)
     assert torch.all(err <= bound), float((err / bound).max())
 
 
@@ -43,3 +43,51 @@ def test_cache_weights_keep_their_bits(db, rows, before):
     check_rows(out, want, "bf16")
     differ = (out.cpu() != want.to(torch.bfloat16)).double().mean().item()
     assert differ <= 0.01, differ
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+def test_cache_value_scales_far_apart(db, rows):
+    """Blocks of 1e-30, of some units and of 1e20 in one sequence, every row against its own terms."""
+    gen, Hk, group, n = _gen(12), 1, 4, 230
+    k, v = (_randn(gen, n, Hk, 128, dtype=torch.bfloat16) for _ in range(2))
+    v[:64] *= 1e-30
+    v[128:192] *= 1e20
+    for before in (64 - rows // 2 - 1, 128 - rows // 2 - 1, 180, n - rows):
+        q = _randn(gen, rows, Hk * group, 128, dtype=torch.bfloat16)
+        out, want = cached_rows(db, "bf16", k[:before + rows], v[:before + rows], q, before=before)
+        check_rows(out, want, "bf16")
+
+
+@pytest.mark.parametrize("dtype,base", [("bf16", 1.0), ("f16", 1.0), ("f16", 2.0 ** 12)])
+@pytest.mark.parametrize("power", [-22, -20, -18, -16, -12, -4, 4, 12, 20])
+def test_cache_a_later_block_changes_no_earlier_row(db, dtype, base, power):
+    """256 rows at once; the second block's values are 2^-power of the others'.  Rows are as accurate as their own keys
+    allow, and what comes after a row does not reach it.  (base: the larger values; 2^12 keeps f16 outputs out of its
+    subnormals.)"""
+    if base > 1 and power > 0:
+        pytest.skip("the later block would pass f16's largest value")
+    gen, Hk, n = _gen(31 + power), 2, 256
+    q, k, v = (_randn(gen, n, Hk, 128, dtype=TYPES[dtype]) for _ in range(3))
+    v = (v.float() * base * (2.0 ** power if power < 0 else 1.0)).to(TYPES[dtype])
+    v[64:128] = (v[64:128].float() * 2.0 ** -power).to(TYPES[dtype])
+    out, want = cached_rows(db, dtype, k, v, q)
+    check_rows(out, want, dtype)
+    w = v.clone()
+    w[128:] = (w[128:].float() * 256).to(TYPES[dtype])
+    again, _ = cached_rows(db, dtype, k, w, q)
+    assert torch.equal(out[:128], again[:128])
+
+
+def test_cache_scale_of_zero(db):
+    """Codes that another program wrote under a scale of 0 are zeros, beside other blocks and alone."""
+    gen, Hk = _gen(41), 1
+    q, k, v = (_randn(gen, 128, Hk, 128, dtype=torch.bfloat16) for _ in range(3))
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for rows in (2, 128):
+        c = new_cache(db, 1, Hk, "bf16", 128, gen)
+        db.kv8_append(c, k, v, zero)
+        c.v_scales[c.page_table[0, 0].long()] = 0
+        got_k, got_v = (x[0].cpu() for x in db.kv8_read(c, zero + 128, 128))
+        out = db.kv8_attention(c, q[-rows:], zero + 128 - rows)
+        check_rows(out, attention_ref(got_k, got_v, q[-rows:].cpu(), 128 ** -0.5), "bf16")
+        assert rows < 128 or not out[:64].any()
