@@ -284,11 +284,14 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 // half `half` of score tile s, which makes P^T's fragment the four bytes 4s..4s+3 of each 16 of V^T.
 // Codes become f16 exactly; q is scaled by a power of two per row into f16 (bf16 has fewer bits
 // and more range), so the scores' product rounds neither operand.  P enters its product as two f16 parts, 22 bits (one
-// f16 would change one bf16 output in 15 and is as large a rounding as an f16 output's own); its sum is taken from the f32
-// values.  A block's own context is scaled by its value scale when it joins the running one, in f32.
+// f16 would change one bf16 output in 15 and is as large a rounding as an f16 output's own), as 2^15 P, so that f16's
+// subnormals begin 2^-29 below the largest: thousands of weak keys beside one strong one without a value still add up.  Its
+// sum is taken from the f32 values.  A block's own context is scaled by its value scale when it joins the running one, in f32.
 //
 // The tile of 8 NT query rows that a warp works on, with its running maxima and sums (log2 domain; column
 // 2 t + j of n tile n in [n][j], equal in the 8 lanes g) and its context (feature 16 d + 8 (j >> 1) + g).
+constexpr float LIFT = 15.f, DROP = 3.0517578e-5f;  // 2^-15
+
 template <typename T, int NT>
 struct Tile {
     // query fragments, k step 4 c + s: in registers, or for more rows in shared memory ([NT][8][32], the warp's own)
@@ -368,9 +371,9 @@ struct Tile {
                 for (int j = 0; j < 4; ++j) O[i][n][j] = 0.f;
     }
 
-    // S^T of the block at key `base` is in s (16 keys per tile): softmax step; leaves P in f32 in s and the
-    // factors of the running context in alpha
-    __device__ void soften(float (&s)[4][NT][4], const float (&f)[NT][2], int base, float (&alpha)[NT][2]) {
+    // S^T of the block at key `base` is in s (16 keys per tile): softmax step; leaves 2^lift P in f32 in s (drop: 2^-lift)
+    // and the factors of the running context in alpha
+    __device__ void soften(float (&s)[4][NT][4], const float (&f)[NT][2], int base, float (&alpha)[NT][2], float lift, float drop) {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         const bool masked = base + BLK - 1 > first_limit || ragged;
 #pragma unroll
@@ -401,11 +404,11 @@ struct Tile {
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float p = ex2(s[i][n][2 * half + j] - at);
+                        const float p = ex2((s[i][n][2 * half + j] - at) + lift);  // (large scores: the difference first)
                         s[i][n][2 * half + j] = p;
                         sum += p;
                     }
-                l[n][j] = l[n][j] * alpha[n][j] + sum;
+                l[n][j] = fmaf(sum, drop, l[n][j] * alpha[n][j]);
             }
         }
     }
@@ -461,15 +464,17 @@ struct Tile {
             }
         }
         if (after) load_keys(kc, after);
+        const bool lifted = vs >= 1e-30f;  // (the value scale takes the factor back, as long as it stays a normal number)
+        const float drop = lifted ? DROP : 1.f, back = vs * drop;
         float alpha[NT][2], scaled[NT][2], vf[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 scaled[n][j] = factor[n][j] * ks;
-                vf[n][j] = limit[n][j] >= base ? vs : 0.f;  // a block that a row does not see must not reach it (0 x NaN)
+                vf[n][j] = limit[n][j] >= base ? back : 0.f;  // a block that a row does not see must not reach it (0 x NaN)
             }
-        soften(s, scaled, base, alpha);
+        soften(s, scaled, base, alpha, lifted ? LIFT : 0.f, drop);
         uint32_t p[NT][4][2], rest[NT][4][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -545,12 +550,13 @@ struct Tile {
                 }
             }
         }
+        constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+        constexpr float drop = PARTS == 2 ? DROP : 1.f;
         float alpha[NT][2], unscaled[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) unscaled[n][0] = unscaled[n][1] = plain;
-        soften(s, unscaled, base, alpha);
-        // P in parts of the tail's type: two of f16 hold 22 bits, three of bf16 24
-        constexpr int PARTS = std::is_same<T, __half>::value ? 2 : 3;
+        soften(s, unscaled, base, alpha, PARTS == 2 ? LIFT : 0.f, drop);
+        // P in parts of the tail's type: two of f16 hold 22 bits, three of bf16 24 (which has no need of the lift)
         uint32_t p[PARTS][NT][4][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -633,7 +639,7 @@ struct Tile {
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            O[d][n][j] = fmaf(O[d][n][j], alpha[n][j & 1], o[d % BATCH][n][j]);
+                            O[d][n][j] = fmaf(O[d][n][j], alpha[n][j & 1], o[d % BATCH][n][j] * drop);
         }
     }
 

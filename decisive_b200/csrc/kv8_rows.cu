@@ -13,8 +13,8 @@
 // and moves, with the accumulator, to a block whose scale is above it or below 2^-6 of it, so P's parts always lie in
 // f16's normal range; a row depends only on what it sees, because the accumulator's factors are powers of two.  The
 // unit stays above 2^-80 of the largest so far (the accumulator must not overflow): under a block 2^80 times as large,
-// values end at 2^-100 of that block's.  The maximum moves only when a tile raises it by more than 8 (log2), so
-// accumulators are rarely rescaled.
+// values end at 2^-100 of that block's.  The maximum moves only when a tile raises it by more than 4 (log2), so accumulators
+// are rarely rescaled, and f16's subnormals begin 2^-23 below the maximum as a rule, 2^-19 at the least: weak keys add up.
 //
 // Warps: 0-3, 14 and 15 conversion, 4-7 softmax of even tiles, 8-11 of odd tiles, 12 and 13 MMA issue for even and odd
 // tiles (one issuer for both was the kernel's bound: 3600 of 6600 cycles per pair of tiles), 12 tensor memory.
@@ -47,7 +47,8 @@ constexpr uint64_t DRAIN_NS = 100000000ull;
 enum Bar { FULL = 0, EMPTY = FULL + STAGES, S_FULL = EMPTY + STAGES, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4,
            JOIN = PV_DONE + 4, MMA_DONE, END = MMA_DONE + 2, BARS };
 
-constexpr int SHIFT = 7;         // P of the maximum is 2^SHIFT (value scale / unit), of a key up to 8 (log2) above it 2^15 at most
+constexpr float SLACK = 4.f;     // how far (log2) a tile may lie above the running maximum
+constexpr int SHIFT = 11;        // P of the maximum is 2^SHIFT (value scale / unit), so of a key below 2^15
 constexpr int NO_SCALE = -1000;  // a value scale that moves no unit
 constexpr int LEAST = -40;       // P this far down is 0 in both parts
 struct Info {
@@ -83,7 +84,7 @@ __device__ __forceinline__ void sts128u(uint8_t* base, uint32_t at, uint32_t a, 
     *reinterpret_cast<uint4*>(base + at) = make_uint4(a, b, c, d);
 }
 
-// One row's softmax step on a tile's 64 scores: moves the maximum m (and l) if the tile raises it by more than 8, writes
+// One row's softmax step on a tile's 64 scores: moves the maximum m (and l) if the tile raises it by more than SLACK, writes
 // P = 2^(S scale + shift - m) over S as the f16 operand (32 keys to 32 columns: 16 of first parts, 16 of second), returns
 // its sum.  MASKED: only keys 0 .. seen count; a scale of 0 or NaN must not reach the others.
 template <bool MASKED>
@@ -103,7 +104,7 @@ __device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float sc
         for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(r[c][i]));
     const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
     const float mt = top == -INFINITY ? top : top * scale;
-    if (mt > m + 8.f) {  // (the first keys: from -inf)
+    if (mt > m + SLACK) {  // (the first keys: from -inf)
         move = ex2(m - mt);
         m = mt;
         l *= move;

@@ -45,6 +45,21 @@ def test_cache_weights_keep_their_bits(db, rows, before):
     assert differ <= 0.01, differ
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows", [1, 4, 30])
+def test_cache_weak_keys_add_up(db, dtype, rows):
+    """One key holds nearly all of the softmax and has no value (what models do with their first token): the output is the
+    sum of 8000 weights of 2^-24.5 each."""
+    gen, Hk, group, n = _gen(21), 1, 4, 8005
+    k = torch.zeros(n, Hk, 128, dtype=TYPES[dtype], device="cuda")
+    k[0] = 17.0 / 128 ** 0.5
+    v = _randn(gen, 1, Hk, 128, dtype=TYPES[dtype], scale=50.0).repeat(n, 1, 1)
+    v[0] = 0
+    q = torch.ones(rows, Hk * group, 128, dtype=TYPES[dtype], device="cuda")
+    out, want = cached_rows(db, dtype, k, v, q, before=n - rows)
+    check_rows(out, want, dtype)
+
+
 @pytest.mark.parametrize("rows", [1, 4, 40])
 def test_cache_value_scales_far_apart(db, rows):
     """Blocks of 1e-30, of some units and of 1e20 in one sequence, every row against its own terms."""
