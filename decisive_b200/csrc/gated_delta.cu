@@ -166,8 +166,9 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) delta_step_kernel(DeltaArgs a
 // (128 TFLOP/s).
 //
 // Numerics.  The state has to keep f32's accuracy through f16 tensor products: k and q enter them exactly
-// (bf16 rows as f16 after a power of two per row, which loses nothing within 2^-24 of the row's largest
-// value; their lengths are applied afterwards as factors per token), and every f32 operand (S, R, U, T, P) as
+// (as f16 after a power of two per row, which loses nothing within 2^-24 of the row's largest value; f16 queries as they
+// are; their lengths are applied afterwards as factors per token.  Keys need the power in f16 too: the factors of U' hold
+// 1 / |k|, and one short key would push the other tokens' U' into f16's subnormals), and every f32 operand (S, R, U, T, P) as
 // the sum of two f16 parts after a power of two: per row of the state for S and R, per chunk for T and P, so that
 // 22 bits remain of what matters.  lo x lo products are left out (2^-22).  Decay sums are taken in f64: differences
 // of f32 sums would lose what a slow decay has left.
@@ -178,7 +179,7 @@ constexpr int TRI = BLOCKS * 256;        // halves of one triangle
 enum Factor { F_R = 0, F_O = C, F_U = 2 * C, F_DECAY = 3 * C, F_T, F_P, F_OMEGA, F_REACH, F_GROW, FACTORS = 3 * C + 8 };
 
 struct ChunkSpace {
-    __half *k16, *q16;  // bf16 inputs: the rows as f16, [chunk ids][C][k_heads][D]; null for f16 inputs
+    __half *k16, *q16;  // the rows as f16 after their powers, [chunk ids][C][k_heads][D]; q16: null for f16 inputs
     __half* tri;        // [chunk ids][v_heads][4][TRI]: T hi, T lo, P hi, P lo
     float* factor;      // [chunk ids][v_heads][FACTORS]
 };
@@ -186,7 +187,7 @@ struct ChunkSpace {
 // Chunk ids: item b's chunks start at start_b / C + b, which leaves every item room for all of its chunks.
 __host__ __device__ inline int64_t chunk_ids(int64_t rows, int64_t items) { return rows / C + items; }
 
-size_t chunk_space(int64_t items, int64_t rows, int k_heads, int v_heads, bool copies, uint8_t* base, ChunkSpace* w) {
+size_t chunk_space(int64_t items, int64_t rows, int k_heads, int v_heads, bool queries, uint8_t* base, ChunkSpace* w) {
     const int64_t n = chunk_ids(rows, items);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -195,10 +196,8 @@ size_t chunk_space(int64_t items, int64_t rows, int k_heads, int v_heads, bool c
         return p;
     };
     ChunkSpace s{};
-    if (copies) {
-        s.k16 = reinterpret_cast<__half*>(take((size_t)n * C * k_heads * D * 2));
-        s.q16 = reinterpret_cast<__half*>(take((size_t)n * C * k_heads * D * 2));
-    }
+    s.k16 = reinterpret_cast<__half*>(take((size_t)n * C * k_heads * D * 2));
+    if (queries) s.q16 = reinterpret_cast<__half*>(take((size_t)n * C * k_heads * D * 2));
     s.tri = reinterpret_cast<__half*>(take((size_t)n * v_heads * 4 * TRI * 2));
     s.factor = reinterpret_cast<float*>(take((size_t)n * v_heads * FACTORS * 4));
     if (w) *w = s;
@@ -378,9 +377,9 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
     load_gates(first);
 
     // rows into shared memory as f16, with their factors
-    constexpr bool COPY = sizeof(T) == 2 && !std::is_same<T, __half>::value;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
+        const bool scaled = which == 0 || !std::is_same<T, __half>::value;
         const T* src = static_cast<const T*>(which ? a.q : a.k) + (int64_t)hk * D;
         const int64_t ld = which ? a.ldq : a.ldk;
         uint4 raw[8];
@@ -405,11 +404,11 @@ __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArg
 #pragma unroll
             for (int o = 8; o; o >>= 1) {
                 ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (COPY) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (scaled) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             }
             float back = 1.f;
             uint4 y = raw[it];
-            if (COPY) {
+            if (scaled) {
                 // 2^6 below the other operands' scale: products of two rows stay far inside f32
                 const float up = row_power(top, back) * 0.015625f;
                 back *= 64.f;
@@ -727,11 +726,10 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
                 ChainStage& st = stages[s];
                 const int row0 = start + c * C, n = min(C, end - row0);
                 const int64_t id = id0 + c;
-                const __half* k16 = w.k16 ? w.k16 + (id * C * a.k_heads + hk) * D
-                                          : static_cast<const __half*>(a.k) + (int64_t)row0 * a.ldk + (int64_t)hk * D;
+                const __half* k16 = w.k16 + (id * C * a.k_heads + hk) * D;
                 const __half* q16 = w.q16 ? w.q16 + (id * C * a.k_heads + hk) * D
                                           : static_cast<const __half*>(a.q) + (int64_t)row0 * a.ldq + (int64_t)hk * D;
-                const int64_t ldk = w.k16 ? (int64_t)a.k_heads * D : a.ldk, ldq = w.q16 ? (int64_t)a.k_heads * D : a.ldq;
+                const int64_t ldk = (int64_t)a.k_heads * D, ldq = w.q16 ? (int64_t)a.k_heads * D : a.ldq;
                 const uint32_t skq = smem_u32(st.kq), sv = smem_u32(st.v), stri = smem_u32(st.tri);
                 // 16-byte piece p of row r: column p / 8, place p % 8 ^ r % 8
                 const int p16 = lt & 15, r16 = lt >> 4;

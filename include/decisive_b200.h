@@ -276,8 +276,7 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
  * per item, state_stride floats apart (0: one kept prefix state for all items; NULL: zeros); state_out
  * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own).
  * An item without rows passes its state on.  States keep f32's accuracy within 2^-22 of the largest terms of their
- * value row (items longer than DB_DELTA_STEP_TOKENS multiply two f16 parts of every operand; f16 keys enter as they are, so with
- * norm_eps >= 0 a key row far shorter than 2^-14 of the chunk's others counts with fewer bits).  out [rows, v_heads, 128] in v's type.  workspace: device
+ * value row (items longer than DB_DELTA_STEP_TOKENS multiply two f16 parts of every operand).  out [rows, v_heads, 128] in v's type.  workspace: device
  * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0; it is 0 up to max_len =
  * DB_DELTA_STEP_TOKENS). */
 #define DB_DELTA_STEP_TOKENS 16

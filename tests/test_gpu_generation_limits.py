@@ -6,7 +6,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_generation import (EPS16, RefCache, TYPES, _gen, _randn, attention_ref, db, new_cache)  # noqa: E402,F401
+from test_gpu_generation import (EPS16, RefCache, TYPES, _gen, _randn, attention_ref, check_delta, db,  # noqa: E402
+                                 delta_inputs, delta_ref, new_cache)  # noqa: E402,F401
 
 
 def cached_rows(db, dtype, k, v, q, scale=128 ** -0.5, before=0, cache=None):
@@ -106,3 +107,17 @@ def test_cache_scale_of_zero(db):
         out = db.kv8_attention(c, q[-rows:], zero + 128 - rows)
         check_rows(out, attention_ref(got_k, got_v, q[-rows:].cpu(), 128 ** -0.5), "bf16")
         assert rows < 128 or not out[:64].any()
+
+
+@pytest.mark.parametrize("short", [1e-2, 1e-3, 1e-4, 1e-5])
+@pytest.mark.parametrize("size", [1.0, 8.0])
+@pytest.mark.parametrize("T", [64, 130])
+def test_delta_one_short_key(db, T, size, short):
+    """f16 keys as they come from a projection: one far shorter than the others costs the others nothing."""
+    gen, Hk, Hv = _gen(51), 1, 2
+    q, k, v, g, beta = delta_inputs(gen, T, Hk, Hv, torch.float16, decay=0.01)
+    k = (k.float() * size).half()
+    k[20] = (k[20].float() * short).half()
+    s = _randn(gen, 1, Hv, 128, 128, scale=0.3)
+    got = db.gated_delta(q, k, v, g, beta, state=s)
+    check_delta(got, delta_ref(q, k, v, g, beta, [T], s, 128 ** -0.5, 1e-6), "f16")
