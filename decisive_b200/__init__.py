@@ -322,7 +322,8 @@ def gated_delta(q, k, v, g, beta, items: int = 1, cu_seqlens=None, max_len: int 
     projection), g (log decay) and beta f32 [rows, v_heads].  Without cu_seqlens (int32 [items + 1] on the
     device) the items are equal; with it max_len is the longest item's rows (default: all rows, which
     is only slower).  state: f32 [items, v_heads, 128, 128], or with one item in front a kept state that
-    every item starts from; None: zeros.  state_out may be state itself.  q and k are divided by their
+    every item starts from; None: zeros.  state_out may be state itself where every
+    item has its own, and otherwise shares no memory with it.  q and k are divided by their
     lengths unless norm_eps is None.  A value that is not finite makes the outputs of its value feature (in
     v) or head (elsewhere) NaN, from the start of its block of 64 tokens at the earliest."""
     import torch

@@ -1075,6 +1075,17 @@ cudaError_t launch(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
                          db_device_error_ptr());
 }
 
+// Whether a final state lies over an initial state that is not its own item's: other CTAs would read what it writes.
+// stride: floats between initial states, one: floats of a state.
+bool states_meet(const float* in, int64_t stride, const float* out, int64_t items, int64_t one) {
+    if (!in || !out || (in == out && (items == 1 || stride == one))) return false;
+    // in floats from the first initial state: the final ones cover [begin, end); a wide stride leaves gaps between the initial
+    const int64_t begin = ((intptr_t)out - (intptr_t)in) / (int64_t)sizeof(float), end = begin + items * one;
+    if (stride == 0) return begin < one && end > 0;
+    const int64_t first = begin < one ? 0 : (begin - one) / stride + 1;  // the first item whose state ends past begin
+    return first < items && first * stride < end;
+}
+
 }  // namespace
 }  // namespace db
 
@@ -1110,9 +1121,9 @@ int db_gated_delta(const void* q, const void* k, const void* v, int dtype, int64
                        "gated delta rule: rows and states start on 16-byte boundaries");
     if (state_in && state_stride != 0 && state_stride < v_heads * 128 * 128)
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "gated delta rule: states overlap");
-    if (state_in && state_in == state_out && items > 1 && state_stride != v_heads * 128 * 128)
+    if (db::states_meet(state_in, state_stride, state_out, items, v_heads * 128 * 128))
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT",
-                       "gated delta rule: a state shared by several items cannot be updated in place");
+                       "gated delta rule: a state can be updated in place only by its own item");
     if (!workspace && db_gated_delta_workspace_bytes(items, rows, max_len, k_heads, v_heads, dtype))
         return db_fail(DB_ERR_INVALID_ARGUMENT, "INVALID_ARGUMENT", "gated delta rule: a workspace is needed");
     db::DeltaArgs a{};

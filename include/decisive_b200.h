@@ -274,7 +274,8 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
  * norm_eps >= 0: k' = k / sqrt(sum k^2 + norm_eps), q' = scale * q / sqrt(sum q^2 + norm_eps); norm_eps < 0:
  * k' = k, q' = scale * q.  g = -inf forgets everything before the token.  state_in f32 [v_heads, 128, 128]
  * per item, state_stride floats apart (0: one kept prefix state for all items; NULL: zeros); state_out
- * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own).
+ * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own, and otherwise
+ * shares no memory with it).
  * An item without rows passes its state on.  States keep f32's accuracy within 2^-22 of the largest terms of their
  * value row (items longer than DB_DELTA_STEP_TOKENS multiply two f16 parts of every operand).  out [rows, v_heads, 128] in v's type.  workspace: device
  * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0; it is 0 up to max_len =

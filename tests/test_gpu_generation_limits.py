@@ -121,3 +121,17 @@ def test_delta_one_short_key(db, T, size, short):
     s = _randn(gen, 1, Hv, 128, 128, scale=0.3)
     got = db.gated_delta(q, k, v, g, beta, state=s)
     check_delta(got, delta_ref(q, k, v, g, beta, [T], s, 128 ** -0.5, 1e-6), "f16")
+
+
+@pytest.mark.parametrize("T", [3, 70])
+def test_delta_states_side_by_side(db, T):
+    """Initial and final states in one buffer, next to one another or the same, give what separate ones give."""
+    gen, Hk, Hv, B = _gen(52), 1, 2, 2
+    q, k, v, g, beta = delta_inputs(gen, B * T, Hk, Hv, torch.bfloat16)
+    pool = _randn(gen, 5, Hv, 128, 128, scale=0.3)
+    for first, last, shared in ((0, 2, False), (2, 0, False), (3, 3, False), (2, 0, True), (1, 2, True), (0, 3, True)):
+        mine = pool.clone()
+        start = mine[first:first + (1 if shared else B)]
+        want_out, want = db.gated_delta(q, k, v, g, beta, items=B, state=start.clone())
+        out, got = db.gated_delta(q, k, v, g, beta, items=B, state=start, state_out=mine[last:last + B])
+        assert torch.equal(out, want_out) and torch.equal(got, want)
