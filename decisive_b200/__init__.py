@@ -301,6 +301,31 @@ def _raw_stream(device: int):
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+# The library launches on the current device, counts its SMs and notes errors in its error word: calls run with the
+# tensors' device current.
+def _launch(device: int, entry, *args):
+    import torch
+    if torch._C._cuda_getDevice() == device:
+        check(entry(*args, _raw_stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, _raw_stream(device)))
+
+
+def _workspace(device: int, like, size, *args):
+    """The bytes that size(*args) asks for, from torch's allocator: (tensor, its address), or None twice."""
+    import torch
+    if torch._C._cuda_getDevice() == device:
+        need = size(*args)
+    else:
+        with torch.cuda.device(device):
+            need = size(*args)
+    if not need:
+        return None, None
+    ws = torch.empty(need, dtype=torch.uint8, device=like.device)
+    return ws, ws.data_ptr()
+
+
 def _code16(dtype, name):
     import torch
     if dtype == torch.bfloat16:
@@ -364,14 +389,12 @@ def gated_delta(q, k, v, g, beta, items: int = 1, cu_seqlens=None, max_len: int 
         rows_o, ho, ldo = _heads("out", out, dt, dev)
         if rows_o != rows or ho != hv:
             raise ValueError("gated_delta: out differs from v in its shape")
-    lib, ws = load(), None
+    lib, ws, at = load(), None, None
     if max_len > DELTA_STEP_TOKENS:
-        need = lib.db_gated_delta_workspace_bytes(items, rows, max_len, hk, hv, code)
-        ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
-    check(lib.db_gated_delta(q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ldq, ldk, ldv, g.data_ptr(),
-                             beta.data_ptr(), ld[0], ld[1], cu, items, rows, max_len, hk, hv, 128, scale,
-                             -1.0 if norm_eps is None else norm_eps, si, stride, so, out.data_ptr(), ldo,
-                             ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
+        ws, at = _workspace(dev, v, lib.db_gated_delta_workspace_bytes, items, rows, max_len, hk, hv, code)
+    _launch(dev, lib.db_gated_delta, q.data_ptr(), k.data_ptr(), v.data_ptr(), code, ldq, ldk, ldv, g.data_ptr(),
+            beta.data_ptr(), ld[0], ld[1], cu, items, rows, max_len, hk, hv, 128, scale,
+            -1.0 if norm_eps is None else norm_eps, si, stride, so, out.data_ptr(), ldo, at)
     return out, state_out
 
 
@@ -450,8 +473,7 @@ def kv8_append(cache: KvCache8, k, v, lengths, cu_seqlens=None, max_rows: int | 
     if rows_v != rows or heads_v != heads or heads != cache.kv_heads:
         raise ValueError("kv8_append: k or v differs from the cache in its heads or rows")
     items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)
-    check(load().db_kv8_append(cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, ln, cu, items, rows, most,
-                               _raw_stream(dev)))
+    _launch(dev, load().db_kv8_append, cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, ln, cu, items, rows, most)
 
 
 def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | None = None,
@@ -459,7 +481,6 @@ def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | 
     """Attention over the cache after the append of the same rows: row i of item b sees the cached keys
     0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: the longest item's keys, as far as the caller
     knows (default: the table's width); it only sizes the launch and the workspace."""
-    import torch
     dt, dev = cache.dtype, cache.device
     rows, heads, ldq = _heads("q", q, dt, dev)
     items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)
@@ -470,10 +491,9 @@ def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | 
         if rows_o != rows or heads_o != heads:
             raise ValueError("kv8_attention: out differs from q in its shape")
     lib, keys = load(), max(1, max_keys or cache.table_width * 64)
-    need = lib.db_kv8_attention_workspace_bytes(items, most, keys, cache.kv_heads, heads)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(lib.db_kv8_attention(cache.ref, q.data_ptr(), ldq, ln, cu, items, rows, most, keys, heads, scale,
-                               out.data_ptr(), ldo, ws.data_ptr() if ws is not None else None, _raw_stream(dev)))
+    ws, at = _workspace(dev, q, lib.db_kv8_attention_workspace_bytes, items, most, keys, cache.kv_heads, heads)
+    _launch(dev, lib.db_kv8_attention, cache.ref, q.data_ptr(), ldq, ln, cu, items, rows, most, keys, heads, scale,
+            out.data_ptr(), ldo, at)
     return out
 
 
@@ -485,7 +505,7 @@ def kv8_read(cache: KvCache8, lengths, max_keys: int):
     items, _, ln, _ = _kv8_items(dev, 0, lengths, None, None)
     k, v = (torch.empty((items, max_keys, cache.kv_heads, 128), dtype=torch.float32, device=cache.k_tail.device)
             for _ in range(2))
-    check(load().db_kv8_read(cache.ref, ln, items, max_keys, k.data_ptr(), v.data_ptr(), _raw_stream(dev)))
+    _launch(dev, load().db_kv8_read, cache.ref, ln, items, max_keys, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -519,14 +539,15 @@ def logit_rules(logits, history=None, history_lengths=None, repetition=None, pre
         if out.shape != logits.shape or out.dtype != f32 or (vocab > 1 and step != 1) or out.get_device() != dev:
             raise ValueError("logit_rules: out is f32 with dense rows, of the logits' shape")
     best, lse = out.new_empty(one, dtype=i32), out.new_empty(one)
-    check(load().db_logit_rules(
+    _launch(
+        dev, load().db_logit_rules,
         logits.data_ptr(), 0 if dt == f32 else 1 if dt == torch.float16 else 2, ld if rows > 1 else vocab, rows, vocab,
         _array("history", history, i32, (rows, cols), dev), cols,
         _array("history_lengths", history_lengths, i32, one, dev), cols, _array("repetition", repetition, f32, one, dev),
         _array("presence", presence, f32, one, dev), _array("frequency", frequency, f32, one, dev),
         _array("bias_ids", bias_ids, i32, (rows, biases), dev),
         _array("bias_values", bias_values, f32, (rows, biases), dev), biases, _array("mask", mask, i32, (rows, words), dev),
-        words, out.data_ptr(), ldo if rows > 1 else vocab, best.data_ptr(), lse.data_ptr(), _raw_stream(dev)))
+        words, out.data_ptr(), ldo if rows > 1 else vocab, best.data_ptr(), lse.data_ptr())
     return out, best, lse
 
 
