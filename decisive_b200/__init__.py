@@ -404,7 +404,8 @@ class KvCache8:
 
     k_codes [pages, kv_heads, 64, 128], v_codes [pages, kv_heads, 128, 64] int8; k_scales, v_scales f32
     [pages, kv_heads]; k_tail [sequences, kv_heads, 64, 128], v_tail [sequences, kv_heads, 128, 64] f16 or
-    bf16; page_table int32 [sequences, table_width]: the page of each block, the caller's to fill."""
+    bf16; page_table int32 [sequences, table_width]: the page of each block, the caller's to fill.  page_table may be set
+    to another tensor (a wider one, for longer sequences); the others are fixed, and other tensors another KvCache8."""
 
     BLOCK = 64
     __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "page_table", "dtype", "device",
@@ -418,7 +419,7 @@ class KvCache8:
         pages, heads = k_scales.shape
         sequences, width = page_table.shape
         code = _code16(dt, "KvCache8")
-        self._c = _lib.KvCache8(
+        c = _lib.KvCache8(
             _array("k_codes", k_codes, torch.int8, (pages, heads, 64, 128), dev),
             _array("k_scales", k_scales, f32, (pages, heads), dev),
             _array("v_codes", v_codes, torch.int8, (pages, heads, 128, 64), dev),
@@ -427,10 +428,23 @@ class KvCache8:
             _array("v_tail", v_tail, dt, (sequences, heads, 128, 64), dev),
             _array("page_table", page_table, torch.int32, (sequences, width), dev),
             pages, width, sequences, heads, 128, code)
-        self.k_codes, self.k_scales, self.v_codes, self.v_scales = k_codes, k_scales, v_codes, v_scales
-        self.k_tail, self.v_tail, self.page_table = k_tail, v_tail, page_table
-        self.dtype, self.device, self.kv_heads, self.table_width = dt, dev, heads, width
-        self.ref = C.byref(self._c)
+        self._keep(k_codes=k_codes, k_scales=k_scales, v_codes=v_codes, v_scales=v_scales, k_tail=k_tail, v_tail=v_tail,
+                   page_table=page_table, dtype=dt, device=dev, kv_heads=heads, table_width=width, _c=c, ref=C.byref(c))
+
+    def _keep(self, **fields):
+        for name, value in fields.items():
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        # calls read the addresses in _c, so a tensor has to be checked and entered there
+        if name != "page_table":
+            raise AttributeError(f"KvCache8.{name} is fixed")
+        import torch
+        if len(value.shape) != 2:
+            raise ValueError("KvCache8: page_table [sequences, width] is wanted")
+        at = _array("page_table", value, torch.int32, (self._c.sequences, value.shape[1]), self.device)
+        self._c.page_table, self._c.table_width = at, value.shape[1]
+        self._keep(page_table=value, table_width=value.shape[1])
 
     @classmethod
     def allocate(cls, sequences: int, pages: int, table_width: int, kv_heads: int, dtype, device="cuda") -> "KvCache8":

@@ -87,3 +87,26 @@ def test_calls_run_on_the_tensors_device(monkeypatch):
     assert [c[0] for c in launches] == ["db_gated_delta", "db_kv8_append", "db_kv8_attention", "db_kv8_read", "db_logit_rules"]
     assert len(gpu.calls) == 7 and all(c[1] == 1 for c in gpu.calls)  # workspaces are sized for the tensors' device too
     assert all(c[2] == 101 for c in launches) and gpu.current == [0]
+
+
+def test_cache_follows_its_tensors(monkeypatch):
+    """Calls read the addresses that the cache holds: a new page table is entered, nothing else can be swapped unseen."""
+    import decisive_b200 as db
+    torch = pytest.importorskip("torch")
+    f16, f32, i32, i8 = torch.float16, torch.float32, torch.int32, torch.int8
+    gpu = OnGpu1(db, monkeypatch)
+    codes = lambda *s: gpu.zeros(i8, 3, 2, *s)  # noqa: E731
+    scales, tail = gpu.zeros(f32, 3, 2), gpu.zeros(f16, 2, 2, 64, 128)
+    cache = db.KvCache8(codes(64, 128), scales, codes(128, 64), scales, tail, tail.view(2, 2, 128, 64), gpu.zeros(i32, 2, 3))
+    wider = gpu.zeros(i32, 2, 9)
+    cache.page_table = wider
+    assert cache.page_table is wider and cache.table_width == 9
+    held = cache.ref._obj
+    assert held.page_table == wider.data_ptr() and held.table_width == 9 and held.sequences == 2
+    for bad in (gpu.zeros(i32, 3, 9), gpu.zeros(torch.int64, 2, 9), gpu.zeros(i32, 2, 18)[:, ::2], gpu.zeros(i32, 18)):
+        with pytest.raises(ValueError):
+            cache.page_table = bad
+    assert cache.page_table is wider and held.page_table == wider.data_ptr()
+    for name in ("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail", "table_width", "kv_heads", "dtype"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name))
