@@ -43,6 +43,10 @@ cudaError_t db_set_max_smem(const void* kernel, int bytes) {
     return e;
 }
 
+// The error word is a variable of the library's image, there and zero on every device that loads it: a first call may
+// be captured in a CUDA graph, where memory could be neither allocated nor cleared.
+static __device__ int error_word;
+
 int* db_device_error_ptr() {
     static std::mutex mu;
     static std::vector<int*> words;
@@ -51,8 +55,14 @@ int* db_device_error_ptr() {
     std::lock_guard<std::mutex> lock(mu);
     if ((int)words.size() <= dev) words.resize(dev + 1, nullptr);
     if (!words[dev]) {
-        if (cudaMalloc(&words[dev], sizeof(int)) != cudaSuccess) return nullptr;
-        cudaMemset(words[dev], 0, sizeof(int));
+        // (a first look loads the image, which a capture allows in relaxed mode)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        void* p = nullptr;
+        const cudaError_t e = cudaGetSymbolAddress(&p, error_word);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return nullptr;
+        words[dev] = static_cast<int*>(p);
     }
     return words[dev];
 }

@@ -1,5 +1,8 @@
 """The generation operators where their numerics or their bookkeeping are at their limits: few bits of the softmax weights,
 value scales far apart, keys of very different lengths, long sequences, rows that are cut off, graph capture."""
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -8,6 +11,8 @@ pytestmark = pytest.mark.gpu
 
 from test_gpu_generation import (EPS16, RefCache, TYPES, _gen, _randn, attention_ref, check_delta, db,  # noqa: E402
                                  delta_inputs, delta_ref, new_cache)  # noqa: E402,F401
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def cached_rows(db, dtype, k, v, q, scale=128 ** -0.5, before=0, cache=None):
@@ -29,6 +34,9 @@ def check_rows(out, want, dtype):
     err = (out.double().cpu() - want).abs()
     bound = 2 * EPS16[dtype] * (want.abs() + want.square().mean(-1, keepdim=True).sqrt()) + (2.0 ** -24 if dtype == "f16" else 0)
     assert torch.all(err <= bound), float((err / bound).max())
+
+
+
 
 
 @pytest.mark.parametrize("rows,before", [(2, 20), (2, 300), (4, 300), (100, 0), (40, 300)])
@@ -135,3 +143,55 @@ def test_delta_states_side_by_side(db, T):
         want_out, want = db.gated_delta(q, k, v, g, beta, items=B, state=start.clone())
         out, got = db.gated_delta(q, k, v, g, beta, items=B, state=start, state_out=mine[last:last + B])
         assert torch.equal(out, want_out) and torch.equal(got, want)
+
+
+CAPTURE = """
+import sys
+sys.path.insert(0, {root!r})
+import torch, decisive_b200 as db
+gen = torch.Generator("cuda").manual_seed(1)
+B, Hk, Hq, V = 2, 2, 8, 5000
+def randn(*shape): return torch.randn(shape, generator=gen, device="cuda").bfloat16()
+def inputs(T):
+    q, k, v = randn(B * T, Hq, 128), randn(B * T, Hk, 128), randn(B * T, Hk, 128)
+    return [q, k, v, -torch.rand(B * T, Hq, generator=gen, device="cuda"), torch.rand(B * T, Hq, generator=gen, device="cuda"),
+            randn(B, V)]
+def state():
+    c = db.KvCache8.allocate(B, 20, 10, Hk, torch.bfloat16)
+    return [c, torch.zeros(B, Hq, 128, 128, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda"),
+            torch.randint(V, (B, 7), generator=torch.Generator("cuda").manual_seed(2), device="cuda", dtype=torch.int32)]
+def step(x, s, T):
+    q, k, v, g, beta, logits = x
+    db.kv8_append(s[0], k, v, s[2])
+    a = db.kv8_attention(s[0], q, s[2])
+    d, _ = db.gated_delta(k, k, q, g, beta, items=B, state=s[1], state_out=s[1])
+    r = db.logit_rules(logits, s[3], repetition=torch.full((B,), 1.5, device="cuda"))
+    s[2].add_(T)
+    return [a, d, *r]
+plan = [(40, [inputs(40) for _ in range(2)]), (1, [inputs(1) for _ in range(3)])]
+eager, captured = state(), state()
+torch.cuda.synchronize()
+for T, steps in plan:
+    hold = [x.clone() for x in steps[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # the first calls of this process
+        got = step(hold, captured, T)
+    for x in steps:
+        for a, b in zip(hold, x):
+            a.copy_(b)
+        graph.replay()
+        want = step(x, eager, T)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+assert torch.equal(eager[1], captured[1]) and torch.equal(eager[2], captured[2])
+assert db.device_error_word() == 0
+print("captured")
+"""
+
+
+def test_calls_can_be_captured(db):
+    """A process whose first calls are captured in a CUDA graph; replays with other inputs, lengths and states are what
+    calls outside a graph give."""
+    r = subprocess.run([sys.executable, "-c", CAPTURE.format(root=ROOT)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
