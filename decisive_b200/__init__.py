@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 import json
 from dataclasses import dataclass, field
+from operator import attrgetter
 
 from . import _lib
 from ._lib import CudaError, check, load
@@ -408,8 +409,8 @@ class KvCache8:
     to another tensor (a wider one, for longer sequences); the others are fixed, and other tensors another KvCache8."""
 
     BLOCK = 64
-    __slots__ = ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "page_table", "dtype", "device",
-                 "kv_heads", "table_width", "_c", "ref")
+    __slots__ = ("_k_codes", "_k_scales", "_v_codes", "_v_scales", "_k_tail", "_v_tail", "_page_table", "_dtype", "_device",
+                 "_kv_heads", "_table_width", "_c", "ref")
 
     def __init__(self, k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, page_table):
         import torch
@@ -428,23 +429,29 @@ class KvCache8:
             _array("v_tail", v_tail, dt, (sequences, heads, 128, 64), dev),
             _array("page_table", page_table, torch.int32, (sequences, width), dev),
             pages, width, sequences, heads, 128, code)
-        self._keep(k_codes=k_codes, k_scales=k_scales, v_codes=v_codes, v_scales=v_scales, k_tail=k_tail, v_tail=v_tail,
-                   page_table=page_table, dtype=dt, device=dev, kv_heads=heads, table_width=width, _c=c, ref=C.byref(c))
+        self._k_codes, self._k_scales, self._v_codes, self._v_scales = k_codes, k_scales, v_codes, v_scales
+        self._k_tail, self._v_tail, self._page_table = k_tail, v_tail, page_table
+        self._dtype, self._device, self._kv_heads, self._table_width = dt, dev, heads, width
+        self._c, self.ref = c, C.byref(c)
 
-    def _keep(self, **fields):
-        for name, value in fields.items():
-            object.__setattr__(self, name, value)
+    # calls read the addresses in _c, so another tensor has to be checked and entered there
+    k_codes, k_scales, v_codes, v_scales, k_tail, v_tail, dtype, device, kv_heads, table_width = (
+        property(attrgetter("_" + name)) for name in ("k_codes", "k_scales", "v_codes", "v_scales", "k_tail", "v_tail", "dtype",
+                                                      "device", "kv_heads", "table_width"))
 
-    def __setattr__(self, name, value):
-        # calls read the addresses in _c, so a tensor has to be checked and entered there
-        if name != "page_table":
-            raise AttributeError(f"KvCache8.{name} is fixed")
+    @property
+    def page_table(self):
+        return self._page_table
+
+    @page_table.setter
+    def page_table(self, value):
         import torch
         if len(value.shape) != 2:
             raise ValueError("KvCache8: page_table [sequences, width] is wanted")
-        at = _array("page_table", value, torch.int32, (self._c.sequences, value.shape[1]), self.device)
-        self._c.page_table, self._c.table_width = at, value.shape[1]
-        self._keep(page_table=value, table_width=value.shape[1])
+        width = value.shape[1]
+        self._c.page_table = _array("page_table", value, torch.int32, (self._c.sequences, width), self._device)
+        self._c.table_width = self._table_width = width
+        self._page_table = value
 
     @classmethod
     def allocate(cls, sequences: int, pages: int, table_width: int, kv_heads: int, dtype, device="cuda") -> "KvCache8":
@@ -481,10 +488,10 @@ def kv8_append(cache: KvCache8, k, v, lengths, cu_seqlens=None, max_rows: int | 
     """Writes the items' new rows (k, v [rows, kv_heads, 128]) at positions lengths[b] (int32, device) on;
     blocks that fill up are quantised.  The lengths stay as they are: advance them once every layer has
     taken the step.  cu_seqlens and max_rows as in gated_delta."""
-    dt, dev = cache.dtype, cache.device
+    dt, dev = cache._dtype, cache._device
     rows, heads, ldk = _heads("k", k, dt, dev)
     rows_v, heads_v, ldv = _heads("v", v, dt, dev)
-    if rows_v != rows or heads_v != heads or heads != cache.kv_heads:
+    if rows_v != rows or heads_v != heads or heads != cache._kv_heads:
         raise ValueError("kv8_append: k or v differs from the cache in its heads or rows")
     items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)
     _launch(dev, load().db_kv8_append, cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, ln, cu, items, rows, most)
@@ -495,7 +502,7 @@ def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | 
     """Attention over the cache after the append of the same rows: row i of item b sees the cached keys
     0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: the longest item's keys, as far as the caller
     knows (default: the table's width); it only sizes the launch and the workspace."""
-    dt, dev = cache.dtype, cache.device
+    dt, dev = cache._dtype, cache._device
     rows, heads, ldq = _heads("q", q, dt, dev)
     items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)
     if out is None:
@@ -504,8 +511,8 @@ def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | 
         rows_o, heads_o, ldo = _heads("out", out, dt, dev)
         if rows_o != rows or heads_o != heads:
             raise ValueError("kv8_attention: out differs from q in its shape")
-    lib, keys = load(), max(1, max_keys or cache.table_width * 64)
-    ws, at = _workspace(dev, q, lib.db_kv8_attention_workspace_bytes, items, most, keys, cache.kv_heads, heads)
+    lib, keys = load(), max(1, max_keys or cache._table_width * 64)
+    ws, at = _workspace(dev, q, lib.db_kv8_attention_workspace_bytes, items, most, keys, cache._kv_heads, heads)
     _launch(dev, lib.db_kv8_attention, cache.ref, q.data_ptr(), ldq, ln, cu, items, rows, most, keys, heads, scale,
             out.data_ptr(), ldo, at)
     return out
@@ -515,9 +522,9 @@ def kv8_read(cache: KvCache8, lengths, max_keys: int):
     """The cached keys and values of tokens 0 .. max_keys - 1, f32 [items, max_keys, kv_heads, 128] each
     (0 from lengths[b] on)."""
     import torch
-    dev = cache.device
+    dev = cache._device
     items, _, ln, _ = _kv8_items(dev, 0, lengths, None, None)
-    k, v = (torch.empty((items, max_keys, cache.kv_heads, 128), dtype=torch.float32, device=cache.k_tail.device)
+    k, v = (torch.empty((items, max_keys, cache._kv_heads, 128), dtype=torch.float32, device=cache._k_tail.device)
             for _ in range(2))
     _launch(dev, load().db_kv8_read, cache.ref, ln, items, max_keys, k.data_ptr(), v.data_ptr())
     return k, v
