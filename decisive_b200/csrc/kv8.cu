@@ -689,11 +689,13 @@ __host__ __device__ constexpr int part_floats(int nt) { return (32 + 4) * nt * 3
 struct Units {
     int64_t total;  // units of all items, one head
     int per;
+    bool cut;       // some item has rows that are cut off
 };
 // Blocks that item b's rows see.
+__device__ __forceinline__ int blocks_of(int count, int len) { return count > 0 ? (len + count - 1) / BLK + 1 : 0; }
 __device__ __forceinline__ int item_blocks(const Kv8Args& a, int b, int& start, int& count, int& len) {
     item_of(a, b, start, count, len);
-    return count > 0 ? (len + count - 1) / BLK + 1 : 0;
+    return blocks_of(count, len);
 }
 __device__ __forceinline__ int item_units(const Kv8Args& a, int b, int& start, int& count, int& len) {
     const int n = item_blocks(a, b, start, count, len);
@@ -706,9 +708,13 @@ __device__ Units count_units(const Kv8Args& a, int64_t* sums) {  // sums: [THREA
     Units u;
     u.per = (a.items + THREADS - 1) / THREADS;
     int64_t mine = 0;
+    int cut = 0;
     for (int b = tid * u.per; b < min((tid + 1) * u.per, a.items); ++b) {
-        int s, c, l;
-        mine += item_units(a, b, s, c, l);
+        int s, c, l, off;
+        item_of(a, b, s, c, l, off);
+        const int n = blocks_of(c, l);
+        mine += n ? n + TILE_COST : 0;
+        cut |= off;
     }
     int64_t run = mine;
 #pragma unroll
@@ -721,7 +727,7 @@ __device__ Units count_units(const Kv8Args& a, int64_t* sums) {  // sums: [THREA
     for (int w = 0; w < (tid >> 5); ++w) run += warp_sum[w];
     sums[tid + 1] = run;
     if (tid == 0) sums[0] = 0;
-    __syncthreads();
+    u.cut = __syncthreads_or(cut);
     u.total = sums[THREADS];
     return u;
 }
@@ -753,6 +759,7 @@ __global__ void __launch_bounds__(32 * DECODE_WARPS, 2) kv8_decode_kernel(AttnAr
     pdl_wait();
     pdl_trigger();
     const Units units = count_units<32 * DECODE_WARPS>(a.kv, sums);
+    for (int b = blockIdx.x; units.cut && b < a.kv.items; b += gridDim.x) zero_cut_rows<T>(a, b, 0, Hk * a.group);
     const int64_t all = units.total * Hk, per = run_length(all, (int64_t)gridDim.x * DECODE_WARPS);
     const int64_t w = (int64_t)blockIdx.x * DECODE_WARPS + warp, begin = w * per, end = min(begin + per, all);
     // units run (item, head, block): the items before x units of one head take x Hk units

@@ -21,24 +21,31 @@ struct Kv8Args {
     int* error;
 };
 
-// Item b: rows [start, start + count) of this call, `len` tokens cached before them.  Offsets and
-// lengths outside the tensors are brought back inside and noted in the error word.
-__device__ __forceinline__ void item_of(const Kv8Args& a, int b, int& start, int& count, int& len) {
+// Item b: rows [start, start + count) of this call, `len` tokens cached before them; `cut` more rows are not taken (past
+// max_rows, or past the table).  Offsets and lengths outside the tensors are brought back inside, and that and cut rows are
+// noted in the error word.
+__device__ __forceinline__ void item_of(const Kv8Args& a, int b, int& start, int& count, int& len, int& cut) {
+    int rows = a.max_rows;
     if (a.cu) {
         start = min(max(a.cu[b], 0), a.rows);
-        count = min(min(max(a.cu[b + 1], start), a.rows) - start, a.max_rows);
+        rows = min(max(a.cu[b + 1], start), a.rows) - start;
     } else {
         start = b * a.max_rows;
-        count = a.max_rows;
     }
     const int64_t most = (int64_t)a.c.table_width * KV8_BLK;
     const int given = a.lengths[b];
+    count = min(rows, a.max_rows);
     len = given;
     if (given < 0 || (int64_t)given + count > most) {
         len = given < 0 ? 0 : (int)min((int64_t)given, most);
         count = (int)min((int64_t)count, most - len);
-        if (a.error && threadIdx.x == 0) atomicOr(a.error, DB_DEV_ERR_SHAPE);
     }
+    cut = rows - count;
+    if ((given != len || cut) && a.error && threadIdx.x == 0) atomicOr(a.error, DB_DEV_ERR_SHAPE);
+}
+__device__ __forceinline__ void item_of(const Kv8Args& a, int b, int& start, int& count, int& len) {
+    int cut;
+    item_of(a, b, start, count, len, cut);
 }
 
 // The page that holds block i of item b, or -1 (noted in the error word) where the table names none.
@@ -96,6 +103,17 @@ struct AttnArgs {
     float factor;  // scale * log2 e
     float* parts;  // decode: partial results, see kv8_decode_kernel
 };
+
+// Item b's cut rows are 0 in the output: its query heads `first` .. + heads - 1, by all threads of a CTA.
+template <typename T>
+__device__ __forceinline__ void zero_cut_rows(const AttnArgs& a, int b, int first, int heads) {
+    int start, count, len, cut;
+    item_of(a.kv, b, start, count, len, cut);
+    T* out = static_cast<T*>(a.out) + (int64_t)(start + count) * a.ldo + (int64_t)first * KV8_D;
+    const int pieces = heads * (KV8_D / 8);
+    for (int64_t i = threadIdx.x; i < (int64_t)cut * pieces; i += blockDim.x)
+        *reinterpret_cast<uint4*>(out + i / pieces * a.ldo + i % pieces * 8) = make_uint4(0, 0, 0, 0);
+}
 
 // Many query rows (kv8_rows.cu).
 template <typename T>

@@ -159,6 +159,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
     const int h = blockIdx.y, b = blockIdx.z, Hk = a.kv.c.kv_heads;
     pdl_wait();
     pdl_trigger();
+    if (blockIdx.x == 0) zero_cut_rows<T>(a, b, h * a.group, a.group);
     int start, count, len;
     item_of(a.kv, b, start, count, len);
     // the last tiles see the most keys: they start first

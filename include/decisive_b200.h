@@ -260,7 +260,8 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
 
 /* ---- generation operators.  Packed rows: `items` sequences' rows lie one after another; cu_seqlens
  * (device, int32 [items + 1]) gives their offsets, NULL means equal items (rows = items * max_len).
- * max_len / max_rows is the longest item's rows; it sizes the launch (the cache entries cut longer items to it).
+ * max_len / max_rows is the longest item's rows; it sizes the launch (the cache entries cut longer items to it; rows cut
+ * off, these and those past the page table, are not cached, 0 in an output, and noted).
  * Row strides are in elements; rows of 16-bit tensors start on 16-byte boundaries (stride % 8 == 0).
  * head_dim is 128; other values give DB_ERR_UNSUPPORTED.  Device-side offsets, lengths and page numbers outside
  * their tensors are brought back inside or skipped; the cache entries note them in the error word

@@ -145,6 +145,36 @@ def test_delta_states_side_by_side(db, T):
         assert torch.equal(out, want_out) and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("rows", [3, 40])
+def test_cache_rows_cut_off_are_zero(db, rows):
+    """Rows past max_rows, past the table, or of an item without room are 0, and the error word says so."""
+    gen, Hk, Hq = _gen(61), 1, 4
+    n = 2 * rows
+    q, k, v = (_randn(gen, n, h, 128, dtype=torch.float16) for h in (Hq, Hk, Hk))
+    cu = torch.tensor([0, rows, n], dtype=torch.int32, device="cuda")
+
+    def call(lengths, most, cu):
+        c = new_cache(db, 2, Hk, "f16", 64, gen)  # two or three blocks
+        lengths = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+        assert db.device_error_word() == 0
+        db.kv8_append(c, k, v, lengths, cu_seqlens=cu, max_rows=most)
+        assert db.device_error_word() == 0x10
+        out = db.kv8_attention(c, q, lengths, cu_seqlens=cu, max_rows=most, out=torch.full_like(q, 7.0))
+        assert db.device_error_word() == 0x10
+        return out, c.table_width * 64
+
+    out, _ = call([0, 0], rows - 1, cu)
+    _, want = cached_rows(db, "f16", k[:rows - 1], v[:rows - 1], q[:rows - 1])
+    check_rows(out[:rows - 1], want, "f16")
+    assert not out[rows - 1].any() and not out[n - 1].any() and out[n - 2].any()
+    width = call([0, 0], rows - 1, cu)[1]
+    for c in (cu, None):
+        out, _ = call([0, width - 1], rows, c)
+        assert out[:rows].any(-1).all() and out[rows].any() and not out[rows + 1:].any()
+        out, _ = call([width, 2**31 - 1], rows, c)
+        assert not out.any()
+
+
 CAPTURE = """
 import sys
 sys.path.insert(0, {root!r})
