@@ -4,13 +4,14 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_gpu_generation import (EPS16, RefCache, TYPES, _gen, _randn, attention_ref, check_delta, db,  # noqa: E402
-                                 delta_inputs, delta_ref, new_cache)  # noqa: E402,F401
+                                 delta_inputs, delta_ref, new_cache, rules_ref)  # noqa: F401
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -175,6 +176,36 @@ def test_cache_rows_cut_off_are_zero(db, rows):
         assert not out.any()
 
 
+def test_cache_attention_over_long_histories(db):
+    """9000 keys of one head for one token: more parts than the join takes at a time; 3000 keys under a chunk of rows: more
+    blocks than the many-row kernel keeps scales of."""
+    gen, Hk, group = _gen(71), 1, 4
+    for dtype in TYPES:
+        for n, rows in ((9000, 1), (9001, 3), (3000, 40), (2990, 200)):
+            k, v = (_randn(gen, n, Hk, 128, dtype=TYPES[dtype]) for _ in range(2))
+            q = _randn(gen, rows, Hk * group, 128, dtype=TYPES[dtype])
+            out, want = cached_rows(db, dtype, k, v, q, before=n - rows)
+            check_rows(out, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_delta_thousands_of_tokens(db, dtype):
+    """129 chunks under a slow decay.  To the 4e-6 of the state's RMS that one chunk may cost (see check_delta) come the
+    roundings of 129 hand-overs, 2^-23 of the row's largest value (4 x RMS) each and at random: sqrt(129) 2^-21 / sqrt(12) =
+    1.6e-6.  6e-6 and 6e-5 are allowed."""
+    gen, Hk, Hv, T = _gen(81), 1, 2, 8229
+    q, k, v, g, beta = delta_inputs(gen, T, Hk, Hv, TYPES[dtype], decay=0.001)
+    s = _randn(gen, 1, Hv, 128, 128, scale=0.3)
+    out, state = db.gated_delta(q, k, v, g, beta, state=s)
+    want, want_state = delta_ref(q, k, v, g, beta, [T], s, 128 ** -0.5, 1e-6)
+    err = (out.double().cpu() - want).abs()
+    rms = want.square().mean().sqrt().item()
+    assert torch.all(err <= 2 * EPS16[dtype] * (want.abs() + rms)), float((err / (want.abs() + rms)).max())
+    d = state.double().cpu() - want_state
+    srms = want_state.square().mean().sqrt().item()
+    assert d.square().mean().sqrt().item() <= 6e-6 * srms and d.abs().max().item() <= 6e-5 * srms
+
+
 CAPTURE = """
 import sys
 sys.path.insert(0, {root!r})
@@ -225,3 +256,18 @@ def test_calls_can_be_captured(db):
     calls outside a graph give."""
     r = subprocess.run([sys.executable, "-c", CAPTURE.format(root=ROOT)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("V,H,B", [(786432, 70000, 1), (786432, 100, 3), (600001, 65536, 2), (400000, 65535, 5)])
+def test_rules_largest_vocabularies(db, V, H, B):
+    """The largest vocabularies, with histories on both sides of what 16-bit counters hold, one id throughout a row."""
+    gen = _gen(V + H)
+    x = _randn(gen, B, V, scale=3.0)
+    hist = torch.randint(0, V, (B, H), generator=gen, device="cuda", dtype=torch.int32)
+    hist[0] = V - 1
+    rho, pres, freq = (torch.rand(B, generator=gen, device="cuda") + o for o in (0.7, 0.1, 0.1))
+    mask = torch.randint(-2**31, 2**31 - 1, (B, (V + 31) // 32), generator=gen, device="cuda").to(torch.int32)
+    out, best, lse = db.logit_rules(x, hist, None, rho, pres, freq, mask=mask)
+    want, wbest, wlse = rules_ref(x, hist, None, rho, pres, freq, None, None, mask)
+    assert (out.cpu().numpy() == want).all() and best.tolist() == wbest
+    assert np.allclose(lse.cpu().numpy(), np.array(wlse), rtol=2e-6, atol=1e-5)  # as in test_rules_match_the_definition
