@@ -65,7 +65,8 @@ struct Shared {
     int join_unit[2][ROWS];
     uint32_t tmem;
     int abort;
-    uint32_t tail_k, tail_v;        // the open block's largest magnitudes (16-bit bits)
+    uint32_t tail_v;                // bf16: the open block's largest value (its bits)
+    alignas(16) float key_up[BLK], key_back[BLK];  // bf16: the open block's keys' powers of two
     int odd;                        // the open block has values that are not finite
 };
 constexpr int SMEM = 1024 + Q_BYTES + STAGES * STAGE + sizeof(Shared);
@@ -85,9 +86,10 @@ __device__ __forceinline__ void sts128u(uint8_t* base, uint32_t at, uint32_t a, 
 }
 
 // One row's softmax step on a tile's 64 scores: moves the maximum m (and l) if the tile raises it by more than SLACK, writes
-// P = 2^(S scale + shift - m) over S as the f16 operand (32 keys to 32 columns: 16 of first parts, 16 of second), returns
+// P = 2^(S scale + shift - m) over S as the operand (32 keys to 32 columns: 16 of first parts, 16 of second), returns
 // its sum.  MASKED: only keys 0 .. seen count; a scale of 0 or NaN must not reach the others.
-template <bool MASKED>
+// PT: the type of P's parts.
+template <bool MASKED, typename PT = __half>
 __device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float scale, float shift, float& m, float& l, float& move,
                                         uint32_t s_tm) {
     if (MASKED) {
@@ -126,15 +128,45 @@ __device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float sc
             }
             const uint64_t xy = f2_pack(__float_as_uint(x), __float_as_uint(y));
             sum[i & 1] = f2_add(sum[i & 1], xy);
-            pk[i] = pack2<__half>(x, y);
-            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&pk[i]));
-            const uint64_t left = f2_fma(f2_pack(__float_as_uint(h.x), __float_as_uint(h.y)), minus, xy);
-            pk[16 + i] = pack2<__half>(f2_lo(left), f2_hi(left));
+            pk[i] = pack2<PT>(x, y);
+            const uint64_t h = f2_pack(__float_as_uint(from_bits<PT>(pk[i] & 0xffffu)), __float_as_uint(from_bits<PT>(pk[i] >> 16)));
+            const uint64_t left = f2_fma(h, minus, xy);
+            pk[16 + i] = pack2<PT>(f2_lo(left), f2_hi(left));
         }
         chain::tmem_st32(s_tm + 32u * c, pk);
     }
     const uint64_t both = f2_add(sum[0], sum[1]);
     return f2_lo(both) + f2_hi(both);
+}
+
+// The same for the open block of a bf16 cache, whose keys have a power of two each (backs: their inverses, in shared memory)
+// and whose P has bf16 parts, 0 unless `some` -> (sum, m, l, move).  Out of line, because the loop over the full blocks must stay small: with
+// this beside it a tile took half as long again.
+__device__ __noinline__ float4 soften_open(uint32_t s_tm, int seen, float factor, uint32_t backs, float shift, float m, float l, bool some) {
+    uint32_t r[2][32];
+    tmem_ld_32x32b_x32(s_tm, r[0]);
+    tmem_ld_32x32b_x32(s_tm + 32u, r[1]);
+    tmem_wait_ld(r[0]);
+    tie32(r[1]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            float x[4];
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(backs + 128u * c + 4u * i));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[c][i + j] = __float_as_uint(__uint_as_float(r[c][i + j]) * (x[j] * factor));
+        }
+    float move = 1.f;
+    const float sum = soften<true, __nv_bfloat16>(r, seen, 1.f, shift, m, l, move, s_tm);
+    if (!some) {
+        tmem_wait_st();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[0][i] = 0;
+        chain::tmem_st32(s_tm, r[0]);
+        chain::tmem_st32(s_tm + 32u, r[0]);
+    }
+    return make_float4(sum, m, l, move);
 }
 
 // A bounded wait for roles that run ahead: the thread sleeps between its looks.
@@ -148,7 +180,8 @@ __device__ __forceinline__ bool warp_wait_idle(uint64_t* bar, uint32_t parity, v
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
-    constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    constexpr bool WIDE = !std::is_same<T, __half>::value;  // the open block may pass f16's range
+    constexpr uint32_t INF = WIDE ? 0x7f80u : 0x7c00u;
     extern __shared__ uint8_t rows_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rows_smem) + 1023) & ~uintptr_t(1023));
     uint8_t* ring = smem + Q_BYTES;
@@ -188,7 +221,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         mbar_init(&sh.bars[MMA_DONE + 1], 1);
         mbar_init(&sh.bars[END], THREADS / 32);
         sh.abort = 0;
-        sh.tail_k = sh.tail_v = 0;
+        sh.tail_v = 0;
         sh.odd = 0;
         fence_barrier_init();
     }
@@ -217,11 +250,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
         *reinterpret_cast<uint2*>(smem + at) = make_uint2(pack2<__half>(x[0] * up, x[1] * up), pack2<__half>(x[2] * up, x[3] * up));
     }
     __syncthreads();
-    // the open block's magnitudes
+    // The open block is exact, whatever its tokens' magnitudes: f16 as it is (its value scale is 1); bf16 keys as f16 after a
+    // power of two each, which goes into their scores, and bf16 values as bf16 after one for all, with P's parts in bf16.
     {
-        uint32_t km = 0, vm = 0;
+        uint32_t vm = 0;
         bool odd = false;
         for (int e = tid; inside && e < BLK * D / 8; e += THREADS) {
+            uint32_t km = 0;
             const uint4 k = *reinterpret_cast<const uint4*>(kt + 8 * e), v = *reinterpret_cast<const uint4*>(vt + 8 * e);
             const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
             const bool key_there = e / (D / 8) < inside;
@@ -233,13 +268,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                     if (y < INF) vm = max(vm, y); else odd = true;
                 }
             }
+            if constexpr (WIDE) {
+                // 16 lanes hold a key
+#pragma unroll
+                for (int o = 8; o; o >>= 1) km = max(km, __shfl_xor_sync(0xffffffffu, km, o));
+                if (lane % 16 == 0) sh.key_up[e / 16] = code_power(from_bits<T>(km), sh.key_back[e / 16]);
+            }
         }
         if (inside) {
-            km = __reduce_max_sync(0xffffffffu, km);
-            vm = __reduce_max_sync(0xffffffffu, vm);
-            if (lane == 0) {
-                atomicMax(&sh.tail_k, km);
-                atomicMax(&sh.tail_v, vm);
+            if constexpr (WIDE) {
+                vm = __reduce_max_sync(0xffffffffu, vm);
+                if (lane == 0) atomicMax(&sh.tail_v, vm);
             }
             if (__any_sync(0xffffffffu, odd) && lane == 0) sh.odd = 1;
         }
@@ -249,8 +288,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
-    float kt_back, vt_back;
-    const float kt_up = code_power(from_bits<T>(sh.tail_k), kt_back), vt_up = code_power(from_bits<T>(sh.tail_v), vt_back);
+    float vt_back = 1.f;
+    const float vt_up = WIDE ? code_power(from_bits<T>(sh.tail_v), vt_back) : 1.f;
 
     if (warp < 4 || warp > 13) {
         // ---------------------------------------------------------------- codes -> f16 tiles
@@ -312,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             const bool tail = j == whole && inside, paged = (unsigned)page < (unsigned)a.kv.c.pages;
             if (j < known && !paged && lane == 0 && err) atomicOr(err, DB_DEV_ERR_SHAPE);
             Info n;
-            n.ks = paged ? ks : kt_back;
+            n.ks = paged ? ks : 1.f;
             const float v_scale = paged ? vs : vt_back;
             scales_of(i + CONVERTERS, next_page);
             const uint4* src = codes_of(i + CONVERTERS, next_page);
@@ -344,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                     const uint4* from = reinterpret_cast<const uint4*>((is_v ? vt : kt) + 16 * q);
                     const uint4 x = from[0], y = from[1];
                     const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                    const float up = is_v ? vt_up : kt_up;
+                    const float up = is_v ? vt_up : WIDE ? sh.key_up[q >> 3] : 1.f;
                     uint32_t f[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -353,7 +392,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
                         // slots without a token, and values (not keys) that are not finite, stay out of the products
                         if (key >= inside || (is_v && (l & INF) == INF)) l = 0;
                         if (key + (is_v ? 1 : 0) >= inside || (is_v && (g & INF) == INF)) g = 0;
-                        f[e] = pack2<__half>(from_bits<T>(l) * up, from_bits<T>(g) * up);
+                        const float a = from_bits<T>(l) * up, b = from_bits<T>(g) * up;
+                        f[e] = !WIDE ? l | g << 16 : is_v ? pack2<T>(a, b) : pack2<__half>(a, b);
                     }
                     const int r = is_v ? q >> 2 : q >> 3, half = is_v ? 0 : (q >> 2) & 1, p0 = 2 * (q & 3);
                     const uint32_t row = half * K_HALF + r * 128;
@@ -379,6 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
     } else if (warp >= 12) {
         // ---------------------------------------------------------------- MMA issue, one parity of tiles
         constexpr uint32_t IDESC_S = idesc_f16_f32(ROWS, BLK), IDESC_O = idesc_f16_f32(ROWS, D);
+        constexpr uint32_t IDESC_OPEN = WIDE ? IDESC_O | 1u << 7 | 1u << 10 : IDESC_O;  // (bf16 x bf16)
         const int t = warp - 12;
         const uint64_t dQ = sw128_desc(smem_u32(smem)), dR = sw128_desc(smem_u32(ring));
         const uint32_t s_tm = tmem + 128u * t, o_tm = tmem + TM_O + 128u * t;
@@ -411,18 +452,25 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             ok = ok && warp_wait(&sh.bars[P_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_MMA);
             if (!ok) return;
             tc_fence_after();
-            if (chain::elect()) {
-                const uint64_t dV = dR + (uint64_t)((st * STAGE) >> 4);
+            // (the descriptor a constant of each branch: an operand that is not keeps the MMAs' others out of uniform registers)
+            auto issue = [&](auto idesc) {
+                if (chain::elect()) {
+                    const uint64_t dV = dR + (uint64_t)((st * STAGE) >> 4);
 #pragma unroll
-                for (int kk = 0; kk < BLK / 16; ++kk) {
-                    // 32 keys lie in 32 columns: 16 of the first parts, 16 of the second
-                    const uint32_t at = s_tm + 64u * slot + 32u * (kk >> 1) + 8u * (kk & 1);
-                    chain::umma_f16_ts(o_tm, at + 16u, dV + (uint64_t)(kk * 2), IDESC_O, p > 0 || kk > 0);
-                    chain::umma_f16_ts(o_tm, at, dV + (uint64_t)(kk * 2), IDESC_O, 1);
+                    for (int kk = 0; kk < BLK / 16; ++kk) {
+                        // 32 keys lie in 32 columns: 16 of the first parts, 16 of the second
+                        const uint32_t at = s_tm + 64u * slot + 32u * (kk >> 1) + 8u * (kk & 1);
+                        chain::umma_f16_ts(o_tm, at + 16u, dV + (uint64_t)(kk * 2), idesc, p > 0 || kk > 0);
+                        chain::umma_f16_ts(o_tm, at, dV + (uint64_t)(kk * 2), idesc, 1);
+                    }
+                    umma_commit(&sh.bars[EMPTY + st]);
+                    umma_commit(&sh.bars[PV_DONE + 2 * t + slot]);
                 }
-                umma_commit(&sh.bars[EMPTY + st]);
-                umma_commit(&sh.bars[PV_DONE + 2 * t + slot]);
-            }
+            };
+            if (WIDE && 2 * p + t == whole && inside)
+                issue(std::integral_constant<uint32_t, IDESC_OPEN>());
+            else
+                issue(std::integral_constant<uint32_t, IDESC_O>());
             __syncwarp();
         };
         scores(0);
@@ -453,13 +501,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             if (!(ok = warp_wait(&sh.bars[S_FULL + 2 * t + slot], (p >> 1) & 1, abort_flag, err, DB_DEV_ERR_TIMEOUT_EPI))) break;
             tc_fence_after();
             const Info n = sh.info[(2 * p + t) & (INFO - 1)];
-            uint32_t r[2][32];
-            tmem_ld_32x32b_x32(s_tm, r[0]);
-            tmem_ld_32x32b_x32(s_tm + 32u, r[1]);
-            tmem_wait_ld(r[0]);
-            tie32(r[1]);
             const int seen = n.there ? limit - base : -1;  // keys 0 .. seen of the tile
-            const float scale = factor * n.ks;
             float move = 1.f, all;
             int raise = 0;
             if (n.there && n.e != NO_SCALE) {
@@ -474,10 +516,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_rows_kernel(AttnArgs a) {
             }
             const int down = n.e == NO_SCALE ? LEAST : max(SHIFT + n.e - unit, LEAST);
             const float shift = (float)down + n.lf;
-            if (__any_sync(0xffffffffu, seen < BLK - 1))
-                all = soften<true>(r, seen, scale, shift, m, l, move, s_tm);
-            else
-                all = soften<false>(r, seen, scale, shift, m, l, move, s_tm);
+            uint32_t r[2][32];
+            if (WIDE && 2 * p + t == whole && inside) {
+                const float4 x = soften_open(s_tm, seen, factor, smem_u32(sh.key_back), shift, m, l, down > LEAST);
+                all = x.x, m = x.y, l = x.z, move = x.w;
+            } else {
+                tmem_ld_32x32b_x32(s_tm, r[0]);
+                tmem_ld_32x32b_x32(s_tm + 32u, r[1]);
+                tmem_wait_ld(r[0]);
+                tie32(r[1]);
+                const float scale = factor * n.ks;
+                if (__any_sync(0xffffffffu, seen < BLK - 1))
+                    all = soften<true>(r, seen, scale, shift, m, l, move, s_tm);
+                else
+                    all = soften<false>(r, seen, scale, shift, m, l, move, s_tm);
+            }
             if (all != 0.f) l = fmaf(all, n.inv * power2(-down), l);
             move *= power2(raise);
             // O is stable once the previous P V of this parity is done

@@ -117,6 +117,48 @@ def test_cache_scale_of_zero(db):
         check_rows(out, attention_ref(got_k, got_v, q[-rows:].cpu(), 128 ** -0.5), "bf16")
         assert rows < 128 or not out[:64].any()
 
+@pytest.mark.parametrize("dtype,values,keys", [("bf16", 6.0, 0.0), ("bf16", 2.0, 3.0), ("f16", 1.5, 1.0)])
+@pytest.mark.parametrize("rows,before", [(4, 20), (50, 0), (60, 40)])
+def test_cache_open_block_is_exact(db, dtype, values, keys, rows, before):
+    """Tokens of the open block whose keys and values differ by many powers of ten: each row has the accuracy of what it sees.
+    Weights in 16 bits or more (2^-17, twice for their sum), scores from 8 sums of 2^-23 of their terms, the output's own
+    rounding; and weights of the full block end at 2^-30 of the largest (f16's last bit, 2^-25, under 2^5)."""
+    gen, Hk, group, n = _gen(91 + rows), 2, 4, before + rows
+    k, v = (_randn(gen, n, Hk, 128) for _ in range(2))
+    k = (k * torch.exp(keys * _randn(gen, n, 1, 1)).clamp(max=1e3)).to(TYPES[dtype])
+    v = (v * torch.exp(values * _randn(gen, n, 1, 1)).clamp(max=1e3 if dtype == "f16" else 1e30)).to(TYPES[dtype])
+    q = _randn(gen, rows, Hk * group, 128, dtype=TYPES[dtype], scale=0.3)
+    out, want = cached_rows(db, dtype, k, v, q, before=before)
+    ref = RefCache(1, Hk, TYPES[dtype])
+    ref.append(k, v, [n])
+    k64, v64, q64 = ref.values(ref.k[0]).double(), ref.values(ref.v[0]).double(), q.double().cpu()
+    for i in range(rows):
+        seen = before + i + 1
+        for h in range(Hk * group):
+            kh, vh = k64[:seen, h // group], v64[:seen, h // group]
+            weights = torch.softmax((kh @ q64[i, h]) * 128 ** -0.5, 0)
+            terms, size = weights @ vh.abs(), (kh.abs() @ q64[i, h].abs()).max().item() * 128 ** -0.5
+            bound = EPS16[dtype] * want[i, h].abs() + (2 * 2.0 ** -17 + 2 * 1.45 * size * 2.0 ** -20) * terms
+            bound += vh.abs().sum(0) * 2.0 ** -30 + (2.0 ** -24 if dtype == "f16" else 0)
+            err = (out[i, h].double().cpu() - want[i, h]).abs()
+            assert torch.all(err <= bound), (i, h, float((err / bound).nan_to_num().max()))
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_cache_open_block_under_a_far_larger_one(db, rows):
+    """Values of 1e-12 after a block of 1e20: they may end at 2^-100 of it, but come out no larger than they are."""
+    gen, Hk, n = _gen(95), 1, 64 + 45
+    k, v = (_randn(gen, n, Hk, 128, dtype=torch.bfloat16) for _ in range(2))
+    v[:64] *= 1e20
+    v[:64, :, 64:] = 0
+    v[64:] *= 1e-12
+    q = _randn(gen, rows, Hk * 4, 128, dtype=torch.bfloat16)
+    out, want = cached_rows(db, "bf16", k, v, q, before=n - rows)
+    check_rows(out[..., :64], want[..., :64], "bf16")
+    small, exact = out[..., 64:].double().cpu(), want[..., 64:]
+    assert torch.all((small - exact).abs() <= 2 * EPS16["bf16"] * exact.abs() + 1e20 * 2.0 ** -100)
+    assert small.abs().max() < 1e-10
+
 
 @pytest.mark.parametrize("short", [1e-2, 1e-3, 1e-4, 1e-5])
 @pytest.mark.parametrize("size", [1.0, 8.0])
