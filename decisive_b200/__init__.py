@@ -487,7 +487,8 @@ def _kv8_items(device: int, rows: int, lengths, cu_seqlens, max_rows):
 def kv8_append(cache: KvCache8, k, v, lengths, cu_seqlens=None, max_rows: int | None = None) -> None:
     """Writes the items' new rows (k, v [rows, kv_heads, 128]) at positions lengths[b] (int32, device) on;
     blocks that fill up are quantised.  The lengths stay as they are: advance them once every layer has
-    taken the step.  cu_seqlens and max_rows as in gated_delta."""
+    taken the step.  cu_seqlens and max_rows as cu_seqlens and max_len in gated_delta, but rows past max_rows or past
+    the page table are not cached, and device_error_word notes them."""
     dt, dev = cache._dtype, cache._device
     rows, heads, ldk = _heads("k", k, dt, dev)
     rows_v, heads_v, ldv = _heads("v", v, dt, dev)
@@ -501,7 +502,8 @@ def kv8_attention(cache: KvCache8, q, lengths, cu_seqlens=None, max_rows: int | 
                   max_keys: int | None = None, scale: float = 128 ** -0.5, out=None):
     """Attention over the cache after the append of the same rows: row i of item b sees the cached keys
     0 .. lengths[b] + i -> [rows, q_heads, 128].  max_keys: the longest item's keys, as far as the caller
-    knows (default: the table's width); it only sizes the launch and the workspace."""
+    knows (default: the table's width); it only sizes the launch and the workspace.  Rows that the append left out
+    are 0."""
     dt, dev = cache._dtype, cache._device
     rows, heads, ldq = _heads("q", q, dt, dev)
     items, most, ln, cu = _kv8_items(dev, rows, lengths, cu_seqlens, max_rows)

@@ -159,19 +159,21 @@ __global__ void __launch_bounds__(32 * STEP_WARPS) delta_step_kernel(DeltaArgs a
 // the chunk,
 //   A_ij = beta_i e^(G_i - G_j) k_i.k_j (j < i),  T = (I + A)^-1 diag(beta),  P_ij = e^(G_i - G_j) q_i.k_j (j <= i)
 //   U = T (V - diag(e^G) K S0^T),  O = diag(e^G) Q S0^T + P U,  S1 = e^G_C S0 + sum_i e^(G_C - G_i) u_i k_i^T
-// T and P need no state: delta_prepare_kernel forms them for all chunks at once; delta_chain_kernel then
-// walks a sequence's chunks.  Chunks of 64: the walk's steps are a chain whose length is the number of chunks, and
-// 64 is the largest chunk whose triangles' parts fit in shared memory twice.  B200, 16 key and 32 value heads:
-// 512 tokens 55 us, 8229 tokens 625 us (48 TFLOP/s counted as the recurrence), 64 items of 16 to 1024 tokens 0.97 ms
-// (128 TFLOP/s).
+// (the chunked form of the delta rule that was published as "Parallelizing Linear Transformers with the Delta Rule over
+// Sequence Length", 2024, with decays).  T and P need no state: delta_prepare_kernel forms them for all chunks at once;
+// delta_chain_kernel then walks a sequence's chunks.  Chunks of 64: the walk's steps are a chain whose length is the number
+// of chunks, and 64 is the largest chunk whose triangles' parts fit in shared memory twice.  B200, 16 key and 32 value
+// heads: 512 tokens 55 us, 8229 tokens 629 us (48 TFLOP/s counted as the recurrence), 64 items of 16 to 1024 tokens 1.00 ms
+// (124 TFLOP/s).
 //
-// Numerics.  The state has to keep f32's accuracy through f16 tensor products: k and q enter them exactly
-// (as f16 after a power of two per row, which loses nothing within 2^-24 of the row's largest value; f16 queries as they
-// are; their lengths are applied afterwards as factors per token.  Keys need the power in f16 too: the factors of U' hold
-// 1 / |k|, and one short key would push the other tokens' U' into f16's subnormals), and every f32 operand (S, R, U, T, P) as
-// the sum of two f16 parts after a power of two: per row of the state for S and R, per chunk for T and P, so that
-// 22 bits remain of what matters.  lo x lo products are left out (2^-22).  Decay sums are taken in f64: differences
-// of f32 sums would lose what a slow decay has left.
+// Numerics.  The state has to keep f32's accuracy through f16 tensor products: k and q enter them exactly (as f16 after a
+// power of two per row, which loses nothing within 2^-24 of the row's largest value; f16 queries as they are; their lengths
+// are applied afterwards as factors per token.  Keys need the power in f16 too: the factors of U' hold 1 / |k|, and one short
+// key would push the other tokens' U' into f16's subnormals), and every f32 operand (S, R, U, T, P) as the sum of two f16
+// parts after a power of two: per row of the state for S and R, per chunk for T and P, so that 22 bits remain of what
+// matters: a token whose values lie 2^-20 below the largest of their feature in its chunk keeps fewer, a row of the state
+// likewise under terms that its own decay has since removed.  lo x lo products are left out (2^-22).  Decay sums are taken in
+// f64: differences of f32 sums would lose what a slow decay has left.
 constexpr int C = 64;                    // tokens per chunk
 constexpr int BLOCKS = 10;               // 16 x 16 blocks of a lower triangle of 64, 512 bytes each, row-major
 constexpr int TRI = BLOCKS * 256;        // halves of one triangle
@@ -293,7 +295,7 @@ __device__ __forceinline__ void block_product(float (&o)[R], const float* a, con
 // mma.sync, once for the value heads of a key head; the inverse by blocks, -T11 A10 T00 from 16 x 16 to 64 x 64, in f32, because
 // an f16 product would lose what the state is to keep.  Bound by shared memory's latency
 // and wavefronts (58% of their rate; issue 47%) and the barriers between its short steps, which 4 CTAs an SM cover in part.
-// B200: 0.37 ms of the 0.97 ms of 64 items, 0.10 ms of the 0.63 of 8229 tokens.
+// B200: 0.40 ms of the 1.00 ms of 64 items, 0.10 ms of the 0.63 of 8229 tokens.
 template <typename T>
 __global__ void __launch_bounds__(PREP_THREADS, 4) delta_prepare_kernel(DeltaArgs a, ChunkSpace w, int heads) {
     extern __shared__ __align__(16) uint8_t prep_smem[];
@@ -600,8 +602,9 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, boo
 // has them as its rows (A from tensor memory, B from shared memory), and nothing of the chain passes through shared
 // memory:
 //   X = S [K; Q]^T,  R = V - e^G X_k,  U = R T^T,  S <- e^G_C S + U' K,  O = e^G X_q + U P^T
-// The state stays in tensor memory as its two parts (together f32's 24 bits); tensor-core sums enter it by one f32
-// fma, because the cores' own accumulation truncates.  The powers of two that keep parts in range come from bounds,
+// The state stays in tensor memory as its two parts (22 bits and the second part's sign: off by 2^-23 of a value at most,
+// where f32 would be by 2^-24; 129 chunks with hardly any decay stay within 6e-6 of its RMS); tensor-core sums enter it by
+// one f32 fma, because the cores' own accumulation truncates.  The powers of two that keep parts in range come from bounds,
 // max |S k| <= sqrt(128) |k| max |S| for R, e^G_C max |S| + max |U| sum e^(G_C-G_i) |k_i| for the next S; the slack of a
 // bound (2^6) costs nothing, because f16 parts of a row scaled to 2^15 reach down to 2^-40 of it.
 // The code is kept small: what the warps of an SM run between two products has to stay in its instruction cache.
@@ -1048,8 +1051,9 @@ __global__ void __launch_bounds__(CHAIN_THREADS, 1) delta_chain_kernel(DeltaArgs
     }
 }
 
-// Up to this many tokens per item the recurrence is faster than a chunk (128 items of 32 heads, recurrence / chunks, us:
-// 8 tokens 209 / 565, 16 379 / 571, 24 551 / 577, 32 724 / 581; one item: 16 20 / 36, 32 23 / 31, 64 38 / 31).
+// Up to this many tokens per item the recurrence runs, whatever the items: one number, because callers size the workspace by
+// it.  It is on the safe side of both crossings (recurrence / chunks, us, 32 heads, 128 items: 8 tokens 216 / 564, 16 385 / 568,
+// 24 559 / 575, 32 731 / 577; one item: 8 11 / 34, 16 14 / 34, 32 25 / 34, 48 33 / 34, 64 43 / 34).
 constexpr int STEP_TOKENS = DB_DELTA_STEP_TOKENS;
 
 template <typename T>
@@ -1063,7 +1067,7 @@ cudaError_t launch(const DeltaArgs& a, void* workspace, cudaStream_t stream) {
     cudaError_t e = db_set_max_smem(reinterpret_cast<const void*>(delta_prepare_kernel<T>), sizeof(PrepShared));
     if (e != cudaSuccess) return e;
     // a CTA per value head while that still finds idle SMs, else one for all that share a key head (per value head / per
-    // key head, us of the whole call: 512 tokens 57 / 61, 8229 tokens 663 / 636, 64 items of 16 to 1024 tokens 1122 / 1002)
+    // key head, us of the whole call: 512 tokens 58 / 62, 8229 tokens 664 / 632, 64 items of 16 to 1024 tokens 1144 / 1004)
     const int64_t ids = chunk_ids(a.rows, a.items);
     const int group = a.v_heads / a.k_heads, heads = ids * a.k_heads < 4 * db_num_sms() ? 1 : group;
     e = db_launch_pdl(delta_prepare_kernel<T>, dim3((unsigned)ids, a.k_heads, (group + heads - 1) / heads), dim3(PREP_THREADS),

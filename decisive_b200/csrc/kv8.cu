@@ -142,8 +142,9 @@ __global__ void __launch_bounds__(APPEND_THREADS)
             a.c.k_scales[ph] = ks;
             a.c.v_scales[ph] = vs;
         }
-        // round half even (x / s): the product with 1 / s (off by 2^-16 at most) decides unless it lies near a half.  1.5 x
-        // 2^23 + code has the code's two's complement in its low byte, and |x / s| never passes 127.
+        // round half even (x / s): the product with 1 / s (off by 2^-16 at most) decides unless it lies near a half.  Rounding by
+        // a large addend is a common technique: 1.5 x 2^23 + code has the code's two's complement in its low byte, and |x / s|
+        // never passes 127.
         const float ki = __fdiv_rn(1.f, ks), vi = __fdiv_rn(1.f, vs);
         constexpr float MAGIC = 12582912.f;
         auto four = [](const float (&x)[4], float s, float inverse) {
@@ -678,10 +679,10 @@ struct Tile {
 // cost more than their blocks); so sequences of any lengths keep every warp busy alike, and no warp waits for another.  A
 // warp writes the tiles whose blocks it has all; of a tile that it shares it leaves (O, m, l) in its slot
 // 0 (the tile began before its run) or 1 (it goes on after it), and kv8_join_kernel adds the slots up in order.
-// HBM bound: the codes are read once, straight into the fragments' registers.  B200, 32 / 8 heads: 4 items of 60 to 65
-// thousand keys 109 us (4.8 TB/s, 73% of the copy's rate), 64 items of 1 to 8191 keys 130 us (3.9 TB/s; the f16 form's second
-// part of P is what it adds), one item of 544 keys 13 us and 12 us
-// for the join.
+// Bound by HBM and by the issue of what turns codes into products (P's second part, without which bf16 took 90 us where it
+// takes 101): the codes are read once, straight into the fragments' registers.  B200, 32 / 8 heads, this kernel alone, f16
+// and bf16 alike: 4 items of 60 to 65 thousand keys 101 us (5.2 TB/s, 80% of the copy's rate), 64 items of 1 to 8191 keys
+// 111 us (4.6 TB/s); one item of 544 keys 14 us and 12 us for the join.
 constexpr int DECODE_WARPS = 4, TILE_COST = 2;
 __host__ __device__ constexpr int part_floats(int nt) { return (32 + 4) * nt * 32; }  // O and m, l in the lanes' order
 
@@ -904,9 +905,11 @@ __global__ void __launch_bounds__(256 * NT) kv8_join_kernel(AttnArgs a, int64_t 
 }
 
 // ------------------------------------------------------------------ launches
-// n tiles of 8 rows for the dealt-out form; 0: many rows (kv8_rows.cu).  One tile / two / many rows, us, bf16, 8 kv heads:
-// 64 items of 4000 keys, 4 rows per kv head 113 / 213 / 307, 8 rows 114 / 214 / 307, 16 rows - / 216 / 309; one item of 32000
-// keys, 4 rows 54 / 69 / 440, 16 rows - / 70 / 441; 4 items of 512 keys, 16 rows - / 37 / 29.
+// n tiles of 8 rows for the dealt-out form; 0: many rows (kv8_rows.cu), which is all there is above 16.  One tile / two / many
+// rows, us with the join, bf16, 8 kv heads: 64 items of 4000 keys, 4 rows per kv head 132 / 216 / 356, 8 rows 134 / 216 / 358,
+// 16 rows - / 218 / 362; one item of 32000 keys, 4 rows 58 / 73 / 506, 16 rows - / 73 / 506; 4 items of 512 keys, 4 rows
+// 22 / 26 / 23, 16 rows - / 26 / 23.  So rows decide: the many-row form gains 3 us on short histories and loses most of
+// its time on long ones, where it has a CTA per 128 rows and kv head and does not split the keys (20 rows: 367, 510, 23 us).
 int decode_tiles(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 0; }
 // CTAs of the dealt-out form: as many as are resident at once, fewer when there are not that many blocks
 int64_t decode_ctas(int64_t items, int64_t heads, int64_t max_keys) {

@@ -70,7 +70,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Four int8 codes as two pairs of f16, exactly: the bytes become the low bits of 1024 + (code + 128).
+// Four int8 codes as two pairs of f16, exactly, by the common technique of putting bits under a fixed exponent: the bytes
+// become the low bits of 1024 + (code + 128).
 __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t& hi) {
     c ^= 0x80808080u;
     const uint32_t l = __byte_perm(c, 0x64646464u, 0x4140), h = __byte_perm(c, 0x64646464u, 0x4342);

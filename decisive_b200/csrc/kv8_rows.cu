@@ -7,12 +7,12 @@
 //   S = Q K^T (codes as exact f16),  P = 2^(S c - m),  O += P V (codes as exact f16)
 // Six warps turn codes into f16 tiles in shared memory, in the order in which the MMAs take them; a value page is
 // stored [128][64 tokens], which is already the K-major operand.  P stays in tensor memory: it overwrites S
-// and is the A operand of the second product, as two f16 parts, 22 bits (one f16 would change one bf16 output in 15).  Where scales go: a
-// key block's into the exponent's factor, a value block's into P, relative to the accumulator's unit, a power of two
-// of its warpgroup's; the row sum is taken back by the inverse.  The unit starts at 2 to 4 times the first block's value scale
-// and moves, with the accumulator, to a block whose scale is above it or below 2^-6 of it, so P's parts always lie in
-// f16's normal range; a row depends only on what it sees, because the accumulator's factors are powers of two.  The
-// unit stays above 2^-80 of the largest so far (the accumulator must not overflow): under a block 2^80 times as large,
+// and is the A operand of the second product, as two f16 parts, 22 bits (one f16 would change one bf16 output in 15).
+// Where scales go: a key block's into the exponent's factor, a value block's into P, relative to the accumulator's unit, a
+// power of two of its warpgroup's; the row sum is taken back by the inverse.  The unit starts at 2 to 4 times the first
+// block's value scale and moves, with the accumulator, to a block whose scale is above it or below 2^-6 of it, so the
+// largest P lie far inside f16's normal range; a row depends only on what it sees, because the accumulator's factors are
+// powers of two.  The unit stays above 2^-80 of the largest so far (the accumulator must not overflow): under a block 2^80 times as large,
 // values end at 2^-100 of that block's.  The maximum moves only when a tile raises it by more than 4 (log2), so accumulators
 // are rarely rescaled, and f16's subnormals begin 2^-23 below the maximum as a rule, 2^-19 at the least: weak keys add up.
 //
@@ -20,8 +20,8 @@
 // tiles (one issuer for both was the kernel's bound: 3600 of 6600 cycles per pair of tiles), 12 tensor memory.
 // Latency bound: each chain hands S, P and O from role to role, and two chains fill the gaps only in part; a CTA takes an
 // SM whole (shared memory, tensor memory), so 2000 rows of 8 kv heads are one round of 128 CTAs.  B200, 1000 rows after 7000
-// keys, 16 / 8 heads: 144 us for f16 (426 TFLOP/s, 26% of the dense f16 rate; P's second part is a third of the products
-// and not counted), 133 us for bf16.
+// keys, 16 / 8 heads: 149 us, f16 and bf16 (412 TFLOP/s, 25% of the dense f16 rate; P's second part is a third of the
+// products and not counted).
 // Tensor memory (512 columns): S / P of (parity, slot) at 128 parity + 64 slot, O even 256-383, O odd 384-511.
 #include <float.h>
 
@@ -140,9 +140,10 @@ __device__ __forceinline__ float soften(uint32_t (&r)[2][32], int seen, float sc
 }
 
 // The same for the open block of a bf16 cache, whose keys have a power of two each (backs: their inverses, in shared memory)
-// and whose P has bf16 parts, 0 unless `some` -> (sum, m, l, move).  Out of line, because the loop over the full blocks must stay small: with
-// this beside it a tile took half as long again.
-__device__ __noinline__ float4 soften_open(uint32_t s_tm, int seen, float factor, uint32_t backs, float shift, float m, float l, bool some) {
+// and whose P has bf16 parts (16 bits), 0 unless `some` -> (sum, m, l, move).  Out of line, because the loop over the full
+// blocks must stay small: 1000 rows after 7000 keys took 218 us with this inside the masked step, 196 us beside it, 165 us so.
+__device__ __noinline__ float4 soften_open(uint32_t s_tm, int seen, float factor, uint32_t backs, float shift, float m, float l,
+                                           bool some) {
     uint32_t r[2][32];
     tmem_ld_32x32b_x32(s_tm, r[0]);
     tmem_ld_32x32b_x32(s_tm + 32u, r[1]);

@@ -278,8 +278,9 @@ int db_attention_decoder(const void *q16, const void *k16, const void *v16, int6
  * f32 [items, v_heads, 128, 128] (NULL: not kept; may be state_in itself when every item has its own, and otherwise
  * shares no memory with it).
  * An item without rows passes its state on.  States keep f32's accuracy within 2^-22 of the largest terms of their
- * value row (items longer than DB_DELTA_STEP_TOKENS multiply two f16 parts of every operand).  out [rows, v_heads, 128] in v's type.  workspace: device
- * bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0; it is 0 up to max_len =
+ * value row (items longer than DB_DELTA_STEP_TOKENS multiply two f16 parts of every operand; there a token
+ * whose value lies below 2^-20 of the largest of its feature in a block of 64 tokens keeps fewer bits).
+ * out [rows, v_heads, 128] in v's type.  workspace: device bytes from db_gated_delta_workspace_bytes (may be NULL where that is 0; it is 0 up to max_len =
  * DB_DELTA_STEP_TOKENS). */
 #define DB_DELTA_STEP_TOKENS 16
 size_t db_gated_delta_workspace_bytes(int64_t items, int64_t rows, int64_t max_len, int64_t k_heads, int64_t v_heads,
