@@ -174,6 +174,22 @@ def test_delta_one_short_key(db, T, size, short):
     check_delta(got, delta_ref(q, k, v, g, beta, [T], s, 128 ** -0.5, 1e-6), "f16")
 
 
+@pytest.mark.parametrize("dtype,large", [("bf16", 1.0), ("f16", 2.0 ** 12)])
+@pytest.mark.parametrize("T", [64, 150])
+def test_delta_small_values_before_large_ones(db, T, dtype, large):
+    """The first tokens' values are 2^-20 of the later ones', in every feature: their outputs are as accurate as alone."""
+    gen, Hk, Hv = _gen(53), 1, 2
+    q, k, v, g, beta = delta_inputs(gen, T, Hk, Hv, TYPES[dtype])
+    v = (v.float() * large).to(TYPES[dtype])
+    v[:40] = (v[:40].float() * 2.0 ** -20).to(TYPES[dtype])
+    out, _ = db.gated_delta(q, k, v, g, beta)
+    want, _ = delta_ref(q, k, v, g, beta, [T], None, 128 ** -0.5, 1e-6)
+    for part in (slice(0, 40), slice(40, T)):
+        err, rms = (out[part].double().cpu() - want[part]).abs(), want[part].square().mean().sqrt().item()
+        bound = 2 * EPS16[dtype] * (want[part].abs() + rms) + (2.0 ** -24 if dtype == "f16" else 0)
+        assert torch.all(err <= bound), float((err / bound).max())
+
+
 @pytest.mark.parametrize("T", [3, 70])
 def test_delta_states_side_by_side(db, T):
     """Initial and final states in one buffer, next to one another or the same, give what separate ones give."""
